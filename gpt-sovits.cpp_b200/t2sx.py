@@ -18,7 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libt2sx.so")
 
 OK, ERR_INVALID, ERR_IO, ERR_FORMAT, ERR_CUDA, ERR_OOM, ERR_STATE, ERR_BOUNDS, ERR_TIMEOUT = range(9)
-F32, F16, Q4_0, Q8_0, Q4_K = 0, 1, 2, 8, 12
+F32, F16, Q4_0, Q8_0, Q4_K, BF16 = 0, 1, 2, 8, 12, 30
 
 # Every symbol include/t2sx.h declares: (restype, argtypes).
 _P, _I, _I64, _F, _U32P = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.POINTER(C.c_uint32)
@@ -69,6 +69,21 @@ SIGNATURES = {
     "t2sx_kvcache_attn_decode": (C.c_int, [_P, _I, _P, _P, _P, _P, _P]),
     "t2sx_kvcache_attn_prefill": (C.c_int, [_P, _I, _P, _P, _P, _P, _P]),
     "t2sx_extract_latent": (C.c_int, [_P, _P, _I, _P]),
+    "t2sx_pool_create": (C.c_int, [_I, _I, _I, _I, _I, _I, _I, _P, _P, _P]),
+    "t2sx_pool_free": (None, [_P]),
+    "t2sx_pool_available": (C.c_int, [_P, _P]),
+    "t2sx_pool_length": (_I64, [_P, _I]),
+    "t2sx_pool_table": (C.c_int, [_P, _I, _P, _I, _P]),
+    "t2sx_pool_extend": (C.c_int, [_P, _I, _P, _P]),
+    "t2sx_pool_fork": (C.c_int, [_P, _I, _P, _P, _P]),
+    "t2sx_pool_copy": (C.c_int, [_P, _I, _P, _P, _P]),
+    "t2sx_pool_release": (C.c_int, [_P, _I, _P]),
+    "t2sx_pool_compact": (C.c_int, [_P, _P, _P]),
+    "t2sx_plan_create": (C.c_int, [_P, _I, _P]),
+    "t2sx_plan_free": (None, [_P]),
+    "t2sx_plan_update": (C.c_int, [_P, _I, _P, _P, _P]),
+    "t2sx_plan_attend": (C.c_int, [_P, _I, _P, _I64, _P, _P, _I64, _F, _P, _I64, _P, _P]),
+    "t2sx_token_logprobs": (C.c_int, [_I, _I, _I64, _I64, _P, _I64, _P, _I, _P, _P, _P, _P, _P, _P]),
 }
 NOALLOC_MAX_ELEMS = 1 << 21
 
@@ -421,3 +436,142 @@ class KVCache:
             self.close()
         except Exception:
             pass
+
+
+def _i32(a):
+    return np.ascontiguousarray(np.atleast_1d(a), dtype=np.int32)
+
+
+class PagePool:
+    """Pages of 64 positions of a K/V cache that sequences share.  The caller owns the storage, K and V
+    each [n_layers][n_pages][n_kv_heads][64][head_dim] of f16 or bf16 on the device, and keeps it alive."""
+
+    PAGE = 64
+
+    def __init__(self, dtype: int, n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, max_seqs: int,
+                 k_ptr: int, v_ptr: int, device: int = 0):
+        self.h = None
+        h = C.c_void_p()
+        _ck(lib().t2sx_pool_create(device, dtype, n_layers, n_pages, n_kv_heads, head_dim, max_seqs, k_ptr, v_ptr,
+                                   C.byref(h)))
+        self.h = h
+        self.dtype, self.n_layers, self.n_pages = dtype, n_layers, n_pages
+        self.n_kv_heads, self.head_dim, self.max_seqs = n_kv_heads, head_dim, max_seqs
+
+    def available(self) -> int:
+        """Pages that no sequence uses."""
+        n = C.c_int32(0)
+        _ck(lib().t2sx_pool_available(self.h, C.byref(n)))
+        return n.value
+
+    def length(self, seq: int) -> int:
+        n = lib().t2sx_pool_length(self.h, seq)
+        if n < 0:
+            _ck(ERR_INVALID)
+        return n
+
+    def table(self, seqs) -> np.ndarray:
+        """Page ids of the sequences, int32 [n][most pages of one], filled up with -1."""
+        seqs = _i32(seqs)
+        width = max((-(-self.length(int(s)) // self.PAGE) for s in seqs), default=0)
+        out = np.empty((seqs.size, width), dtype=np.int32)
+        _ck(lib().t2sx_pool_table(self.h, seqs.size, _p(seqs), width, _p(out)))
+        return out
+
+    def _pairs(self, fn, srcs, dsts, stream):
+        srcs, dsts = _i32(srcs), _i32(dsts)
+        if srcs.size != dsts.size:
+            raise ValueError("as many sources as destinations are needed")
+        _ck(fn(self.h, srcs.size, _p(srcs), _p(dsts), stream))
+
+    def extend(self, seqs, counts):
+        """counts[i] more positions for seqs[i]."""
+        seqs = _i32(seqs)
+        counts = np.ascontiguousarray(np.atleast_1d(counts), dtype=np.int64)
+        if seqs.size != counts.size:
+            raise ValueError("as many counts as sequences are needed")
+        _ck(lib().t2sx_pool_extend(self.h, seqs.size, _p(seqs), _p(counts)))
+
+    def fork(self, srcs, dsts, stream: int = 0):
+        """dsts[i] := a continuation of srcs[i] that shares its full pages."""
+        self._pairs(lib().t2sx_pool_fork, srcs, dsts, stream)
+
+    def copy(self, srcs, dsts, stream: int = 0):
+        """dsts[i] := srcs[i] on pages of its own."""
+        self._pairs(lib().t2sx_pool_copy, srcs, dsts, stream)
+
+    def release(self, seqs):
+        seqs = _i32(seqs)
+        _ck(lib().t2sx_pool_release(self.h, seqs.size, _p(seqs)))
+
+    def compact(self, stream: int = 0) -> int:
+        """Moves the pages in use to the lowest ids; how many moved."""
+        n = C.c_int32(0)
+        _ck(lib().t2sx_pool_compact(self.h, C.byref(n), stream))
+        return n.value
+
+    def plan(self, n_heads: int) -> "AttnPlan":
+        return AttnPlan(self, n_heads)
+
+    def close(self):
+        if self.h:
+            lib().t2sx_pool_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class AttnPlan:
+    """Attention of a step's tokens over a PagePool: update() once per step, attend() once per layer."""
+
+    def __init__(self, pool: PagePool, n_heads: int):
+        self.h = None
+        h = C.c_void_p()
+        _ck(lib().t2sx_plan_create(pool.h, n_heads, C.byref(h)))
+        self.h = h
+        self.pool, self.n_heads, self.rows = pool, n_heads, 0
+
+    def update(self, seqs, n_new, stream: int = 0):
+        """The step's sequences and how many of their last positions are rows of the step."""
+        seqs, n_new = _i32(seqs), _i32(n_new)
+        if seqs.size != n_new.size:
+            raise ValueError("as many row counts as sequences are needed")
+        _ck(lib().t2sx_plan_update(self.h, seqs.size, _p(seqs), _p(n_new), stream))
+        self.rows = int(n_new.sum())
+
+    def attend(self, layer: int, q_ptr: int, out_ptr: int, scale: float, k_new_ptr: int | None = None,
+               v_new_ptr: int | None = None, lse_ptr: int | None = None, q_stride: int | None = None,
+               kv_stride: int | None = None, out_stride: int | None = None, stream: int = 0):
+        """out[r] = softmax(scale * q[r] . K) . V over the positions that row r sees, after the rows' own
+        k_new, v_new (if given) have been written to the cache.  Strides in elements; default: dense rows."""
+        dim = self.pool.head_dim
+        row = self.n_heads * dim
+        _ck(lib().t2sx_plan_attend(self.h, layer, q_ptr, row if q_stride is None else q_stride, k_new_ptr, v_new_ptr,
+                                   self.pool.n_kv_heads * dim if kv_stride is None else kv_stride, scale, out_ptr,
+                                   row if out_stride is None else out_stride, lse_ptr, stream))
+
+    def close(self):
+        if self.h:
+            lib().t2sx_plan_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def token_logprobs(dtype: int, rows: int, vocab: int, logits_ptr: int, tokens_ptr: int, logprob_ptr: int,
+                   entropy_ptr: int | None = None, rank_ptr: int | None = None, top_k: int = 0,
+                   top_ids_ptr: int | None = None, top_logprobs_ptr: int | None = None, stride: int | None = None,
+                   device: int = 0, stream: int = 0):
+    """Log probability, entropy and rank of tokens[r] under row r of the logits, and the top_k (<= 32) best
+    tokens with theirs.  stride: elements between rows (default: dense)."""
+    _ck(lib().t2sx_token_logprobs(device, dtype, rows, vocab, logits_ptr, vocab if stride is None else stride,
+                                  tokens_ptr, top_k, logprob_ptr, entropy_ptr, rank_ptr, top_ids_ptr,
+                                  top_logprobs_ptr, stream))

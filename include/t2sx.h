@@ -247,6 +247,89 @@ T2SX_API int t2sx_kvcache_attn_decode(t2sx_kvcache* c, int32_t n, const int32_t*
 T2SX_API int t2sx_kvcache_attn_prefill(t2sx_kvcache* c, int32_t n, const int32_t* seqs, const int32_t* lens,
                                        const uint16_t* q_dev, float* out_dev, void* stream);
 
+/* ---- candidates of a prompt: cache pages that sequences share, attention over them, scores ----
+ * No counterpart in the reference (one cache slot per sequence, and a sampled token without its
+ * probability).  Drawing several candidates from one prompt takes three things: a cache whose
+ * sequences share the prompt's pages, an attention that reads shared pages once for all of
+ * them, and the log probability of the tokens drawn, to rank the candidates by. */
+#define T2SX_TYPE_F32 0
+#define T2SX_TYPE_F16 1
+#define T2SX_TYPE_BF16 30
+
+/* A pool of cache pages of 64 positions.  The caller owns the storage: k_dev and v_dev are each
+ * [n_layers][n_pages][n_kv_heads][64][head_dim] of f16 or bf16 (16-byte aligned; 128 or more is
+ * best), and outlive the pool.  Sequences are ids 0 .. max_seqs - 1, empty at first.  A sequence
+ * is a list of pages, position p in page p / 64.  A page of several sequences is always full:
+ * a fork copies the last, partly filled page, so no write ever reaches a shared page.
+ * Pages are taken lowest free id first; every call either takes full effect or none.
+ * head_dim: 32, 64 or 128.  n_pages at most 2^26.
+ * Threading: single-owner, as a session.  Streams: calls take effect in call order, whatever
+ * streams they are given; a call on another stream than the last one waits for the latter.  The
+ * caller orders its own accesses to the storage and to tensors.  Not for stream capture. */
+typedef struct t2sx_pool t2sx_pool;
+T2SX_API int t2sx_pool_create(int32_t device, int32_t type, int32_t n_layers, int32_t n_pages, int32_t n_kv_heads,
+                              int32_t head_dim, int32_t max_seqs, void* k_dev, void* v_dev, t2sx_pool** out);
+/* Waits for the pool's device work.  A pool freed while plans use it goes with its last plan. */
+T2SX_API void t2sx_pool_free(t2sx_pool* p);
+/* Pages that no sequence uses. */
+T2SX_API int t2sx_pool_available(t2sx_pool* p, int32_t* n_pages);
+/* Positions of a sequence; -1 for a bad argument. */
+T2SX_API int64_t t2sx_pool_length(t2sx_pool* p, int32_t seq);
+/* Page ids of n sequences: out [n][width], rows filled up with -1; width >= the longest's pages. */
+T2SX_API int t2sx_pool_table(t2sx_pool* p, int32_t n, const int32_t* seqs, int32_t width, int32_t* out);
+/* counts[i] (>= 0) positions more for sequence seqs[i] (distinct), in order; their values are
+ * undefined until written.  T2SX_ERR_OOM if the pool has not enough pages. */
+T2SX_API int t2sx_pool_extend(t2sx_pool* p, int32_t n, const int32_t* seqs, const int64_t* counts);
+/* dsts[i] (empty, distinct; T2SX_ERR_STATE otherwise) becomes a continuation of srcs[i]: it
+ * shares the full pages and gets its own copy of the filled positions of a partial last one. */
+T2SX_API int t2sx_pool_fork(t2sx_pool* p, int32_t n, const int32_t* srcs, const int32_t* dsts, void* stream);
+/* As fork, but sharing nothing: dsts[i] gets pages of its own for all positions. */
+T2SX_API int t2sx_pool_copy(t2sx_pool* p, int32_t n, const int32_t* srcs, const int32_t* dsts, void* stream);
+/* Empties n sequences (distinct; an empty one stays so).  Pages that no other one uses are free. */
+T2SX_API int t2sx_pool_release(t2sx_pool* p, int32_t n, const int32_t* seqs);
+/* Moves the pages in use down to ids 0 .. in use - 1: the i-th page above that line goes to the
+ * i-th free id below it.  *moved (may be null) = pages moved. */
+T2SX_API int t2sx_pool_compact(t2sx_pool* p, int32_t* moved, void* stream);
+
+/* Attention of one step's tokens over a pool.  A plan holds what all layers of a step share: which
+ * token sees what, which pages several sequences read, and the workspace.  n_heads query heads, a
+ * multiple of n_kv_heads; query head h reads K/V head h / (n_heads / n_kv_heads). */
+typedef struct t2sx_plan t2sx_plan;
+T2SX_API int t2sx_plan_create(t2sx_pool* p, int32_t n_heads, t2sx_plan** out);
+T2SX_API void t2sx_plan_free(t2sx_plan* a);
+/* The step's sequences (distinct) and their last n_new[i] (>= 0, <= length) positions: rows are
+ * these positions in the order of the call.  Pages that sequences have in common from their
+ * start on are found here, whatever the order.  The pool's later fork, copy and extend calls
+ * leave a plan valid; after a release or a compact that moved pages attend gives T2SX_ERR_STATE
+ * until the next update. */
+T2SX_API int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, const int32_t* n_new, void* stream);
+/* Row r with query head h, at position lim - 1 of its sequence:
+ *     out = sum_{j < lim} softmax_j(scale * q . k_j) v_j,   lse = log sum_{j < lim} exp(scale * q . k_j)
+ * q_dev, out_dev: [rows][n_heads][head_dim] of the pool's type, rows q_stride / out_stride
+ * elements apart (multiples of 8); lse_dev: f32 [rows][n_heads] or null.  With k_new_dev and
+ * v_new_dev ([rows][n_kv_heads][head_dim], rows kv_stride elements apart) the rows' keys and
+ * values are first written to the cache; null: they are there already.  All 16-byte aligned.
+ * Cache positions below a sequence's length must hold finite values; beyond it anything may stand.
+ * Products are accumulated, and maxima and sums held, in f32; the softmax weights are rounded to
+ * the pool's type before they multiply v, as the tensor cores take them. */
+T2SX_API int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, int64_t q_stride, const void* k_new_dev,
+                              const void* v_new_dev, int64_t kv_stride, float scale, void* out_dev, int64_t out_stride,
+                              float* lse_dev, void* stream);
+
+/* Scores of given tokens under rows of logits (f32, f16 or bf16; stride elements apart):
+ * logprob [rows]: log softmax of the row at tokens[r]; entropy [rows] (nats); rank [rows]: how many
+ * tokens come before it in descending order, ties to the lower id; top_ids, top_logprobs
+ * [rows][top_k]: the first top_k (0 .. 32) tokens of that order.  entropy, rank, and with top_k = 0
+ * the top lists may be null.  -inf is a masked token: probability 0, never listed; lists that
+ * run out of tokens are filled up with -1 and -inf.  A row of -inf only: logprob -inf, entropy 0.
+ * A row with NaN or +inf: logprob, entropy and top_logprobs NaN; NaN is not listed.  Token -1 (none,
+ * padding): logprob 0, rank -1; any other id outside [0, vocab): logprob NaN, rank -1.
+ * The sums are f32, the result is the same for the same row wherever it stands in a call. */
+T2SX_API int t2sx_token_logprobs(int32_t device, int32_t type, int64_t rows, int64_t vocab, const void* logits_dev,
+                                 int64_t stride, const int32_t* tokens_dev, int32_t top_k, float* logprob_dev,
+                                 float* entropy_dev, int32_t* rank_dev, int32_t* top_ids_dev, float* top_logprobs_dev,
+                                 void* stream);
+
 #ifdef __cplusplus
 }
 #endif

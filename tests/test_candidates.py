@@ -1,0 +1,518 @@
+"""Shared cache pages, attention over them and token log probabilities, against plain 64-bit forms.
+
+Tolerances (u = half a unit in the last place of the 16-bit type: 2^-11 for f16, 2^-8 for bf16):
+attention: with a = sum_j p_j |v_j|, rounding the softmax weights moves an output by at most u a and rounding
+the output by u |out|; a score of up to 128 products accumulated in f32, its exponential, and sums
+of up to 2^17 terms in f32 parts leave less than 2^-14 a.  Absolute log-sum-exp error: 2^-14 likewise.
+Log probabilities: sums of f32 terms in blocks, 2^-17 of the values' scale (the largest |x - max|, at
+least 1).  Ids, ranks, tables and moved values are equal."""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+gpu = pytest.mark.gpu
+PAGE = 64
+TORCH = {1: torch.float16, 30: torch.bfloat16, 0: torch.float32}
+UNIT = {1: 2.0 ** -11, 30: 2.0 ** -8}
+
+
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.fail("CUDA device required for -m gpu tests")
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _store(dtype, layers, pages, kv, dim, fill=float("nan")):
+    shape = (layers, pages, kv, PAGE, dim)
+    return [torch.full(shape, fill, dtype=TORCH[dtype], device="cuda") for _ in range(2)]
+
+
+class Cache:
+    """A pool, its storage, and for each sequence what its positions must hold ([layers][len][kv][dim], K and V)."""
+
+    def __init__(self, t2sx, dtype, layers, pages, kv, dim, seqs, seed=0):
+        self.k, self.v = _store(dtype, layers, pages, kv, dim)
+        self.pool = t2sx.PagePool(dtype, layers, pages, kv, dim, seqs, self.k.data_ptr(), self.v.data_ptr())
+        self.gen = torch.Generator(device="cuda").manual_seed(seed)
+        self.want = {s: [torch.empty((layers, 0, kv, dim), dtype=TORCH[dtype], device="cuda")] * 2 for s in range(seqs)}
+
+    def at(self, seq):
+        pages = torch.as_tensor(self.pool.table([seq])[0], device="cuda").long()
+        n = self.pool.length(seq)
+        return [x[:, pages].movedim(2, 3).flatten(1, 2)[:, :n] for x in (self.k, self.v)]
+
+    def extend(self, seq, count, write=True):
+        had = self.pool.length(seq)
+        self.pool.extend([seq], [count])
+        table = torch.as_tensor(self.pool.table([seq])[0], device="cuda").long()
+        pos = torch.arange(had, had + count, device="cuda")
+        for i, x in enumerate((self.k, self.v)):
+            rows = torch.randn((x.shape[0], count, x.shape[2], x.shape[4]), generator=self.gen, device="cuda").to(x.dtype)
+            if write and count:
+                x[:, table[pos // PAGE], :, pos % PAGE] = rows.movedim(1, 0)
+            self.want[seq] = self.want[seq][:i] + [torch.cat([self.want[seq][i], rows], 1)] + self.want[seq][i + 1:]
+
+    def derive(self, op, srcs, dsts):
+        getattr(self.pool, op)(srcs, dsts, _stream())
+        for a, b in zip(srcs, dsts):
+            self.want[b] = list(self.want[a])
+
+    def release(self, seqs):
+        self.pool.release(seqs)
+        for s in seqs:
+            self.want[s] = [x[:, :0] for x in self.want[s]]
+
+    def check(self):
+        users = {}
+        for s, want in self.want.items():
+            assert self.pool.length(s) == want[0].shape[1]
+            for got, x in zip(self.at(s), want):
+                assert torch.equal(got.view(torch.int16), x.contiguous().view(torch.int16)), s
+            for j, page in enumerate(self.pool.table([s])[0]):
+                users.setdefault(int(page), set()).add((s, j))
+        assert self.pool.available() == self.pool.n_pages - len(users)
+        for held in users.values():   # shared pages are full in each of their sequences
+            if len(held) > 1:
+                assert all((j + 1) * PAGE <= self.pool.length(s) for s, j in held)
+        return set(users)
+
+
+# ---- pages ---------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dtype,layers,kv,dim", [(1, 3, 2, 32), (30, 1, 1, 128), (1, 2, 5, 64)])
+def test_pool_random_life(t2sx_mod, dtype, layers, kv, dim):
+    """Random extend, fork, copy, release and compact calls against the values that sequences must hold."""
+    _need_gpu()
+    rng = np.random.default_rng(dim + layers)
+    c = Cache(t2sx_mod, dtype, layers, 120, kv, dim, 12)
+    for step in range(160):
+        live = [s for s in c.want if c.pool.length(s)]
+        free = [s for s in c.want if not c.pool.length(s)]
+        op = rng.choice(["extend", "fork", "copy", "release", "compact"], p=[0.35, 0.25, 0.1, 0.2, 0.1])
+        try:
+            if op == "extend":
+                c.extend(int(rng.choice(12)), int(rng.choice([0, 1, 5, 63, 64, 65, 200])))
+            elif op in ("fork", "copy") and live and free:
+                n = int(rng.integers(1, len(free) + 1))
+                c.derive(op, rng.choice(live, n).tolist(), rng.choice(free, n, replace=False).tolist())
+            elif op == "release" and live:
+                c.release(rng.choice(live, int(rng.integers(1, len(live) + 1)), replace=False).tolist())
+            elif op == "compact":
+                before = c.check()
+                moved = c.pool.compact(_stream())
+                assert moved == sum(p >= len(before) for p in before)
+                assert c.check() == set(range(len(before)))
+        except t2sx_mod.T2SXError as e:
+            assert e.code == t2sx_mod.ERR_OOM
+        c.check()
+
+
+@gpu
+def test_pool_lowest_free_page_first(t2sx_mod):
+    _need_gpu()
+    c = Cache(t2sx_mod, 1, 1, 70, 1, 32, 6)
+    c.pool.extend([0, 1, 2], [130, 1, 64])
+    assert c.pool.table([0, 1, 2]).tolist() == [[0, 1, 2], [3, -1, -1], [4, -1, -1]]
+    c.pool.fork([0], [3], _stream())
+    assert c.pool.table([3]).tolist() == [[0, 1, 5]]
+    c.pool.release([0, 1])
+    c.pool.extend([4], [66 * PAGE])   # 64 pages are free above, and 2 and 3
+    assert c.pool.table([4])[0].tolist() == [2, 3] + list(range(6, 70))
+    assert c.pool.available() == 0
+    with pytest.raises(t2sx_mod.T2SXError) as e:
+        c.pool.extend([1], [1])
+    assert e.value.code == t2sx_mod.ERR_OOM and c.pool.length(1) == 0
+
+
+@gpu
+def test_pool_many_moves(t2sx_mod):
+    """More page copies than one launch's list holds."""
+    _need_gpu()
+    n = 700
+    c = Cache(t2sx_mod, 1, 1, n + 2, 1, 32, n + 1)
+    c.extend(0, 70)
+    c.derive("fork", [0] * n, list(range(1, n + 1)))
+    c.check()
+    c.release(list(range(0, n, 2)))
+    assert c.pool.compact(_stream()) > 0
+    c.check()
+
+
+@gpu
+def test_pool_refusals(t2sx_mod):
+    _need_gpu()
+    k, v = _store(1, 1, 8, 1, 32)
+    make = lambda **kw: t2sx_mod.PagePool(*[{**dict(dtype=1, layers=1, pages=8, kv=1, dim=32, seqs=4, k=k.data_ptr(), v=v.data_ptr()), **kw}[n]
+                                            for n in ("dtype", "layers", "pages", "kv", "dim", "seqs", "k", "v")])
+    for kw in (dict(dtype=0), dict(layers=0), dict(pages=0), dict(kv=0), dict(dim=48), dict(seqs=0), dict(k=0),
+               dict(k=k.data_ptr() + 2), dict(pages=(1 << 26) + 1)):
+        with pytest.raises(t2sx_mod.T2SXError) as e:
+            make(**kw)
+        assert e.value.code == t2sx_mod.ERR_INVALID, kw
+    pool = make()
+    pool.extend([0], [65])
+    for call, code in ((lambda: pool.fork([0], [0]), t2sx_mod.ERR_STATE), (lambda: pool.fork([0, 0], [1, 1]), t2sx_mod.ERR_INVALID),
+                       (lambda: pool.fork([4], [1]), t2sx_mod.ERR_INVALID), (lambda: pool.copy([0], [-1]), t2sx_mod.ERR_INVALID),
+                       (lambda: pool.extend([1, 1], [1, 1]), t2sx_mod.ERR_INVALID), (lambda: pool.extend([1], [-1]), t2sx_mod.ERR_INVALID),
+                       (lambda: pool.extend([1], [1 << 40]), t2sx_mod.ERR_INVALID), (lambda: pool.release([9]), t2sx_mod.ERR_INVALID),
+                       (lambda: pool.length(4), t2sx_mod.ERR_INVALID), (lambda: pool.plan(0), t2sx_mod.ERR_INVALID),
+                       (lambda: pool.copy([0, 0, 0, 0], [1, 2, 3, 3]), t2sx_mod.ERR_INVALID),
+                       (lambda: pool.extend([1], [7 * 64]), t2sx_mod.ERR_OOM)):
+        with pytest.raises(t2sx_mod.T2SXError) as e:
+            call()
+        assert e.value.code == code
+    assert pool.available() == 6 and pool.length(0) == 65
+    plan = pool.plan(3)
+    for seqs, new in (([0], [66]), ([0, 0], [1, 1]), ([7], [1]), ([0], [-1]), ([1], [1])):
+        with pytest.raises(t2sx_mod.T2SXError) as e:
+            plan.update(seqs, new)
+        assert e.value.code == t2sx_mod.ERR_INVALID
+    x = torch.zeros((1, 3, 32), dtype=torch.float16, device="cuda")
+    with pytest.raises(t2sx_mod.T2SXError) as e:
+        plan.attend(0, x.data_ptr(), x.data_ptr(), 1.0)
+    assert e.value.code == t2sx_mod.ERR_STATE
+    plan.update([0], [1], _stream())
+    for kw in (dict(layer=1), dict(layer=-1), dict(q_ptr=None), dict(q_ptr=x.data_ptr() + 2), dict(q_stride=88), dict(q_stride=100),
+               dict(k_new_ptr=x.data_ptr()), dict(scale=float("nan")), dict(out_ptr=None), dict(lse_ptr=x.data_ptr() + 2)):
+        with pytest.raises(t2sx_mod.T2SXError) as e:
+            plan.attend(**{**dict(layer=0, q_ptr=x.data_ptr(), out_ptr=x.data_ptr(), scale=1.0), **kw})
+        assert e.value.code == t2sx_mod.ERR_INVALID, kw
+    pool.extend([1], [1])
+    pool.release([1])
+    with pytest.raises(t2sx_mod.T2SXError) as e:
+        plan.attend(0, x.data_ptr(), x.data_ptr(), 1.0)
+    assert e.value.code == t2sx_mod.ERR_STATE
+    with pytest.raises(t2sx_mod.T2SXError):
+        pool.plan(1 << 20)
+    torch.cuda.synchronize()
+
+
+def test_refusals_without_device(t2sx_mod):
+    """Arguments are checked before any device work."""
+    import ctypes as C
+    L, h, one = t2sx_mod.lib(), C.c_void_p(), 4096
+    assert L.t2sx_pool_create(0, 2, 1, 1, 1, 32, 1, one, one, C.byref(h)) == t2sx_mod.ERR_INVALID and not h.value
+    assert b"f16 or bf16" in L.t2sx_last_error()
+    assert L.t2sx_pool_create(0, 1, 1, 1, 1, 32, 1, one, one, None) == t2sx_mod.ERR_INVALID
+    assert L.t2sx_plan_create(None, 1, C.byref(h)) == t2sx_mod.ERR_INVALID
+    assert L.t2sx_pool_fork(None, 0, None, None, None) == t2sx_mod.ERR_INVALID
+    assert L.t2sx_pool_length(None, 0) == -1
+    assert L.t2sx_plan_attend(None, 0, one, 32, None, None, 0, 1.0, one, 32, None, None) == t2sx_mod.ERR_INVALID
+    L.t2sx_pool_free(None)
+    L.t2sx_plan_free(None)
+    bad = lambda **kw: L.t2sx_token_logprobs(*{**dict(dev=0, type=0, rows=1, vocab=8, x=one, stride=8, t=one, k=2, lp=one, h=None, r=None,
+                                                      ids=one, top=one, st=None), **kw}.values())
+    for kw in (dict(type=2), dict(rows=-1), dict(vocab=0), dict(stride=7), dict(k=33), dict(k=-1), dict(x=None), dict(t=None), dict(lp=None),
+               dict(ids=None), dict(top=None), dict(x=one + 2), dict(type=1, x=one + 1), dict(h=one + 2)):
+        assert bad(**kw) == t2sx_mod.ERR_INVALID, kw
+    assert bad(rows=0) == t2sx_mod.OK
+
+
+# ---- attention -----------------------------------------------------------------------------------------
+
+def _reference(c, layer, seqs, n_new, q, heads, scale):
+    """out, sum p |v| and log-sum-exp in 64 bits, from what the sequences must hold."""
+    kv = c.k.shape[2]
+    out, mag, lse, at = [], [], [], 0
+    for s, n in zip(seqs, n_new):
+        k, v = (x[layer].double().repeat_interleave(heads // kv, 1) for x in c.want[s])
+        a = torch.einsum("nhd,lhd->hnl", q[at:at + n].double(), k) * scale
+        length = k.shape[0]
+        pos = torch.arange(length, device="cuda")[None] > torch.arange(length - n, length, device="cuda")[:, None]
+        a = a.masked_fill(pos[None], float("-inf"))
+        z = a.logsumexp(-1, keepdim=True)
+        p = (a - z).exp()
+        out.append(torch.einsum("hnl,lhd->nhd", p, v))
+        mag.append(torch.einsum("hnl,lhd->nhd", p, v.abs()))
+        lse.append(z[..., 0].T)
+        at += n
+    return torch.cat(out), torch.cat(mag), torch.cat(lse)
+
+
+def _attend(c, dtype, layer, seqs, n_new, heads, scale=None, q_scale=1.5, write=False, pad=0, seed=1):
+    """attend() against the reference; write: the rows' keys and values are passed to the call."""
+    kv, dim = c.k.shape[2], c.k.shape[4]
+    scale = 1.0 / math.sqrt(dim) if scale is None else scale
+    rows = sum(n_new)
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    row = heads * dim + pad
+    q = (torch.randn((rows, row), generator=gen, device="cuda") * q_scale).to(TORCH[dtype])
+    out = torch.full((rows, row), 7.0, dtype=TORCH[dtype], device="cuda")
+    lse = torch.full((rows, heads), 7.0, device="cuda")
+    kn = vn = None
+    if write:
+        kn, vn = (torch.cat([c.want[s][i][layer, c.want[s][i].shape[1] - n:] for s, n in zip(seqs, n_new)]) for i in (0, 1))
+        kn, vn = (torch.nn.functional.pad(x.flatten(1), (0, 8)).contiguous() for x in (kn, vn))
+    plan = c.pool.plan(heads)
+    plan.update(seqs, n_new, _stream())
+    assert plan.rows == rows
+    call = lambda: plan.attend(layer, q.data_ptr(), out.data_ptr(), scale, lse_ptr=lse.data_ptr(), q_stride=row, out_stride=row,
+                               k_new_ptr=kn.data_ptr() if write else None, v_new_ptr=vn.data_ptr() if write else None,
+                               kv_stride=kv * dim + 8, stream=_stream())
+    call()
+    first = out.clone()
+    call()   # the same plan again: the same bits
+    assert torch.equal(first.view(torch.int16), out.view(torch.int16))
+    ref, mag, zref = _reference(c, layer, seqs, n_new, q[:, :heads * dim].unflatten(1, (heads, dim)), heads, scale)
+    assert (out[:, heads * dim:] == 7.0).all()
+    got = out[:, :heads * dim].unflatten(1, (heads, dim)).double()
+    u = UNIT[dtype]
+    err = (got - ref).abs() - (u * (mag + ref.abs()) + 2.0 ** -14 * mag + 2.0 ** -24)
+    assert torch.isfinite(got).all() and (err <= 0).all(), (float((got - ref).abs().max()), int((err > 0).sum()))
+    assert ((lse.double() - zref).abs() <= 2.0 ** -14 * (1 + zref.abs())).all()
+    plan.close()
+
+
+SHAPES = [(1, 16, 16, 32), (30, 8, 2, 64), (30, 8, 1, 128), (1, 14, 2, 128), (1, 6, 3, 32), (30, 20, 1, 64)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype,heads,kv,dim", SHAPES)
+@pytest.mark.parametrize("length", [1, 2, 63, 64, 65, 127, 128, 129, 700])
+def test_attend_lengths(t2sx_mod, dtype, heads, kv, dim, length):
+    """One token, alone, at lengths around the page; what stands beyond the length is NaN."""
+    _need_gpu()
+    c = Cache(t2sx_mod, dtype, 2, 40, kv, dim, 3)
+    c.extend(0, 3)
+    c.extend(1, length)
+    _attend(c, dtype, 1, [1], [1], heads)
+    _attend(c, dtype, 0, [1, 0], [1, 1], heads, write=True)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,heads,kv,dim", SHAPES)
+@pytest.mark.parametrize("prompt,each", [(350, 5), (64, 3), (63, 20), (1000, 40), (130, 150)])
+def test_attend_forked(t2sx_mod, dtype, heads, kv, dim, prompt, each):
+    """Candidates of two prompts, ragged, in a shuffled order, one of them still of the prompt's length."""
+    _need_gpu()
+    rng = np.random.default_rng(prompt + each)
+    c = Cache(t2sx_mod, dtype, 1, 2 * (prompt // PAGE + 1) + 8 * each, kv, dim, 2 + 2 * each)
+    c.extend(0, prompt)
+    c.extend(1, max(1, prompt - 40))
+    cand = list(range(2, 2 + 2 * each))
+    c.derive("fork", [i % 2 for i in cand], cand)
+    for s in cand[1:]:
+        c.extend(s, int(rng.integers(1, 200)))
+    rng.shuffle(cand)
+    _attend(c, dtype, 0, cand, [1] * len(cand), heads, write=True, pad=8)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,heads,kv,dim", SHAPES)
+def test_attend_forks_of_forks(t2sx_mod, dtype, heads, kv, dim):
+    """Three generations; sequences of no rows, a prompt beside its candidates, chunks of several rows."""
+    _need_gpu()
+    rng = np.random.default_rng(dim)
+    c = Cache(t2sx_mod, dtype, 1, 260, kv, dim, 40)
+    c.extend(0, 200)
+    c.derive("fork", [0] * 3, [1, 2, 3])
+    for s in (1, 2, 3):
+        c.extend(s, int(rng.integers(60, 200)))
+    c.derive("fork", [1] * 4 + [2] * 4, list(range(4, 12)))
+    for s in range(4, 12):
+        c.extend(s, int(rng.integers(1, 130)))
+    c.derive("fork", [5] * 12, list(range(12, 24)))
+    for s in range(12, 24):
+        c.extend(s, int(rng.integers(0, 70)))
+    c.extend(30, 77)
+    seqs = rng.permutation(list(range(24)) + [30]).tolist()
+    new = [int(rng.choice([0, 1, 1, 2, 9])) for _ in seqs]
+    new[0] = 1
+    _attend(c, dtype, 0, seqs, new, heads)
+    _attend(c, dtype, 0, seqs, new, heads, write=True)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,heads,kv,dim", SHAPES)
+@pytest.mark.parametrize("cached,new", [(0, 1), (0, 2), (0, 64), (0, 65), (37, 130), (300, 200), (63, 129), (1, 517)])
+def test_attend_chunk(t2sx_mod, dtype, heads, kv, dim, cached, new):
+    """Rows of a prompt over what is cached, causal, two ragged prompts in a call."""
+    _need_gpu()
+    c = Cache(t2sx_mod, dtype, 1, 40, kv, dim, 3)
+    c.extend(0, cached + new, write=False)
+    c.extend(1, 5, write=False)
+    for s in (0, 1):   # the rows come with the call; only what is cached is there before
+        t = torch.as_tensor(c.pool.table([s])[0], device="cuda").long()
+        pos = torch.arange(cached if s == 0 else 2, device="cuda")
+        for i, x in enumerate((c.k, c.v)):
+            x[:, t[pos // PAGE], :, pos % PAGE] = c.want[s][i][:, :len(pos)].movedim(1, 0)
+    _attend(c, dtype, 0, [0, 1], [new, 3], heads, write=True)
+    c.check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,heads,kv,dim", SHAPES)
+def test_attend_long_and_peaked(t2sx_mod, dtype, heads, kv, dim):
+    """A long axis with few rows; scores of several hundreds, rising and falling along it; a zero scale."""
+    _need_gpu()
+    c = Cache(t2sx_mod, dtype, 1, 330, kv, dim, 4)
+    c.extend(0, 20000)
+    c.derive("fork", [0, 0], [1, 2])
+    c.extend(1, 70)
+    _attend(c, dtype, 0, [0], [1], heads)
+    _attend(c, dtype, 0, [0, 1, 2], [1, 3, 1], heads)
+    _attend(c, dtype, 0, [0, 1, 2], [1, 3, 1], heads, scale=0.0)
+    # keys that grow along the sequence: the running maximum keeps changing
+    x = c.want[0][0]
+    x.mul_(torch.linspace(0.0, 12.0, x.shape[1], device="cuda", dtype=x.dtype)[None, :, None, None])
+    t = torch.as_tensor(c.pool.table([0])[0], device="cuda").long()
+    pos = torch.arange(c.pool.length(0), device="cuda")
+    c.k[:, t[pos // PAGE], :, pos % PAGE] = x.movedim(1, 0)
+    # the bound of 2^-14 on what scores leave holds for scores up to about 2^6: the scale keeps them there
+    _attend(c, dtype, 0, [0], [1], heads, scale=0.25 / math.sqrt(dim))
+
+
+@gpu
+def test_attend_other_stream(t2sx_mod):
+    """Calls on two streams in turn take effect in the order of the calls."""
+    _need_gpu()
+    c = Cache(t2sx_mod, 1, 1, 3000, 4, 64, 60)
+    c.extend(0, 3000)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in range(1, 40):
+        with torch.cuda.stream(streams[s % 2]):
+            c.derive("copy", [s - 1], [s])   # each reads what the other stream's call wrote
+    torch.cuda.synchronize()
+    c.check()
+    with torch.cuda.stream(streams[0]):
+        c.derive("fork", [39], [50])
+        c.release(list(range(39)))
+        with torch.cuda.stream(streams[1]):
+            c.pool.compact(_stream())
+        _attend(c, 1, 0, [39, 50], [2, 2], 8)
+    torch.cuda.synchronize()
+    c.check()
+
+
+@gpu
+def test_plan_outlives_pool_and_updates_grow(t2sx_mod):
+    _need_gpu()
+    c = Cache(t2sx_mod, 1, 1, 400, 2, 32, 200)
+    plan = c.pool.plan(4)
+    q = torch.randn((400, 4, 32), device="cuda").half()
+    out = torch.empty_like(q)
+    plan.update([], [], _stream())
+    plan.attend(0, q.data_ptr(), out.data_ptr(), 0.2, stream=_stream())
+    for n in (1, 30, 180, 7):
+        for s in range(n):
+            c.extend(s, 1 + s % 3)
+        plan.update(list(range(n)), [1] * n, _stream())
+        plan.attend(0, q.data_ptr(), out.data_ptr(), 0.2, stream=_stream())
+        ref, mag, _ = _reference(c, 0, list(range(n)), [1] * n, q[:n], 4, 0.2)
+        assert ((out[:n].double() - ref).abs() <= 2.0 ** -11 * (mag + ref.abs()) + 2.0 ** -14 * mag + 2.0 ** -24).all()
+    c.pool.close()
+    with pytest.raises(t2sx_mod.T2SXError):
+        plan.attend(0, q.data_ptr(), out.data_ptr(), 0.2, stream=_stream())
+    plan.close()
+
+
+# ---- log probabilities -----------------------------------------------------------------------------------
+
+def _scores(t2sx, x, tokens, top, stream=None):
+    rows, vocab = x.shape
+    dtype = {torch.float32: t2sx.F32, torch.float16: t2sx.F16, torch.bfloat16: t2sx.BF16}[x.dtype]
+    lp, h = (torch.full((rows,), 7.0, device="cuda") for _ in range(2))
+    rank = torch.full((rows,), 7, dtype=torch.int32, device="cuda")
+    ids = torch.full((rows, top), 7, dtype=torch.int32, device="cuda")
+    tl = torch.full((rows, top), 7.0, device="cuda")
+    t2sx.token_logprobs(dtype, rows, vocab, x.data_ptr(), tokens.data_ptr(), lp.data_ptr(), h.data_ptr(), rank.data_ptr(), top,
+                        ids.data_ptr() if top else None, tl.data_ptr() if top else None, stride=x.stride(0), stream=_stream())
+    return lp, h, rank, ids, tl
+
+
+def _check_scores(t2sx, x, tokens, top):
+    got = [a.cpu() for a in _scores(t2sx, x, tokens, top)]
+    x, tokens = x.double().cpu(), tokens.cpu().long()
+    lp, h, rank, ids, tl = got
+    ref = x.log_softmax(-1)
+    span = (x.amax(-1, keepdim=True) - x).masked_fill(x == float("-inf"), 0).amax(-1).clamp(min=1)
+    tol = 2.0 ** -17 * span
+    want = ref.gather(1, tokens[:, None])[:, 0]
+    same = (lp.double() == want) | ((lp.double() - want).abs() <= tol)
+    assert same.all(), (lp.double() - want).abs().max()
+    href = -torch.special.xlogy(ref.exp(), ref.exp()).sum(-1)
+    assert ((h.double() - href).abs() <= tol).all(), (h.double() - href).abs().max()
+    xt = x.gather(1, tokens[:, None])
+    before = (x > xt) | ((x == xt) & (torch.arange(x.shape[1])[None] < tokens[:, None]))
+    assert torch.equal(rank.long(), before.sum(-1))
+    order = torch.sort(x, dim=1, descending=True, stable=True)
+    k = min(top, x.shape[1])
+    listed = order.values[:, :k] > float("-inf")
+    assert torch.equal(ids[:, :k].long(), torch.where(listed, order.indices[:, :k], -1))
+    assert (ids[:, k:] == -1).all() and (tl[:, k:] == float("-inf")).all()
+    tref = ref.gather(1, order.indices[:, :k])
+    assert ((tl[:, :k].double() == tref) | ((tl[:, :k].double() - tref).abs() <= tol[:, None])).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [0, 1, 30])
+@pytest.mark.parametrize("rows,vocab,top,pad", [(1, 1, 1, 0), (3, 2, 5, 0), (1, 31, 32, 1), (5, 33, 0, 3), (8, 1025, 5, 0), (2, 1025, 32, 7),
+                                                (257, 1024, 15, 0), (1, 4097, 20, 0), (2, 70001, 20, 0), (300, 70001, 20, 1),
+                                                (40, 131072, 32, 0), (1, 140001, 1, 0), (3000, 200, 3, 5)])
+def test_logprobs(t2sx_mod, dtype, rows, vocab, top, pad):
+    """Sizes from one token to wide, strided rows, masked tokens (the given one among them), many ties in 16 bits."""
+    _need_gpu()
+    gen = torch.Generator(device="cuda").manual_seed(rows + vocab)
+    x = (torch.randn((rows, vocab + pad), generator=gen, device="cuda") * 2.5).to(TORCH[dtype])
+    x[:, vocab:] = float("nan")
+    x = x[:, :vocab]
+    tokens = torch.randint(0, vocab, (rows,), generator=gen, device="cuda", dtype=torch.int32)
+    if vocab > 2:
+        x[:, torch.randint(0, vocab, (vocab // 5,), generator=gen, device="cuda")] = float("-inf")
+        x[::3, 1:][x[::3, 1:] > 3.0] = float("-inf")
+        x[:, 0] = 1.0   # one token at least is open
+    _check_scores(t2sx_mod, x, tokens, top)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [0, 1, 30])
+@pytest.mark.parametrize("vocab", [700, 50000])
+def test_logprobs_orders(t2sx_mod, dtype, vocab):
+    """Rows that rise, fall, are all equal, have one open token, or few distinct values: every list is hard somewhere."""
+    _need_gpu()
+    j = torch.arange(vocab, device="cuda", dtype=torch.float32)
+    rows = [j / vocab * 9, -j / vocab * 9, torch.zeros_like(j), torch.where(j == vocab - 3, 2.0, float("-inf")), (j * 7919 % 5) - 2,
+            torch.where(j % 1000 == 999, 5.0, 0.0), torch.where(j >= vocab - 40, j / vocab, -3.0), -1e4 + j % 3, (j % 2) * -0.0]
+    x = torch.stack(rows).to(TORCH[dtype])
+    tokens = torch.tensor([0, vocab - 1, vocab // 2, vocab - 3, 4, 5, vocab - 40, 2, 3], device="cuda", dtype=torch.int32)
+    _check_scores(t2sx_mod, x, tokens, 32)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [0, 1, 30])
+@pytest.mark.parametrize("rows,vocab", [(8, 300), (8, 90001), (600, 1025)])
+def test_logprobs_empty_rows_and_padding(t2sx_mod, dtype, rows, vocab):
+    _need_gpu()
+    inf, nan = float("inf"), float("nan")
+    x = torch.randn((rows, vocab), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(TORCH[dtype])
+    x[0] = -inf
+    x[1, vocab // 2] = nan
+    x[2, vocab - 1] = inf
+    tokens = torch.full((rows,), 5, dtype=torch.int32, device="cuda")
+    tokens[3], tokens[4], tokens[5] = -1, vocab, -7
+    lp, h, rank, ids, tl = (a.cpu() for a in _scores(t2sx_mod, x, tokens, 4))
+    assert lp[0] == -inf and h[0] == 0 and rank[0] == 5 and (ids[0] == -1).all() and (tl[0] == -inf).all()
+    for r in (1, 2):
+        assert lp[r].isnan() and h[r].isnan() and tl[r].isnan().all()
+    assert ids[2, 0] == vocab - 1 and vocab // 2 not in ids[1].tolist()
+    assert torch.equal(ids[1, :4].long(), torch.sort(x[1].nan_to_num(nan=-inf).double().cpu(), descending=True, stable=True).indices[:4])
+    assert lp[3] == 0 and rank[3] == -1 and h[3].isfinite()
+    assert lp[4].isnan() and lp[5].isnan() and rank[4] == rank[5] == -1
+    assert torch.isfinite(lp[6:]).all() and (ids[3:] >= 0).all()
+
+
+@gpu
+def test_logprobs_optional_outputs(t2sx_mod):
+    _need_gpu()
+    x = torch.randn((4, 50), device="cuda")
+    t = torch.zeros(4, dtype=torch.int32, device="cuda")
+    lp = torch.empty(4, device="cuda")
+    t2sx_mod.token_logprobs(0, 4, 50, x.data_ptr(), t.data_ptr(), lp.data_ptr(), stream=_stream())
+    assert ((lp.double() - x.double().log_softmax(-1)[:, 0]).abs() < 2.0 ** -14).all()
