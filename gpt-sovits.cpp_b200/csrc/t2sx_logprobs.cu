@@ -3,6 +3,12 @@
 //   m = max x,  s = sum e^(x - m),  w = sum e^(x - m) (x - m)     (over x > -inf)
 //   logprob = x_t - m - log s,   entropy = log s - w / s
 //   rank = #{x > x_t} + #{j < t: x_j = x_t}
+//
+// One pass over the logits: each thread holds a running (m, s, w), rescaled when its maximum grows
+// (s' = s e^(m - m'), w' = e^(m - m') (w + (m - m') s)), and leaves the maximum of each slot of
+// kGroup x slot_groups vectors in shared memory.  A value T that at least top_k elements reach follows
+// from the threads' maxima alone (T0 below); the slots that reach T, a few, are read again
+// and their elements >= T are the candidates, whose places in the list are counted.
 #include "../../include/t2sx.h"
 #include "t2sx_kernels.cuh"
 
@@ -12,6 +18,7 @@
 
 #include <cmath>
 #include <cstdio>
+#include <mutex>
 
 using namespace t2sx;
 
@@ -23,7 +30,11 @@ __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-constexpr int kThreads = 256;
+constexpr int kGroup = 4;            // 16-byte vectors that a thread has in flight
+constexpr int kCandidates = 1024;    // of one CTA (a warp's share of it for rows of one warp)
+constexpr int kMaxTop = 32;
+constexpr int kMaxSplit = 8;         // CTAs per row (a portable cluster)
+constexpr float kLog2e = 1.4426950408889634f;
 
 // Value and id of a candidate as one key: greater keys come first (values descending, ids
 // ascending).  -inf and NaN have no place in a list.
@@ -32,83 +43,440 @@ __device__ __forceinline__ unsigned long long order_key(float x, unsigned id) {
     b = (b & 0x80000000u) ? ~b : b | 0x80000000u;
     return (unsigned long long)b << 32 | (0xFFFFFFFFu - id);
 }
+__device__ __forceinline__ float key_value(unsigned long long key) {
+    unsigned b = (unsigned)(key >> 32);
+    return __uint_as_float((b & 0x80000000u) ? b & 0x7FFFFFFFu : ~b);
+}
 
-__device__ __forceinline__ float block_sum(float v, float* sh) {
-    for (int x = 16; x; x >>= 1) v += __shfl_xor_sync(~0u, v, x);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0f;
-    for (int i = 0; i < kThreads / 32; ++i) v += sh[i];
+// 2^x; the instruction's error is two units in the last place
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if one of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+    return *reinterpret_cast<float2*>(&r);
+}
+
+// A 16-byte vector of logits: its elements in f32, its maximum (NaN left out), -inf in every place.
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+    static constexpr int E = 4;
+    static __device__ __forceinline__ uint4 none() { return make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u); }
+    static __device__ __forceinline__ float2 pair(unsigned const (&w)[4], int i) {
+        return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    }
+    static __device__ __forceinline__ float max(const uint4& u) {
+        return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    }
+    static __device__ __forceinline__ unsigned bits(const float* p) { return __float_as_uint(*p); }
+};
+template <>
+struct Vec<__half> {
+    static constexpr int E = 8;
+    static __device__ __forceinline__ uint4 none() { return make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u); }
+    static __device__ __forceinline__ float2 pair(unsigned const (&w)[4], int i) { return __half22float2(*reinterpret_cast<const __half2*>(&w[i])); }
+    static __device__ __forceinline__ float max(const uint4& u) {
+        const __half2* h = reinterpret_cast<const __half2*>(&u);
+        const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ unsigned bits(const __half* p) { return __half_as_ushort(*p); }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+    static constexpr int E = 8;
+    static __device__ __forceinline__ uint4 none() { return make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u); }
+    static __device__ __forceinline__ float2 pair(unsigned const (&w)[4], int i) {
+        return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+    }
+    static __device__ __forceinline__ float max(const uint4& u) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+        const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ unsigned bits(const __nv_bfloat16* p) { return __bfloat16_as_ushort(*p); }
+};
+
+// A slot's maximum in 16 bits, never below it (the upper half of an f32, rounded up).
+__device__ __forceinline__ unsigned short slot_up(float x) {
+    const unsigned b = __float_as_uint(x);
+    return (unsigned short)((b & 0x80000000u) ? b >> 16 : (b + 0xFFFFu) >> 16);
+}
+__device__ __forceinline__ float slot_value(unsigned short b) { return __uint_as_float((unsigned)b << 16); }
+
+struct Stat {   // of part of a row
+    float m, s, w;      // s, w relative to m; all of them 0 but m where every element is -inf
+    int before;
+};
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
+    Stat r;
+    r.m = fmaxf(a.m, b.m);
+    // a part without an element above -inf has s = w = 0 (or NaN, which stays)
+    const float da = a.m == r.m ? 0.0f : fmaxf(a.m - r.m, -1e30f), db = b.m == r.m ? 0.0f : fmaxf(b.m - r.m, -1e30f);
+    const float fa = ex2(da * kLog2e), fb = ex2(db * kLog2e);
+    r.s = fmaf(a.s, fa, b.s * fb);
+    r.w = fmaf(fa, fmaf(da, a.s, a.w), fb * fmaf(db, b.s, b.w));
+    r.before = a.before + b.before;
+    return r;
+}
+__device__ __forceinline__ Stat warp_join(Stat a) {
+    for (int x = 16; x; x >>= 1) {
+        Stat b;
+        b.m = __shfl_xor_sync(~0u, a.m, x);
+        b.s = __shfl_xor_sync(~0u, a.s, x);
+        b.w = __shfl_xor_sync(~0u, a.w, x);
+        b.before = __shfl_xor_sync(~0u, a.before, x);
+        // both lanes take the same operands in the same order
+        a = (threadIdx.x & x) ? join(b, a) : join(a, b);
+    }
+    return a;
+}
+
+// The lanes' values in descending order.
+__device__ __forceinline__ float warp_sort(float v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int x = size >> 1; x; x >>= 1) {
+            const float o = __shfl_xor_sync(~0u, v, x);
+            const bool keep_max = ((lane & x) == 0) == ((lane & size) == 0);
+            v = keep_max ? fmaxf(v, o) : fminf(v, o);
+        }
     return v;
 }
 
-// One CTA per row, the row read once for each statistic and each place of the list.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-k_logprobs(const T* __restrict__ logits, long long stride, int vocab, const int32_t* __restrict__ tokens, int top_k,
-           float* __restrict__ logprob, float* __restrict__ entropy, int32_t* __restrict__ rank, int32_t* __restrict__ top_ids,
-           float* __restrict__ top_logprobs) {
-    __shared__ float sh[kThreads / 32];
-    __shared__ unsigned long long shk[kThreads / 32];
-    const long long row = blockIdx.x;
-    const T* x = logits + row * stride;
-    const int tid = threadIdx.x, t = tokens[row];
-    const bool given = t >= 0 && t < vocab;
-    const float xt = given ? to_f32(x[t]) : 0.0f;
-    float m = -INFINITY, bad = 0.0f;
-    for (int j = tid; j < vocab; j += kThreads) {
-        const float v = to_f32(x[j]);
-        if (!(v < INFINITY)) bad = 1.0f;
-        m = fmaxf(m, v);
-    }
-    for (int y = 16; y; y >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, y));
-    if ((tid & 31) == 0) sh[tid >> 5] = m;
-    __syncthreads();
-    for (int i = 0; i < kThreads / 32; ++i) m = fmaxf(m, sh[i]);
-    bad = block_sum(bad, sh);
-    float s = 0.0f, w = 0.0f, before = 0.0f;
-    for (int j = tid; j < vocab; j += kThreads) {
-        const float v = to_f32(x[j]);
-        if (v > xt || (v == xt && j < t)) before += 1.0f;
-        if (v == -INFINITY) continue;
-        const float d = v - m, e = expf(d);
-        s += e;
-        w = fmaf(e, d, w);
-    }
-    s = block_sum(s, sh);
-    w = block_sum(w, sh);
-    before = block_sum(before, sh);
-    const float log_s = s > 0.0f ? logf(s) : 0.0f;
-    if (tid == 0) {
-        logprob[row] = t == -1 ? 0.0f : !given || bad > 0.0f ? NAN : s > 0.0f ? xt - m - log_s : -INFINITY;
-        if (entropy) entropy[row] = bad > 0.0f ? NAN : s > 0.0f ? log_s - w / s : 0.0f;
-        if (rank) rank[row] = given ? (int)before : -1;
-    }
-    unsigned long long last = ~0ull;
-    for (int i = 0; i < top_k; ++i) {
-        unsigned long long best = 0;
-        for (int j = tid; j < vocab; j += kThreads) {
-            const float v = to_f32(x[j]);
-            if (!(v > -INFINITY)) continue;
-            const unsigned long long key = order_key(v, j);
-            if (key < last && key > best) best = key;
+struct Args {
+    long long stride;
+    int rows, vocab, top_k, slot_groups;
+    const int32_t* tokens;
+    float *logprob, *entropy;
+    int32_t *rank, *top_ids;
+    float* top_logprobs;
+};
+
+template <int WARPS>
+struct Shared {   // of one row's threads in a CTA
+    Stat stat[WARPS];
+    float best_max[WARPS][32];
+    int count;
+    unsigned long long best[WARPS];
+    static constexpr int PARTS = WARPS == 1 ? 1 : kMaxSplit;
+    Stat joined[PARTS];                                  // in the first CTA of a row: all of its CTAs'
+    unsigned long long lists[PARTS][kMaxTop];
+    unsigned long long cand[WARPS == 1 ? kCandidates / 4 : kCandidates];
+};
+
+// WARPS == 1: a warp per row, four rows in a CTA.  Else a row per CTA, or per cluster of `split` CTAs:
+// each takes a range of the row's vectors, and the first one joins what they found.
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS)
+k_logprobs(const T* __restrict__ logits, Args a) {
+    constexpr int E = Vec<T>::E, N = 32 * WARPS, ROWS = WARPS == 1 ? 4 : 1;
+    constexpr int CAND = WARPS == 1 ? kCandidates / 4 : kCandidates;
+    extern __shared__ __align__(16) unsigned char raw[];
+    const int sub = WARPS == 1 ? threadIdx.x >> 5 : 0, tid = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
+    const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
+    Shared<WARPS>& sh = reinterpret_cast<Shared<WARPS>*>(raw)[sub];
+    const int split = WARPS == 1 ? 1 : (int)gridDim.y, part = WARPS == 1 ? 0 : (int)blockIdx.y;
+    const long long row = (long long)blockIdx.x * ROWS + sub;
+    if (WARPS == 1 && row >= a.rows) return;   // warps of such a CTA wait for none of the others
+    auto sync = [] {
+        if constexpr (WARPS == 1) __syncwarp();
+        else __syncthreads();
+    };
+    if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA runs: its memory may be written
+    const T* x = logits + row * a.stride;
+    const int t = a.tokens[row];
+    const bool given = t >= 0 && t < a.vocab;
+
+    // The row on the grid of aligned vectors: the first and last ones may be partly outside it.
+    const int off = (int)(((uintptr_t)x & 15) / sizeof(T));
+    const int n_vec = (int)(((long long)off + a.vocab + E - 1) / E);
+    const int per = (n_vec + split - 1) / split, v0 = part * per, v1 = min(n_vec, v0 + per);
+    const uint4* xv = reinterpret_cast<const uint4*>(x - off);
+    auto load = [&](int v) -> uint4 {
+        if (v >= v1) return Vec<T>::none();
+        const int j = v * E - off;
+        if (j >= 0 && j + E <= a.vocab) return xv[v];
+        uint4 u = Vec<T>::none();
+        unsigned* w = reinterpret_cast<unsigned*>(&u);
+        for (int e = 0; e < E; ++e) {
+            if (j + e < 0 || j + e >= a.vocab) continue;
+            const unsigned b = Vec<T>::bits(x + j + e);
+            if (E == 4) w[e] = b;
+            else w[e / 2] = (e & 1) ? (w[e / 2] & 0x0000FFFFu) | b << 16 : (w[e / 2] & 0xFFFF0000u) | b;
         }
-        for (int y = 16; y; y >>= 1) {
-            const unsigned long long o = __shfl_xor_sync(~0u, best, y);
-            best = o > best ? o : best;
+        return u;
+    };
+
+    uint4 u[kGroup];
+#pragma unroll
+    for (int g = 0; g < kGroup; ++g) u[g] = load(v0 + g * N + tid);
+    const float xt = given ? to_f32(x[t]) : INFINITY;
+    unsigned short* slots = reinterpret_cast<unsigned short*>(raw + ROWS * sizeof(Shared<WARPS>));
+    int n_slots = 0;
+    float m = -INFINITY, slot = -INFINITY;
+    float2 s = {0.0f, 0.0f}, w = {0.0f, 0.0f};
+    int before = 0;
+    for (int base = v0, group = 0; base < v1; base += kGroup * N) {
+        uint4 c[kGroup];
+        float g_max = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+            c[g] = u[g];
+            u[g] = load(base + (kGroup + g) * N + tid);
+            g_max = fmaxf(g_max, Vec<T>::max(c[g]));
+        }
+        slot = fmaxf(slot, g_max);
+        if (++group == a.slot_groups) {
+            slots[(n_slots++ * ROWS + sub) * N + tid] = slot_up(slot);
+            slot = -INFINITY;
+            group = 0;
+        }
+        if (g_max > m) {
+            if (m > -INFINITY) {
+                const float d = fmaxf(m - g_max, -1e30f), f = ex2(d * kLog2e);
+                w = mul2(make_float2(f, f), fma2(make_float2(d, d), s, w));
+                s = mul2(make_float2(f, f), s);
+            }
+            m = g_max;
+        }
+        // x - m is exact or rounded once, also where x and m are the lowest values of the type; -inf becomes a
+        // finite number with the weight 0, and NaN (of +inf, too) stays in the sums
+        const float neg = m > -INFINITY ? -m : 0.0f;
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+            const unsigned b[4] = {c[g].x, c[g].y, c[g].z, c[g].w};
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i) {
+                float2 d = add2(Vec<T>::pair(b, i), make_float2(neg, neg));
+                d.x = max_nan(d.x, -1e30f);
+                d.y = max_nan(d.y, -1e30f);
+                const float2 y = mul2(d, make_float2(kLog2e, kLog2e));
+                const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                s = add2(s, e);
+                w = fma2(e, d, w);
+            }
+        }
+        if (g_max >= xt) {   // seldom, for a token that is likely
+#pragma unroll
+            for (int g = 0; g < kGroup; ++g) {
+                const unsigned b[4] = {c[g].x, c[g].y, c[g].z, c[g].w};
+                const int vec = base + g * N + tid, j = vec * E - off;
+                if (vec >= v1) break;
+#pragma unroll
+                for (int i = 0; i < E; ++i) {   // (the -inf in front of the row equals a masked token's logit)
+                    const float2 p = Vec<T>::pair(b, i / 2);
+                    const float v = (i & 1) ? p.y : p.x;
+                    before += v > xt || (v == xt && j + i < t && j + i >= 0);
+                }
+            }
+        }
+        if (base + kGroup * N >= v1 && group) slots[(n_slots++ * ROWS + sub) * N + tid] = slot_up(slot);
+    }
+
+    // this thread's part, then the warp's, then the CTA's
+    Stat st = warp_join(Stat{m, s.x + s.y, w.x + w.y, before});
+    // T0: the top_k-th greatest of the threads' maxima, so at least top_k elements reach it (-inf: fewer than
+    // top_k threads have an element above -inf)
+    float T0 = a.top_k ? warp_sort(m) : -INFINITY;
+    if constexpr (WARPS > 1) {
+        if (lane == 0) sh.stat[warp] = st;
+        if (tid == 0) sh.count = 0;
+        if (a.top_k) {
+            sh.best_max[warp][lane] = T0;
+            for (int h = WARPS / 2; h; h /= 2) {   // the 32 greatest of two lists, again in order
+                __syncthreads();
+                if (warp < h) {
+                    T0 = fmaxf(T0, sh.best_max[warp + h][31 - lane]);
+#pragma unroll
+                    for (int y = 16; y; y >>= 1) {
+                        const float o = __shfl_xor_sync(~0u, T0, y);
+                        T0 = (lane & y) ? fminf(T0, o) : fmaxf(T0, o);
+                    }
+                    sh.best_max[warp][lane] = T0;
+                }
+            }
         }
         __syncthreads();
-        if ((tid & 31) == 0) shk[tid >> 5] = best;
-        __syncthreads();
-        for (int k = 0; k < kThreads / 32; ++k) best = shk[k] > best ? shk[k] : best;
-        last = best;
+        st = sh.stat[0];
+        for (int i = 1; i < WARPS; ++i) st = join(st, sh.stat[i]);
+        if (a.top_k) T0 = sh.best_max[0][a.top_k - 1];
+    } else {
+        if (a.top_k) T0 = __shfl_sync(~0u, T0, a.top_k - 1);
+        if (lane == 0) sh.count = 0;
+        __syncwarp();
+    }
+
+    if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (a.top_k) {
+        // the elements that reach T0, from the slots that do (each thread reads its own)
+        for (int k = 0; k < n_slots; ++k) {
+            if (!(slot_value(slots[(k * ROWS + sub) * N + tid]) >= T0)) continue;
+            for (int g = 0; g < kGroup * a.slot_groups; ++g) {
+                const int v = v0 + (k * kGroup * a.slot_groups + g) * N + tid;
+                if (v >= v1) break;
+                const uint4 q = load(v);
+                const unsigned b[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const float2 p = Vec<T>::pair(b, i / 2);
+                    const float y = (i & 1) ? p.y : p.x;
+                    if (y >= T0 && y > -INFINITY) {
+                        const int at = atomicAdd(&sh.count, 1);
+                        if (at < CAND) sh.cand[at] = order_key(y, v * E - off + i);
+                    }
+                }
+            }
+        }
+        sync();
+        const int n = sh.count;
+        unsigned long long* list = sh.lists[0];
+        if (split > 1) {   // in the first CTA of the row
+            unsigned long long* mine = sh.lists[part];
+            asm("mapa.u64 %0, %1, 0;" : "=l"(list) : "l"(mine));
+        }
+        for (int i = tid; i < a.top_k; i += N) list[i] = 0;
+        sync();
+        if (n <= CAND) {
+            // a candidate's place is the number of greater ones: keys differ, whatever order they came in
+            for (int i = tid; i < n; i += N) {
+                const unsigned long long key = sh.cand[i];
+                int place = 0;
+                for (int j = 0; j < n; ++j) place += sh.cand[j] > key;
+                if (place < a.top_k) list[place] = key;
+            }
+        } else {
+            // more ties than the list of candidates holds: place by place, the greatest key below the last one
+            unsigned long long last = ~0ull;
+            for (int i = 0; i < a.top_k && last; ++i) {
+                unsigned long long best = 0;
+                for (int v = v0 + tid; v < v1; v += N) {
+                    const uint4 q = load(v);
+                    const unsigned b[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const float2 p = Vec<T>::pair(b, e / 2);
+                        const float y = (e & 1) ? p.y : p.x;
+                        if (!(y > -INFINITY)) continue;
+                        const unsigned long long key = order_key(y, v * E - off + e);
+                        if (key < last && key > best) best = key;
+                    }
+                }
+                for (int y = 16; y; y >>= 1) {
+                    const unsigned long long o = __shfl_xor_sync(~0u, best, y);
+                    best = o > best ? o : best;
+                }
+                if constexpr (WARPS > 1) {
+                    __syncthreads();
+                    if (lane == 0) sh.best[warp] = best;
+                    __syncthreads();
+                    for (int k = 0; k < WARPS; ++k) best = sh.best[k] > best ? sh.best[k] : best;
+                }
+                if (tid == 0) list[i] = best;
+                last = best;
+            }
+        }
+    }
+    if (split > 1) {
         if (tid == 0) {
-            const unsigned id = 0xFFFFFFFFu - (unsigned)best;
-            top_ids[row * top_k + i] = best ? (int)id : -1;
-            top_logprobs[row * top_k + i] = bad > 0.0f ? NAN : best ? to_f32(x[id]) - m - log_s : -INFINITY;
+            Stat *mine = &sh.joined[part], *first;
+            asm("mapa.u64 %0, %1, 0;" : "=l"(first) : "l"(mine));
+            *first = st;
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (part != 0) return;
+        st = sh.joined[0];
+        for (int i = 1; i < split; ++i) st = join(st, sh.joined[i]);
+    } else {
+        sync();
+    }
+    const bool bad = !(st.s < INFINITY);   // NaN or +inf in the row
+    const float log_s = st.s > 0.0f ? logf(st.s) : 0.0f;
+    if (tid == 0) {
+        a.logprob[row] = t == -1 ? 0.0f : !given || bad ? NAN : st.s > 0.0f ? xt - st.m - log_s : -INFINITY;
+        if (a.entropy) a.entropy[row] = bad ? NAN : st.s > 0.0f ? log_s - st.w / st.s : 0.0f;
+        if (a.rank) a.rank[row] = given ? st.before : -1;
+    }
+    // the parts' lists, each in order: an entry's place is the number of greater ones
+    const int n = split * a.top_k;
+    for (int i = tid; i < n; i += N) {
+        const unsigned long long key = sh.lists[i / a.top_k][i % a.top_k];
+        int place = i % a.top_k;
+        if (split > 1) {
+            place = 0;
+            for (int j = 0; j < n; ++j) {
+                const unsigned long long o = sh.lists[j / a.top_k][j % a.top_k];
+                place += o > key || (o == key && j < i);   // empty entries are equal
+            }
+        }
+        if (place < a.top_k) {
+            const unsigned id = 0xFFFFFFFFu - (unsigned)key;
+            a.top_ids[row * a.top_k + place] = key ? (int)id : -1;
+            a.top_logprobs[row * a.top_k + place] = bad ? NAN : key ? key_value(key) - st.m - log_s : -INFINITY;
         }
     }
+}
+
+template <typename T, int WARPS>
+cudaError_t launch(const T* x, Args a, int split, cudaStream_t st) {
+    constexpr int N = 32 * WARPS, ROWS = WARPS == 1 ? 4 : 1;
+    // slots of 16 bits: at most 32 KB of them, so that a CTA's share of shared memory stays small
+    const long long vecs = ((long long)a.vocab / Vec<T>::E + 2 + split - 1) / split;
+    const long long groups = (vecs + (long long)kGroup * N - 1) / ((long long)kGroup * N);
+    const int most = (32 << 10) / (2 * N * ROWS);
+    a.slot_groups = (int)((groups + most - 1) / most);
+    const size_t smem = ROWS * sizeof(Shared<WARPS>) + (size_t)((groups + a.slot_groups - 1) / a.slot_groups) * ROWS * N * 2;
+    static std::once_flag once[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::call_once(once[dev & 63], [&] {
+        cudaFuncSetAttribute(k_logprobs<T, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (32 << 10) + ROWS * (int)sizeof(Shared<WARPS>));
+    });
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((a.rows + ROWS - 1) / ROWS), split);
+    cfg.blockDim = WARPS == 1 ? 128 : N;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 1;
+    at.val.clusterDim.y = split;
+    at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = split > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, k_logprobs<T, WARPS>, x, a);
+}
+
+template <typename T>
+cudaError_t dispatch(const T* x, const Args& a, cudaStream_t st) {
+    if (a.vocab <= 2048) return launch<T, 1>(x, a, 1, st);
+    int split = 1;
+    while (split < kMaxSplit && (long long)a.rows * split * 2 <= 296 && a.vocab / (2 * split) >= 4096) split *= 2;
+    return launch<T, 16>(x, a, split, st);
 }
 
 int bad(const char* m) { return t2sx_set_error(T2SX_ERR_INVALID, m); }
@@ -135,14 +503,11 @@ extern "C" int t2sx_token_logprobs(int32_t device, int32_t type, int64_t rows, i
     cudaError_t e = dg.set(device);
     if (e != cudaSuccess) return t2sx_set_error(T2SX_ERR_CUDA, cudaGetErrorString(e));
     cudaStream_t st = (cudaStream_t)stream;
-    auto go = [&](auto kernel, auto* x) {
-        kernel<<<(unsigned)rows, kThreads, 0, st>>>(x, (long long)stride, (int)vocab, tokens_dev, top_k, logprob_dev, entropy_dev,
-                                                   rank_dev, top_ids_dev, top_logprobs_dev);
-    };
-    if (type == T2SX_TYPE_F32) go(k_logprobs<float>, (const float*)logits_dev);
-    else if (type == T2SX_TYPE_F16) go(k_logprobs<__half>, (const __half*)logits_dev);
-    else go(k_logprobs<__nv_bfloat16>, (const __nv_bfloat16*)logits_dev);
-    e = cudaGetLastError();
+    const Args a = {(long long)stride, (int)rows, (int)vocab, top_k, 1, tokens_dev, logprob_dev, entropy_dev, rank_dev, top_ids_dev,
+                    top_logprobs_dev};
+    if (type == T2SX_TYPE_F32) e = dispatch((const float*)logits_dev, a, st);
+    else if (type == T2SX_TYPE_F16) e = dispatch((const __half*)logits_dev, a, st);
+    else e = dispatch((const __nv_bfloat16*)logits_dev, a, st);
     if (e != cudaSuccess) return t2sx_set_error(T2SX_ERR_CUDA, cudaGetErrorString(e));
     return T2SX_OK;
 }
