@@ -1,4 +1,12 @@
 // Attention of one step's tokens over a pool of shared cache pages.
+//
+// A plan arranges the sequences' page lists as a trie: a node is a run of pages that a set of sequences has
+// in common, and the tokens of that set are its rows.  Each node's pages are read once for all of
+// its rows.  Per node, K/V head and range of pages (a split), rows x keys is a small attention of its own:
+//     m = max_j s_j,  l = sum_j 2^(s_j - m + c),  O = sum_j 2^(s_j - m + c) v_j,   s_j = scale log2(e) q . k_j
+// and a token's result follows from its parts: M = max m_i, out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
+// The constant c keeps small weights above the subnormal numbers of f16 (and is harmless for bf16).
+// A row is a (token, query head of the K/V head's group); `group` heads of a token are neighbours.
 #include "t2sx_pool.cuh"
 
 #include <cuda_bf16.h>
@@ -8,99 +16,366 @@
 #include <cmath>
 #include <cstring>
 #include <memory>
+#include <mutex>
 
 using namespace t2sx;
 
 namespace {
 
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kWeightExp = 7.0f;   // c above: weights are at most 2^7
+constexpr int kTileRows = 16;        // rows of a warp's tile (the m of mma.m16n8k16)
 
-// The rows of a plan on the device.
-struct RowView {
-    const int32_t* limit;       // [rows] positions that the row sees; its own is the last of them
-    const int32_t* table_at;    // [rows] where its sequence's page ids start in `table`
-    const int32_t* table;
-    int rows;
+// A tile of rows against a range of a node's pages.
+struct Item {
+    int32_t tokens_at;   // the node's tokens start here in `tokens`
+    int32_t row0, rows;  // rows of the node: token row / group, head row % group
+    int32_t pages_at;    // page ids
+    int32_t n_pages;
+    int32_t pos0;        // position of the first page's first key
+    int32_t part;        // row r's part is number part + r
+    int32_t end;         // the node's filled positions end here
 };
+
+struct Token {
+    int32_t limit;       // positions that it sees; its own is the last of them
+    int32_t page;        // page of its own position
+    int32_t part_at;     // its parts' numbers (of its first head) start here in `parts`
+    int32_t n_parts;     // one: the item writes the result itself
+};
+
+struct PlanView {
+    const Token* info;       // [rows of the step]
+    const int32_t* tokens;   // nodes' tokens, as rows of the step
+    const int32_t* pages;
+    const Item* items;
+    const int32_t* parts;
+    const int32_t* joins;    // tokens of several parts
+    float* part_o;           // [part][K/V head][dim]
+    float2* part_ml;         // [part][K/V head]
+    int rows, n_items, n_joins, group, n_kv;
+};
+
+// Strided tensors of one call.
+template <typename T>
+struct Tensors {
+    const T *q, *k, *v;      // k, v: the layer's first page
+    T* out;
+    float* lse;
+    long long q_stride, out_stride;
+    float scale2;            // scale * log2(e)
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack2(__half, float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void mma16816(__half, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816(__nv_bfloat16, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t smem, const void* gmem) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void dependents_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // One 16-byte word per thread: the rows' keys and values go to their positions.
 __global__ void __launch_bounds__(256)
-k_write_rows(RowView r, const uint4* __restrict__ kn, const uint4* __restrict__ vn, long long stride_vec, uint4* __restrict__ k,
-             uint4* __restrict__ v, size_t layer_page0, int n_kv, int row_vec) {
+k_write_rows(const Token* __restrict__ info, int rows, const uint4* __restrict__ kn, const uint4* __restrict__ vn,
+             long long stride_vec, uint4* __restrict__ k, uint4* __restrict__ v, int n_kv, int row_vec) {
+    dependents_launch();
     const int per_row = n_kv * row_vec;
     const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (long long)r.rows * per_row) return;
+    if (i >= (long long)rows * per_row) return;
     const int row = (int)(i / per_row), j = (int)(i - (long long)row * per_row), h = j / row_vec, c = j - h * row_vec;
-    const int pos = r.limit[row] - 1;
-    const size_t page = layer_page0 + r.table[r.table_at[row] + pos / kPoolPage];
-    const size_t dst = ((page * n_kv + h) * kPoolPage + pos % kPoolPage) * row_vec + c;
+    const Token t = info[row];
+    const size_t dst = (((size_t)t.page * n_kv + h) * kPoolPage + (t.limit - 1) % kPoolPage) * row_vec + c;
     k[dst] = kn[row * stride_vec + j];
     v[dst] = vn[row * stride_vec + j];
 }
 
-// One warp per (row, query head): 32 positions at a time, one per lane for the scores, the lanes'
-// shares of the head for the output.
+// Tiles of a head dimension: keys per stage of the ring and stages.
+template <int D>
+struct TileShape {
+    static constexpr int KEYS = D == 32 ? 64 : 32, STAGES = 3;
+    static constexpr int HALF = KEYS * D * 2;   // bytes of a stage's K (or V)
+    static constexpr int SMEM = STAGES * 2 * HALF;
+};
+
+// 16-byte chunk `c` of key `row` in a tile: chunks are exchanged within 128 bytes so that the eight rows
+// of an ldmatrix matrix lie in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t tile_at(int row, int c) {
+    if constexpr (D == 32) return row * 64 + ((c ^ (row >> 1)) & 3) * 16;
+    else return row * (D * 2) + ((c & ~7) | ((c ^ row) & 7)) * 16;
+}
+
+// One warp per (item, K/V head): at most 16 rows, keys streamed through a ring of its own.
 template <typename T, int D>
-__global__ void __launch_bounds__(128)
-k_attend_rows(RowView r, const T* __restrict__ q, long long q_stride, const T* __restrict__ k, const T* __restrict__ v,
-              size_t layer_page0, int n_heads, int n_kv, float scale, T* __restrict__ out, long long out_stride,
-              float* __restrict__ lse) {
-    const int lane = threadIdx.x & 31, head = blockIdx.y * 4 + (threadIdx.x >> 5), row = blockIdx.x;
-    if (head >= n_heads) return;
-    const int kvh = head / (n_heads / n_kv), limit = r.limit[row];
-    const int32_t* table = r.table + r.table_at[row];
-    const T* qr = q + row * q_stride + head * D;
-    float m = -INFINITY, l = 0.0f, o[D / 32] = {};
-    for (int p0 = 0; p0 < limit; p0 += 32) {
-        const size_t at = (((layer_page0 + table[p0 / kPoolPage]) * n_kv + kvh) * kPoolPage + p0 % kPoolPage) * D;
-        float s = 0.0f;
-        for (int d = 0; d < D; ++d) s = fmaf(to_f32(qr[d]), to_f32(k[at + lane * D + d]), s);
-        s = p0 + lane < limit ? s * scale : -INFINITY;
-        float mx = s;
-        for (int x = 16; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, x));
-        mx = fmaxf(mx, m);
-        const float base = mx == -INFINITY ? 0.0f : mx;
-        const float p = expf(s - base), f = expf(m - base);
-        m = mx;
-        l = fmaf(l, f, p);
-        for (int j = 0; j < D / 32; ++j) o[j] *= f;
-        for (int t = 0; t < 32 && p0 + t < limit; ++t) {
-            const float pt = __shfl_sync(~0u, p, t);
-            for (int j = 0; j < D / 32; ++j) o[j] = fmaf(pt, to_f32(v[at + t * D + j * 32 + lane]), o[j]);
+__global__ void __launch_bounds__(32)
+k_attend_tiles(PlanView pv, Tensors<T> x) {
+    using S = TileShape<D>;
+    constexpr int NT = S::KEYS / 8, DT = D / 8, KS = D / 16;   // key tiles, dim tiles, steps along the dims
+    extern __shared__ __align__(1024) unsigned char ring[];
+    const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring);
+    const int lane = threadIdx.x, kvh = blockIdx.x % pv.n_kv;   // neighbours read one page
+    const Item it = pv.items[blockIdx.x / pv.n_kv];
+    const int group = pv.group;
+
+    const int tiles = it.n_pages * (kPoolPage / S::KEYS);
+    int page_id = it.pages_at >= 0 && lane < it.n_pages ? pv.pages[it.pages_at + lane] : 0;
+    int page_base = 0;                                // pages [page_base, page_base + 32) are in the lanes
+    auto request = [&](int t) {
+        if (t < tiles) {
+            const int pg = t / (kPoolPage / S::KEYS), sub = t % (kPoolPage / S::KEYS);
+            if (pg - page_base >= 32) {
+                page_base += 32;
+                page_id = page_base + lane < it.n_pages ? pv.pages[it.pages_at + page_base + lane] : 0;
+            }
+            const int page = __shfl_sync(~0u, page_id, pg - page_base);
+            const size_t at = (((size_t)page * pv.n_kv + kvh) * kPoolPage + sub * S::KEYS) * D;
+            const uint32_t dst = ring0 + (t % S::STAGES) * 2 * S::HALF;
+            const char *ks = reinterpret_cast<const char*>(x.k + at), *vs = reinterpret_cast<const char*>(x.v + at);
+#pragma unroll
+            for (int i = 0; i < S::HALF / 512; ++i) {
+                const int c = i * 32 + lane;
+                const uint32_t d = tile_at<D>(c / (D / 8), c % (D / 8));
+                cp16(dst + d, ks + c * 16);
+                cp16(dst + S::HALF + d, vs + c * 16);
+            }
+        }
+        cp_commit();
+    };
+
+    // rows lane / 4 and lane / 4 + 8
+    int row_of[2], head_of[2], limit[2];
+    bool live[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = lane / 4 + 8 * i, mr = it.row0 + r;
+        live[i] = r < it.rows;
+        row_of[i] = live[i] ? pv.tokens[it.tokens_at + mr / group] : 0;
+        head_of[i] = kvh * group + mr % group;
+        limit[i] = live[i] ? pv.info[row_of[i]].limit : 0;
+    }
+    dependents_wait();   // the step's own keys and values
+    for (int t = 0; t < S::STAGES - 1; ++t) request(t);
+    uint32_t qf[KS][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(x.q + row_of[i] * x.q_stride + head_of[i] * D);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            qf[k][i] = live[i] ? src[k * 8 + lane % 4] : 0;
+            qf[k][i + 2] = live[i] ? src[k * 8 + 4 + lane % 4] : 0;
         }
     }
-    for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(~0u, l, x);
-    for (int j = 0; j < D / 32; ++j)
-        out[row * out_stride + head * D + j * 32 + lane] = from_f32<T>(l > 0.0f ? o[j] / l : 0.0f);
-    if (lse && lane == 0) lse[(size_t)row * n_heads + head] = l > 0.0f ? m + logf(l) : -INFINITY;
+    // the smallest limit of the rows: keys below it need no mask
+    int free_to = min(live[0] ? limit[0] : INT32_MAX, live[1] ? limit[1] : INT32_MAX);
+    for (int y = 16; y; y >>= 1) free_to = min(free_to, __shfl_xor_sync(~0u, free_to, y));
+
+    const bool upper = it.rows > 8;
+    float o[DT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    for (int t = 0; t < tiles; ++t) {
+        cp_wait<S::STAGES - 2>();
+        __syncwarp();
+        const uint32_t kt = ring0 + (t % S::STAGES) * 2 * S::HALF, vt = kt + S::HALF;
+        const int pos = it.pos0 + t * S::KEYS;
+        if (pos + S::KEYS > it.end) {   // what stands beyond the filled positions may be NaN: as values it counts 0
+            for (int c = max(0, it.end - pos) * (D / 8) + lane; c < S::KEYS * (D / 8); c += 32)
+                *reinterpret_cast<uint4*>(ring + (vt - ring0) + tile_at<D>(c / (D / 8), c % (D / 8))) = make_uint4(0, 0, 0, 0);
+            __syncwarp();
+        }
+        float s[NT][4] = {};
+#pragma unroll
+        for (int n = 0; n < NT; n += 2)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint32_t b[4];
+                ldsm4(b, kt + tile_at<D>(n * 8 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+                mma16816(T(), s[n], qf[k], b[0], b[1]);
+                mma16816(T(), s[n + 1], qf[k], b[2], b[3]);
+            }
+        const bool masked = pos + S::KEYS > free_to;
+        uint32_t p[NT][2];
+        bool grew = false;
+        float alpha[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (i == 1 && !upper) {
+                alpha[1] = 1.0f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) p[n][1] = 0;
+                break;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float y = s[n][2 * i + e] * x.scale2;
+                    if (masked && pos + n * 8 + 2 * (lane % 4) + e >= limit[i]) y = -INFINITY;
+                    s[n][2 * i + e] = y;
+                    mx = fmaxf(mx, y);
+                }
+            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+            mx = fmaxf(mx, m[i]);
+            const float base = mx == -INFINITY ? 0.0f : mx - kWeightExp;
+            alpha[i] = m[i] == -INFINITY ? 0.0f : ex2(m[i] - mx);
+            grew |= mx > m[i];
+            m[i] = mx;
+            float sum = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float a = ex2(s[n][2 * i] - base), b = ex2(s[n][2 * i + 1] - base);
+                sum += a + b;
+                p[n][i] = pack2(T(), a, b);
+            }
+            l[i] = fmaf(l[i], alpha[i], sum);
+        }
+        if (__any_sync(~0u, grew)) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                o[d][0] *= alpha[0]; o[d][1] *= alpha[0];
+                o[d][2] *= alpha[1]; o[d][3] *= alpha[1];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+            const uint32_t a[4] = {p[n][0], p[n][1], p[n + 1][0], p[n + 1][1]};
+#pragma unroll
+            for (int d = 0; d < DT; d += 2) {
+                uint32_t b[4];
+                ldsm4_t(b, vt + tile_at<D>(n * 8 + (lane & 15), d + (lane >> 4)));
+                mma16816(T(), o[d], a, b[0], b[1]);
+                mma16816(T(), o[d + 1], a, b[2], b[3]);
+            }
+        }
+        __syncwarp();
+        request(t + S::STAGES - 1);
+    }
+    cp_wait<0>();
+    dependents_launch();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float sum = l[i];
+        sum += __shfl_xor_sync(~0u, sum, 1);
+        sum += __shfl_xor_sync(~0u, sum, 2);
+        if (!live[i] || limit[i] <= it.pos0) continue;   // such a row has no part here
+        if (pv.info[row_of[i]].n_parts == 1) {
+            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+            uint32_t* dst = reinterpret_cast<uint32_t*>(x.out + row_of[i] * x.out_stride + head_of[i] * D);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dst[d * 4 + lane % 4] = pack2(T(), o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
+            if (x.lse && lane % 4 == 0)
+                x.lse[(size_t)row_of[i] * (pv.n_kv * group) + head_of[i]] =
+                    sum > 0.0f ? (m[i] - kWeightExp + log2f(sum)) * kLn2 : -INFINITY;
+        } else {
+            const size_t at = (size_t)(it.part + it.row0 + lane / 4 + 8 * i) * pv.n_kv + kvh;
+            float2* dst = reinterpret_cast<float2*>(pv.part_o + at * D);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dst[d * 4 + lane % 4] = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+            if (lane % 4 == 0) pv.part_ml[at] = make_float2(m[i], sum);
+        }
+    }
+}
+
+// One warp per (token of several parts, query head): the parts in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(128)
+k_join_parts(PlanView pv, Tensors<T> x) {
+    dependents_wait();
+    const int lane = threadIdx.x & 31, heads = pv.n_kv * pv.group;
+    const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (w >= (long long)pv.n_joins * heads) return;
+    const int row = pv.joins[w / heads], head = (int)(w % heads), kvh = head / pv.group, g = head % pv.group;
+    const Token t = pv.info[row];
+    float M = -INFINITY;
+    for (int i = lane; i < t.n_parts; i += 32) M = fmaxf(M, pv.part_ml[(size_t)(pv.parts[t.part_at + i] + g) * pv.n_kv + kvh].x);
+    for (int y = 16; y; y >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, y));
+    float acc[D / 32] = {}, l = 0.0f;
+    for (int i = 0; i < t.n_parts; ++i) {
+        const size_t at = (size_t)(pv.parts[t.part_at + i] + g) * pv.n_kv + kvh;
+        const float2 ml = pv.part_ml[at];
+        const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+        l = fmaf(f, ml.y, l);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) acc[j] = fmaf(f, pv.part_o[at * D + j * 32 + lane], acc[j]);
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+        const uint32_t h = pack2(T(), acc[j] * inv, 0.0f);
+        reinterpret_cast<uint16_t*>(x.out + row * x.out_stride + head * D)[j * 32 + lane] = (uint16_t)h;
+    }
+    if (x.lse && lane == 0) x.lse[(size_t)row * heads + head] = l > 0.0f ? (M - kWeightExp + log2f(l)) * kLn2 : -INFINITY;
 }
 
 int bad(const char* m) { return t2sx_set_error(T2SX_ERR_INVALID, m); }
+
+// A run of pages that a set of sequences shares (or that one has for itself).
+struct Node {
+    int32_t tokens_at, n_tokens;
+    int32_t pages_at, n_pages;
+    int32_t pos0, end;
+};
+
+int sm_count(int device) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) return 148;
+    return n;
+}
 
 }  // namespace
 
 struct t2sx_plan {
     t2sx_pool* pool = nullptr;
-    int n_heads = 0;
-    bool ready = false;
+    int n_heads = 0, n_sm = 148;
+    bool ready = false, shared_rows = false;
     uint64_t version = 0;          // of the pool at the update
-    int rows = 0;
     // host copy of what the device gets, in pinned memory: two buffers, so that an update need not
     // wait for the previous one's upload
     uint8_t* host[2] = {};
     size_t host_bytes[2] = {};
     cudaEvent_t sent[2] = {};
     int turn = 0;
-    uint8_t* dev = nullptr;
-    size_t dev_bytes = 0;
-    RowView view = {};
+    uint8_t *dev = nullptr, *work = nullptr;
+    size_t dev_bytes = 0, work_bytes = 0;
+    PlanView view = {};
+    // scratch of an update
+    std::vector<int32_t> order, next_order, group_of, count, group_page, tokens, pages, parts, joins;
+    std::vector<int32_t> stamp, stamp_group, row0;
+    std::vector<Token> info;
+    std::vector<Node> nodes;
+    std::vector<Item> items;
 };
 
 static void plan_release(t2sx_plan* a) {
@@ -113,6 +388,7 @@ static void plan_release(t2sx_plan* a) {
         if (a->host[i]) cudaFreeHost(a->host[i]);
     }
     if (a->dev) cudaFree(a->dev);
+    if (a->work) cudaFree(a->work);
     delete a;
     if (--p->n_plans == 0 && p->closed) t2sx_pool_release_object(p);
 }
@@ -129,6 +405,7 @@ extern "C" int t2sx_plan_create(t2sx_pool* p, int32_t n_heads, t2sx_plan** out) 
         a->pool = p;
         a->n_heads = n_heads;
         ++p->n_plans;
+        a->n_sm = sm_count(p->device);
         for (int i = 0; i < 2; ++i) POOL_CK(cudaEventCreateWithFlags(&a->sent[i], cudaEventDisableTiming));
         *out = a.release();
         return T2SX_OK;
@@ -137,6 +414,144 @@ extern "C" int t2sx_plan_create(t2sx_pool* p, int32_t n_heads, t2sx_plan** out) 
 
 extern "C" void t2sx_plan_free(t2sx_plan* a) {
     if (a) plan_release(a);
+}
+
+// The trie of the sequences' page lists: every entry of a list is looked at once or twice.  Sequences are
+// split by the page that follows their common run, keeping their order.
+static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int32_t* n_new) {
+    t2sx_pool* p = a->pool;
+    a->nodes.clear(); a->tokens.clear(); a->pages.clear();
+    a->order.clear();
+    for (int32_t i = 0; i < n; ++i)
+        if (n_new[i] > 0) a->order.push_back(i);
+    if (a->stamp.size() < (size_t)p->n_pages) { a->stamp.assign(p->n_pages, -1); a->stamp_group.assign(p->n_pages, 0); }
+    struct Set { int32_t lo, hi, depth; };   // a range of `order`, and the pages above it
+    std::vector<Set> todo;
+    if (!a->order.empty()) todo.push_back({0, (int32_t)a->order.size(), 0});
+    int32_t round = 0;
+    std::fill(a->stamp.begin(), a->stamp.end(), -1);
+    auto emit = [&](const Set& s, int32_t to) {
+        Node nd;
+        nd.tokens_at = (int32_t)a->tokens.size();
+        for (int32_t j = s.lo; j < s.hi; ++j) {
+            const int32_t i = a->order[j];
+            for (int32_t k = 0; k < n_new[i]; ++k) a->tokens.push_back(a->row0[i] + k);
+        }
+        nd.n_tokens = (int32_t)a->tokens.size() - nd.tokens_at;
+        const std::vector<int32_t>& t = p->table[seqs[a->order[s.lo]]];
+        nd.pages_at = (int32_t)a->pages.size();
+        a->pages.insert(a->pages.end(), t.begin() + s.depth, t.begin() + to);
+        nd.n_pages = to - s.depth;
+        nd.pos0 = s.depth * kPoolPage;
+        // pages of several sequences are full; a sequence's own ones end with it
+        nd.end = s.hi - s.lo > 1 ? to * kPoolPage : (int32_t)std::min<int64_t>((int64_t)to * kPoolPage, p->len[seqs[a->order[s.lo]]]);
+        a->nodes.push_back(nd);
+    };
+    while (!todo.empty()) {
+        const Set s = todo.back();
+        todo.pop_back();
+        const std::vector<int32_t>& t = p->table[seqs[a->order[s.lo]]];
+        if (s.hi - s.lo == 1) {
+            if ((size_t)s.depth < t.size()) emit(s, (int32_t)t.size());
+            continue;
+        }
+        int32_t common = (int32_t)t.size();
+        for (int32_t j = s.lo + 1; j < s.hi; ++j) {
+            const std::vector<int32_t>& o = p->table[seqs[a->order[j]]];
+            const int32_t most = std::min<int32_t>(common, (int32_t)o.size());
+            int32_t k = s.depth;
+            while (k < most && o[k] == t[k]) ++k;
+            common = k;
+        }
+        if (common > s.depth) emit(s, common);
+        // split by the next page
+        const int32_t here = round++;
+        a->count.clear();
+        a->group_of.assign(s.hi - s.lo, -1);
+        for (int32_t j = s.lo; j < s.hi; ++j) {
+            const std::vector<int32_t>& o = p->table[seqs[a->order[j]]];
+            if (o.size() <= (size_t)common) continue;   // ends here
+            const int32_t page = o[common];
+            if (a->stamp[page] != here) {
+                a->stamp[page] = here;
+                a->stamp_group[page] = (int32_t)a->count.size();
+                a->count.push_back(0);
+            }
+            a->group_of[j - s.lo] = a->stamp_group[page];
+            ++a->count[a->stamp_group[page]];
+        }
+        a->next_order.resize(s.hi - s.lo);
+        int32_t at = 0;
+        for (int32_t& c : a->count) { const int32_t size = c; c = at; at += size; }
+        a->group_page.assign(a->count.begin(), a->count.end());   // where each one starts
+        for (int32_t j = s.lo; j < s.hi; ++j)
+            if (a->group_of[j - s.lo] >= 0) a->next_order[a->count[a->group_of[j - s.lo]]++] = a->order[j];
+        std::copy(a->next_order.begin(), a->next_order.begin() + at, a->order.begin() + s.lo);
+        for (size_t g = a->count.size(); g-- > 0;)
+            todo.push_back({s.lo + a->group_page[g], s.lo + a->count[g], common});
+    }
+}
+
+// Items and parts from the nodes.  A node's pages are split so that there are several items for each warp
+// that the device holds, and each part's result is small against the keys that it stands for.
+static void build_items(t2sx_plan* a) {
+    const int group = a->n_heads / a->pool->n_kv, n_kv = a->pool->n_kv;
+    a->items.clear(); a->parts.clear(); a->joins.clear();
+    int64_t work = 0;
+    for (const Node& nd : a->nodes) work += (int64_t)nd.n_pages * ((nd.n_tokens * (int64_t)group + kTileRows - 1) / kTileRows);
+    const int64_t warps = (int64_t)a->n_sm * 9;
+    const int64_t chunk = std::max<int64_t>(2, work * n_kv / (warps * 3));
+    struct Split { int32_t node, page, n_pages; int64_t part; };
+    std::vector<Split> splits;
+    int64_t part = 0;
+    for (size_t i = 0; i < a->nodes.size(); ++i) {
+        const Node& nd = a->nodes[i];
+        const int32_t n = (int32_t)((nd.n_pages + chunk - 1) / chunk), per = (nd.n_pages + n - 1) / n;
+        for (int32_t pg = 0; pg < nd.n_pages; pg += per) {
+            splits.push_back({(int32_t)i, pg, std::min(per, nd.n_pages - pg), part});
+            part += (int64_t)nd.n_tokens * group;
+        }
+    }
+    for (const Split& s : splits) {
+        const Node& nd = a->nodes[s.node];
+        const int32_t start = nd.pos0 + s.page * kPoolPage;
+        const int32_t* tok = a->tokens.data() + nd.tokens_at;
+        for (int32_t j = 0; j < nd.n_tokens; ++j)
+            if (a->info[tok[j]].limit > start) ++a->info[tok[j]].n_parts;
+        const int64_t rows = (int64_t)nd.n_tokens * group;
+        for (int64_t r = 0; r < rows; r += kTileRows) {
+            const int32_t n = (int32_t)std::min<int64_t>(kTileRows, rows - r);
+            int32_t sees = 0;
+            for (int64_t j = r / group; j <= (r + n - 1) / group; ++j) sees = std::max(sees, a->info[tok[j]].limit);
+            const int32_t pages = std::min(s.n_pages, pages_of(sees) - start / kPoolPage);
+            if (pages <= 0) continue;
+            a->items.push_back({nd.tokens_at, (int32_t)r, n, nd.pages_at + s.page, pages, start, (int32_t)s.part, nd.end});
+        }
+    }
+    std::stable_sort(a->items.begin(), a->items.end(), [](const Item& x, const Item& y) { return x.n_pages > y.n_pages; });
+    int32_t at = 0;
+    for (size_t r = 0; r < a->info.size(); ++r) {
+        Token& t = a->info[r];
+        t.part_at = at;
+        at += t.n_parts;
+        if (t.n_parts > 1) a->joins.push_back((int32_t)r);
+        t.n_parts = 0;
+    }
+    a->parts.resize(at);
+    for (const Split& s : splits) {
+        const Node& nd = a->nodes[s.node];
+        const int32_t start = nd.pos0 + s.page * kPoolPage;
+        for (int32_t j = 0; j < nd.n_tokens; ++j) {
+            Token& t = a->info[a->tokens[nd.tokens_at + j]];
+            if (t.limit > start) a->parts[t.part_at + t.n_parts++] = (int32_t)(s.part + (int64_t)j * group);
+        }
+    }
+    a->view.n_items = (int)a->items.size();
+    a->view.n_joins = (int)a->joins.size();
+    a->view.group = group;
+    a->view.n_kv = n_kv;
+    a->view.rows = (int)a->info.size();
+    a->view.part_ml = reinterpret_cast<float2*>((uintptr_t)part);   // their number; the caller places the arrays
 }
 
 extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, const int32_t* n_new, void* stream) {
@@ -153,18 +568,37 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
             entries += (int64_t)p->table[seqs[i]].size();
         }
         if (rows > (1 << 24) || entries > (1 << 28)) return bad("t2sx_plan_update: too many rows");
-        for (int32_t i = 0; i < n; ++i) {
-            if (p->mark[seqs[i]]) {
-                for (int32_t j = 0; j < i; ++j) p->mark[seqs[j]] = 0;
-                return bad("t2sx_plan_update: a sequence is given twice");
-            }
-            p->mark[seqs[i]] = 1;
-        }
+        bool twice = false;
+        for (int32_t i = 0; i < n; ++i) { twice |= p->mark[seqs[i]]; p->mark[seqs[i]] = 1; }
         for (int32_t i = 0; i < n; ++i) p->mark[seqs[i]] = 0;
+        if (twice) return bad("t2sx_plan_update: a sequence is given twice");
         a->ready = false;
+        a->shared_rows = false;
+        a->info.resize(rows);
+        a->row0.resize(n);
+        int32_t r = 0;
+        for (int32_t i = 0; i < n; ++i) {
+            a->row0[i] = r;
+            for (int32_t j = 0; j < n_new[i]; ++j, ++r) {
+                const int32_t limit = (int32_t)(p->len[seqs[i]] - n_new[i] + j + 1);
+                const int32_t page = p->table[seqs[i]][(limit - 1) / kPoolPage];
+                a->shared_rows |= p->users[page] > 1;
+                a->info[r] = Token{limit, page, 0, 0};
+            }
+        }
+        build_nodes(a, n, seqs, n_new);
+        build_items(a);
+        const int64_t n_parts = (int64_t)(uintptr_t)a->view.part_ml;
+        if (n_parts > INT32_MAX || a->parts.size() > (size_t)INT32_MAX || a->items.size() * p->n_kv > (size_t)INT32_MAX ||
+            a->joins.size() * (size_t)a->n_heads > (size_t)INT32_MAX)
+            return bad("t2sx_plan_update: too many rows");
+
         DeviceGuard dg;
         POOL_CK(dg.set(p->device));
-        const size_t bytes = (size_t)(2 * rows + entries) * 4;
+        size_t bytes = 0;
+        auto place = [&](auto const& v) { const size_t at = bytes; bytes = (bytes + v.size() * sizeof(v[0]) + 15) & ~(size_t)15; return at; };
+        const size_t o_info = place(a->info), o_items = place(a->items), o_tokens = place(a->tokens), o_pages = place(a->pages),
+                     o_parts = place(a->parts), o_joins = place(a->joins);
         const int b = a->turn ^= 1;
         POOL_CK(cudaEventSynchronize(a->sent[b]));
         if (a->host_bytes[b] < bytes) {
@@ -175,49 +609,80 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
             a->host_bytes[b] = bytes * 2;
         }
         POOL_CK(p->begin(st));
-        if (a->dev_bytes < bytes) {
-            POOL_CK(cudaEventSynchronize(p->done));
-            if (a->dev) POOL_CK(cudaFree(a->dev));
-            a->dev = nullptr;
-            a->dev_bytes = 0;
-            POOL_CK(cudaMalloc(&a->dev, bytes * 2));
-            a->dev_bytes = bytes * 2;
-        }
-        int32_t *limit = (int32_t*)a->host[b], *table_at = limit + rows, *table = table_at + rows;
-        int64_t r = 0, e = 0;
-        for (int32_t i = 0; i < n; ++i) {
-            const std::vector<int32_t>& t = p->table[seqs[i]];
-            for (int32_t j = 0; j < n_new[i]; ++j, ++r) {
-                limit[r] = (int32_t)(p->len[seqs[i]] - n_new[i] + j + 1);
-                table_at[r] = (int32_t)e;
-            }
-            std::copy(t.begin(), t.end(), table + e);
-            e += (int64_t)t.size();
-        }
+        auto grow = [&](uint8_t*& mem, size_t& have, size_t want) -> cudaError_t {
+            if (have >= want) return cudaSuccess;
+            cudaError_t e = cudaEventSynchronize(p->done);   // nothing of the plan runs any more
+            if (e == cudaSuccess && mem) e = cudaFree(mem);
+            mem = nullptr;
+            have = 0;
+            if (e == cudaSuccess) e = cudaMalloc(&mem, want + want / 2);
+            if (e == cudaSuccess) have = want + want / 2;
+            else cudaGetLastError();
+            return e;
+        };
+        POOL_CK(grow(a->dev, a->dev_bytes, bytes));
+        // results of parts, where tokens have several
+        const size_t part_rows = a->joins.empty() ? 0 : (size_t)n_parts * p->n_kv, o_bytes = part_rows * p->dim * 4;
+        POOL_CK(grow(a->work, a->work_bytes, o_bytes + part_rows * 8));
+        auto put = [&](size_t at, auto const& v) { if (!v.empty()) memcpy(a->host[b] + at, v.data(), v.size() * sizeof(v[0])); };
+        put(o_info, a->info); put(o_items, a->items); put(o_tokens, a->tokens); put(o_pages, a->pages); put(o_parts, a->parts);
+        put(o_joins, a->joins);
         if (bytes) POOL_CK(cudaMemcpyAsync(a->dev, a->host[b], bytes, cudaMemcpyHostToDevice, st));
         POOL_CK(cudaEventRecord(a->sent[b], st));
         POOL_CK(p->end(st));
-        const int32_t* d = (const int32_t*)a->dev;
-        a->view = RowView{d, d + rows, d + 2 * rows, (int)rows};
-        a->rows = (int)rows;
+        PlanView& w = a->view;
+        w.info = (const Token*)(a->dev + o_info);
+        w.items = (const Item*)(a->dev + o_items);
+        w.tokens = (const int32_t*)(a->dev + o_tokens);
+        w.pages = (const int32_t*)(a->dev + o_pages);
+        w.parts = (const int32_t*)(a->dev + o_parts);
+        w.joins = (const int32_t*)(a->dev + o_joins);
+        w.part_o = (float*)a->work;
+        w.part_ml = (float2*)(a->work + o_bytes);
         a->version = p->version;
         a->ready = true;
         return T2SX_OK;
     });
 }
 
+// With `early` the kernel may start while the one before it runs (it waits for it itself).
+template <typename... P, typename... A>
+static cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, bool early, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = threads;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = early ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
+
+template <typename T, int D>
+static cudaError_t launch_attend(t2sx_plan* a, const Tensors<T>& x, bool wrote, cudaStream_t st) {
+    const PlanView& w = a->view;
+    using S = TileShape<D>;
+    static std::once_flag once[64];
+    std::call_once(once[a->pool->device & 63],
+                   [] { cudaFuncSetAttribute(k_attend_tiles<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
+    cudaError_t e = launch(k_attend_tiles<T, D>, dim3((unsigned)(w.n_items * w.n_kv)), 32, S::SMEM, st, wrote, w, x);
+    if (e == cudaSuccess && w.n_joins)
+        e = launch(k_join_parts<T, D>, dim3((unsigned)(((long long)w.n_joins * a->n_heads + 3) / 4)), 128, 0, st, true, w, x);
+    return e;
+}
+
 template <typename T>
-static void launch_attend(t2sx_plan* a, size_t page0, const void* q, int64_t q_stride, float scale, void* out, int64_t out_stride,
-                          float* lse, cudaStream_t st) {
+static cudaError_t attend(t2sx_plan* a, size_t page0, const void* q, int64_t q_stride, float scale, void* out, int64_t out_stride,
+                          float* lse, bool wrote, cudaStream_t st) {
     t2sx_pool* p = a->pool;
-    const dim3 grid(a->rows, (a->n_heads + 3) / 4);
-    auto go = [&](auto kernel) {
-        kernel<<<grid, 128, 0, st>>>(a->view, (const T*)q, q_stride, (const T*)p->k, (const T*)p->v, page0, a->n_heads, p->n_kv,
-                                     scale, (T*)out, out_stride, lse);
-    };
-    if (p->dim == 32) go(k_attend_rows<T, 32>);
-    else if (p->dim == 64) go(k_attend_rows<T, 64>);
-    else go(k_attend_rows<T, 128>);
+    const size_t first = page0 * p->n_kv * kPoolPage * p->dim;
+    const Tensors<T> x = {(const T*)q, (const T*)p->k + first, (const T*)p->v + first, (T*)out, lse, q_stride, out_stride, scale * kLog2e};
+    if (p->dim == 32) return launch_attend<T, 32>(a, x, wrote, st);
+    if (p->dim == 64) return launch_attend<T, 64>(a, x, wrote, st);
+    return launch_attend<T, 128>(a, x, wrote, st);
 }
 
 extern "C" int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, int64_t q_stride, const void* k_new_dev,
@@ -229,7 +694,7 @@ extern "C" int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, 
     if (!a->ready || a->version != p->version)
         return t2sx_set_error(T2SX_ERR_STATE, "t2sx_plan_attend: the plan has no update since pages were released or moved");
     if (layer < 0 || layer >= p->n_layers) return bad("t2sx_plan_attend: layer out of range");
-    if (a->rows == 0) return T2SX_OK;
+    if (a->view.rows == 0) return T2SX_OK;
     if (!q_dev || !out_dev || !k_new_dev != !v_new_dev) return bad("t2sx_plan_attend: null q or out, or only one of k_new and v_new");
     if (!std::isfinite(scale)) return bad("t2sx_plan_attend: scale must be finite");
     const int64_t row = (int64_t)a->n_heads * p->dim, kv_row = (int64_t)p->n_kv * p->dim;
@@ -237,6 +702,8 @@ extern "C" int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, 
         return bad("t2sx_plan_attend: strides must be multiples of 8 and no less than a row");
     if (((uintptr_t)q_dev | (uintptr_t)out_dev | (uintptr_t)k_new_dev | (uintptr_t)v_new_dev) & 15 || ((uintptr_t)lse_dev & 3))
         return bad("t2sx_plan_attend: tensors must be 16-byte aligned");
+    if (k_new_dev && a->shared_rows)
+        return t2sx_set_error(T2SX_ERR_STATE, "t2sx_plan_attend: a row's position is in a page of several sequences, which is not written");
     cudaStream_t st = (cudaStream_t)stream;
     DeviceGuard dg;
     POOL_CK(dg.set(p->device));
@@ -244,14 +711,16 @@ extern "C" int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, 
     const size_t page0 = (size_t)layer * p->n_pages;
     if (k_new_dev) {
         const int row_vec = p->dim * 2 / 16;
-        const int64_t vecs = (int64_t)a->rows * p->n_kv * row_vec;
-        k_write_rows<<<(unsigned)((vecs + 255) / 256), 256, 0, st>>>(a->view, (const uint4*)k_new_dev, (const uint4*)v_new_dev,
-                                                                    kv_stride / 8, (uint4*)p->k, (uint4*)p->v, page0, p->n_kv, row_vec);
+        const int64_t vecs = (int64_t)a->view.rows * p->n_kv * row_vec;
+        const size_t first = page0 * p->n_kv * kPoolPage * row_vec;
+        k_write_rows<<<(unsigned)((vecs + 255) / 256), 256, 0, st>>>(a->view.info, a->view.rows, (const uint4*)k_new_dev,
+                                                                    (const uint4*)v_new_dev, kv_stride / 8, (uint4*)p->k + first,
+                                                                    (uint4*)p->v + first, p->n_kv, row_vec);
         POOL_CK(cudaGetLastError());
     }
-    if (p->type == T2SX_TYPE_F16) launch_attend<__half>(a, page0, q_dev, q_stride, scale, out_dev, out_stride, lse_dev, st);
-    else launch_attend<__nv_bfloat16>(a, page0, q_dev, q_stride, scale, out_dev, out_stride, lse_dev, st);
-    POOL_CK(cudaGetLastError());
+    const bool wrote = k_new_dev != nullptr;
+    if (p->type == T2SX_TYPE_F16) POOL_CK(attend<__half>(a, page0, q_dev, q_stride, scale, out_dev, out_stride, lse_dev, wrote, st));
+    else POOL_CK(attend<__nv_bfloat16>(a, page0, q_dev, q_stride, scale, out_dev, out_stride, lse_dev, wrote, st));
     POOL_CK(p->end(st));
     return T2SX_OK;
 }

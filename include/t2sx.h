@@ -308,7 +308,8 @@ T2SX_API int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, cons
  * q_dev, out_dev: [rows][n_heads][head_dim] of the pool's type, rows q_stride / out_stride
  * elements apart (multiples of 8); lse_dev: f32 [rows][n_heads] or null.  With k_new_dev and
  * v_new_dev ([rows][n_kv_heads][head_dim], rows kv_stride elements apart) the rows' keys and
- * values are first written to the cache; null: they are there already.  All 16-byte aligned.
+ * values are first written to the cache (T2SX_ERR_STATE if a row's position is in a page of several
+ * sequences); null: they are there already.  All 16-byte aligned.
  * Cache positions below a sequence's length must hold finite values; beyond it anything may stand.
  * Products are accumulated, and maxima and sums held, in f32; the softmax weights are rounded to
  * the pool's type before they multiply v, as the tensor cores take them. */

@@ -299,8 +299,11 @@ def test_attend_forked(t2sx_mod, dtype, heads, kv, dim, prompt, each):
     c.derive("fork", [i % 2 for i in cand], cand)
     for s in cand[1:]:
         c.extend(s, int(rng.integers(1, 200)))
+    grown = cand[1:]
     rng.shuffle(cand)
-    _attend(c, dtype, 0, cand, [1] * len(cand), heads, write=True, pad=8)
+    rng.shuffle(grown)
+    _attend(c, dtype, 0, cand, [1] * len(cand), heads)
+    _attend(c, dtype, 0, grown, [1] * len(grown), heads, write=True, pad=8)
 
 
 @gpu
@@ -325,7 +328,15 @@ def test_attend_forks_of_forks(t2sx_mod, dtype, heads, kv, dim):
     new = [int(rng.choice([0, 1, 1, 2, 9])) for _ in seqs]
     new[0] = 1
     _attend(c, dtype, 0, seqs, new, heads)
-    _attend(c, dtype, 0, seqs, new, heads, write=True)
+    # a row in a page of several sequences is not written; the rows behind those pages are
+    users = np.zeros(c.pool.n_pages, dtype=int)
+    for s in c.want:
+        users[c.pool.table([s])[0]] += 1
+    with pytest.raises(t2sx_mod.T2SXError) as e:
+        _attend(c, dtype, 0, [0, 1], [150, 1], heads, write=True)
+    assert e.value.code == t2sx_mod.ERR_STATE
+    own = [c.pool.length(s) - PAGE * int((users[c.pool.table([s])[0]] > 1).sum()) for s in seqs]
+    _attend(c, dtype, 0, seqs, [min(n, o) for n, o in zip(new, own)], heads, write=True)
 
 
 @gpu
