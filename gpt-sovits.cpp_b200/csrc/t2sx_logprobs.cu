@@ -32,9 +32,14 @@ __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162flo
 
 constexpr int kGroup = 4;            // 16-byte vectors that a thread has in flight
 constexpr int kCandidates = 1024;    // of one CTA (a warp's share of it for rows of one warp)
+constexpr int kHits = 512;           // slots of one CTA that candidates come from (a warp's share likewise)
 constexpr int kMaxTop = 32;
 constexpr int kMaxSplit = 8;         // CTAs per row (a portable cluster)
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kExtreme = 5e37f;    // maxima from here on (also below -5e37) leave the range of x log2(e)
+
+// What a thread subtracts from x log2(e): 0 while it has seen nothing.
+__device__ __forceinline__ float reference(float m) { return m > -INFINITY ? fminf(fmaxf(m, -kExtreme), kExtreme) * kLog2e : 0.0f; }
 
 // Value and id of a candidate as one key: greater keys come first (values descending, ids
 // ascending).  -inf and NaN have no place in a list.
@@ -86,22 +91,65 @@ struct Vec<float> {
     static __device__ __forceinline__ float2 pair(unsigned const (&w)[4], int i) {
         return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
     }
-    static __device__ __forceinline__ float max(const uint4& u) {
-        return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    static __device__ __forceinline__ void raise(uint4&) {}   // done to y instead
+    static constexpr float kLow = -kExtreme;
+    static __device__ __forceinline__ float max(const uint4 (&u)[kGroup]) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g)
+            m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(u[g].x), __uint_as_float(u[g].y)), fmaxf(__uint_as_float(u[g].z), __uint_as_float(u[g].w))));
+        return m;
     }
-    static __device__ __forceinline__ unsigned bits(const float* p) { return __float_as_uint(*p); }
+    // elements greater than a threshold, counted in the halves of acc
+    struct Count {
+        int n = 0;
+        __device__ __forceinline__ void add(const uint4& u, float above) {
+            n += (__uint_as_float(u.x) > above) + (__uint_as_float(u.y) > above) + (__uint_as_float(u.z) > above) + (__uint_as_float(u.w) > above);
+        }
+        __device__ __forceinline__ int sum() const { return n; }
+    };
+    // the greatest value of the type below x (not for -inf)
+    static __device__ __forceinline__ float below(float x) {
+        const unsigned b = __float_as_uint(x);
+        return __uint_as_float((b & 0x7FFFFFFFu) == 0 ? 0x80000001u : (b & 0x80000000u) ? b + 1 : b - 1);
+    }
 };
 template <>
 struct Vec<__half> {
     static constexpr int E = 8;
     static __device__ __forceinline__ uint4 none() { return make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u); }
     static __device__ __forceinline__ float2 pair(unsigned const (&w)[4], int i) { return __half22float2(*reinterpret_cast<const __half2*>(&w[i])); }
-    static __device__ __forceinline__ float max(const uint4& u) {
-        const __half2* h = reinterpret_cast<const __half2*>(&u);
-        const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    // the lowest finite value instead of -inf: as good as -inf unless the row's maximum is near it
+    static __device__ __forceinline__ void raise(uint4& u) {
+        __half2* h = reinterpret_cast<__half2*>(&u);
+        const __half2 low = __half2half2(__ushort_as_half(0xFBFFu));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], low);
+    }
+    static constexpr float kLow = -65000.0f;   // rows whose maximum is below have sums of their own
+    static __device__ __forceinline__ float max(const uint4 (&u)[kGroup]) {
+        __half2 m;
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+            const __half2* h = reinterpret_cast<const __half2*>(&u[g]);
+            const __half2 y = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            m = g ? __hmax2(m, y) : y;
+        }
         return fmaxf(__low2float(m), __high2float(m));
     }
-    static __device__ __forceinline__ unsigned bits(const __half* p) { return __half_as_ushort(*p); }
+    struct Count {   // ones added up in 16 bits: exact up to 256, and a group has 16 for each half
+        __half2 acc = __float2half2_rn(0.0f);
+        __device__ __forceinline__ void add(const uint4& u, float above) {
+            const __half2 *h = reinterpret_cast<const __half2*>(&u), a = __float2half2_rn(above);
+            acc = __hadd2(acc, __hadd2(__hadd2(__hgt2(h[0], a), __hgt2(h[1], a)), __hadd2(__hgt2(h[2], a), __hgt2(h[3], a))));
+        }
+        __device__ __forceinline__ int sum() const { return (int)(__low2float(acc) + __high2float(acc)); }
+    };
+    static __device__ __forceinline__ float below(float x) {
+        const unsigned b = __half_as_ushort(__float2half_rn(x));
+        const unsigned short r = (unsigned short)((b & 0x7FFFu) == 0 ? 0x8001u : (b & 0x8000u) ? b + 1 : b - 1);
+        return __half2float(__ushort_as_half(r));
+    }
 };
 template <>
 struct Vec<__nv_bfloat16> {
@@ -110,12 +158,36 @@ struct Vec<__nv_bfloat16> {
     static __device__ __forceinline__ float2 pair(unsigned const (&w)[4], int i) {
         return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
     }
-    static __device__ __forceinline__ float max(const uint4& u) {
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
-        const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    static __device__ __forceinline__ void raise(uint4& u) {   // to -2^127, whose product with log2(e) is finite
+        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+        const __nv_bfloat162 low = __bfloat162bfloat162(__ushort_as_bfloat16(0xFF00u));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], low);
+    }
+    static constexpr float kLow = -kExtreme;
+    static __device__ __forceinline__ float max(const uint4 (&u)[kGroup]) {
+        __nv_bfloat162 m;
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u[g]);
+            const __nv_bfloat162 y = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+            m = g ? __hmax2(m, y) : y;
+        }
         return fmaxf(__low2float(m), __high2float(m));
     }
-    static __device__ __forceinline__ unsigned bits(const __nv_bfloat16* p) { return __bfloat16_as_ushort(*p); }
+    struct Count {   // ones added up in 16 bits: exact up to 256, and a group has 16 for each half
+        __nv_bfloat162 acc = __float2bfloat162_rn(0.0f);
+        __device__ __forceinline__ void add(const uint4& u, float above) {
+            const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162*>(&u), a = __float2bfloat162_rn(above);
+            acc = __hadd2(acc, __hadd2(__hadd2(__hgt2(h[0], a), __hgt2(h[1], a)), __hadd2(__hgt2(h[2], a), __hgt2(h[3], a))));
+        }
+        __device__ __forceinline__ int sum() const { return (int)(__low2float(acc) + __high2float(acc)); }
+    };
+    static __device__ __forceinline__ float below(float x) {
+        const unsigned b = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+        const unsigned short r = (unsigned short)((b & 0x7FFFu) == 0 ? 0x8001u : (b & 0x8000u) ? b + 1 : b - 1);
+        return __bfloat162float(__ushort_as_bfloat16(r));
+    }
 };
 
 // A slot's maximum in 16 bits, never below it (the upper half of an f32, rounded up).
@@ -180,7 +252,8 @@ template <int WARPS>
 struct Shared {   // of one row's threads in a CTA
     Stat stat[WARPS];
     float best_max[WARPS][32];
-    int count;
+    int count, n_hits;
+    unsigned short hits[WARPS == 1 ? kHits / 4 : kHits];   // slots that reach T0: number x threads + thread
     unsigned long long best[WARPS];
     static constexpr int PARTS = WARPS == 1 ? 1 : kMaxSplit;
     Stat joined[PARTS];                                  // in the first CTA of a row: all of its CTAs'
@@ -191,10 +264,10 @@ struct Shared {   // of one row's threads in a CTA
 // WARPS == 1: a warp per row, four rows in a CTA.  Else a row per CTA, or per cluster of `split` CTAs:
 // each takes a range of the row's vectors, and the first one joins what they found.
 template <typename T, int WARPS>
-__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS)
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS, WARPS == 1 ? 6 : 4)
 k_logprobs(const T* __restrict__ logits, Args a) {
     constexpr int E = Vec<T>::E, N = 32 * WARPS, ROWS = WARPS == 1 ? 4 : 1;
-    constexpr int CAND = WARPS == 1 ? kCandidates / 4 : kCandidates;
+    constexpr int CAND = WARPS == 1 ? kCandidates / 4 : kCandidates, HITS = WARPS == 1 ? kHits / 4 : kHits;
     extern __shared__ __align__(16) unsigned char raw[];
     const int sub = WARPS == 1 ? threadIdx.x >> 5 : 0, tid = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
     const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
@@ -211,44 +284,35 @@ k_logprobs(const T* __restrict__ logits, Args a) {
     const int t = a.tokens[row];
     const bool given = t >= 0 && t < a.vocab;
 
-    // The row on the grid of aligned vectors: the first and last ones may be partly outside it.
+    // The row on the grid of aligned vectors, and the elements before and after its whole ones: those are
+    // fewer than E each, and one thread takes one.
     const int off = (int)(((uintptr_t)x & 15) / sizeof(T));
-    const int n_vec = (int)(((long long)off + a.vocab + E - 1) / E);
-    const int per = (n_vec + split - 1) / split, v0 = part * per, v1 = min(n_vec, v0 + per);
     const uint4* xv = reinterpret_cast<const uint4*>(x - off);
-    auto load = [&](int v) -> uint4 {
-        if (v >= v1) return Vec<T>::none();
-        const int j = v * E - off;
-        if (j >= 0 && j + E <= a.vocab) return xv[v];
-        uint4 u = Vec<T>::none();
-        unsigned* w = reinterpret_cast<unsigned*>(&u);
-        for (int e = 0; e < E; ++e) {
-            if (j + e < 0 || j + e >= a.vocab) continue;
-            const unsigned b = Vec<T>::bits(x + j + e);
-            if (E == 4) w[e] = b;
-            else w[e / 2] = (e & 1) ? (w[e / 2] & 0x0000FFFFu) | b << 16 : (w[e / 2] & 0xFFFF0000u) | b;
-        }
-        return u;
-    };
+    const int full0 = off ? 1 : 0, full1 = max(full0, (int)(((long long)off + a.vocab) / E));
+    const int per = (full1 - full0 + split - 1) / split, v0 = full0 + part * per, v1 = min(full1, v0 + per);
+    int edge = tid < E ? tid : full1 * E - off + tid - E;   // its id
+    if (tid < E ? part != 0 || edge >= min(a.vocab, full0 * E - off) : part != split - 1 || tid >= 2 * E || edge < 0) edge = a.vocab;
+    auto load = [&](int v) -> uint4 { return v < v1 ? __ldg(xv + v) : Vec<T>::none(); };
 
     uint4 u[kGroup];
 #pragma unroll
     for (int g = 0; g < kGroup; ++g) u[g] = load(v0 + g * N + tid);
-    const float xt = given ? to_f32(x[t]) : INFINITY;
+    const float edge_x = edge < a.vocab ? to_f32(x[edge]) : -INFINITY;
+    const float xt = given ? to_f32(x[t]) : INFINITY, xt_below = Vec<T>::below(xt);
     unsigned short* slots = reinterpret_cast<unsigned short*>(raw + ROWS * sizeof(Shared<WARPS>));
     int n_slots = 0;
-    float m = -INFINITY, slot = -INFINITY;
-    float2 s = {0.0f, 0.0f}, w = {0.0f, 0.0f};
-    int before = 0;
+    // the edge's element is the first one of the thread: 1 for its weight, NaN for NaN and +inf
+    float m = fmaxf(edge_x, -INFINITY), ref = reference(m), slot = -INFINITY;
+    float2 s = {edge_x == -INFINITY ? 0.0f : edge_x - edge_x + 1.0f, 0.0f}, w = {0.0f, 0.0f};
+    int before = edge < a.vocab && (edge_x > xt || (edge_x == xt && edge < t));
     for (int base = v0, group = 0; base < v1; base += kGroup * N) {
         uint4 c[kGroup];
-        float g_max = -INFINITY;
 #pragma unroll
         for (int g = 0; g < kGroup; ++g) {
             c[g] = u[g];
             u[g] = load(base + (kGroup + g) * N + tid);
-            g_max = fmaxf(g_max, Vec<T>::max(c[g]));
         }
+        const float g_max = Vec<T>::max(c);
         slot = fmaxf(slot, g_max);
         if (++group == a.slot_groups) {
             slots[(n_slots++ * ROWS + sub) * N + tid] = slot_up(slot);
@@ -256,55 +320,63 @@ k_logprobs(const T* __restrict__ logits, Args a) {
             group = 0;
         }
         if (g_max > m) {
+            const float up = reference(g_max);
             if (m > -INFINITY) {
-                const float d = fmaxf(m - g_max, -1e30f), f = ex2(d * kLog2e);
+                const float d = fmaxf(ref - up, -1e30f), f = ex2(d);
                 w = mul2(make_float2(f, f), fma2(make_float2(d, d), s, w));
                 s = mul2(make_float2(f, f), s);
             }
             m = g_max;
+            ref = up;
         }
-        // x - m is exact or rounded once, also where x and m are the lowest values of the type; -inf becomes a
-        // finite number with the weight 0, and NaN (of +inf, too) stays in the sums
-        const float neg = m > -INFINITY ? -m : 0.0f;
+        if (g_max >= xt) {
+            typename Vec<T>::Count more;
+#pragma unroll
+            for (int g = 0; g < kGroup; ++g) {
+                const int vec = base + g * N + tid, j = vec * E - off;
+                if ((j + E <= t || j > t) && xt > -INFINITY) {
+                    // up to the token equal values come before it, too
+                    more.add(c[g], j > t ? xt : xt_below);
+                } else if (vec < v1) {
+                    const unsigned b[4] = {c[g].x, c[g].y, c[g].z, c[g].w};
+#pragma unroll
+                    for (int i = 0; i < E; ++i) {
+                        const float2 p = Vec<T>::pair(b, i / 2);
+                        const float v = (i & 1) ? p.y : p.x;
+                        before += v > xt || (v == xt && j + i < t);
+                    }
+                }
+            }
+            before += more.sum();
+        }
+        // y = x log2(e) - ref, rounded once; what lies below the floor has the weight 0 in finite numbers, and NaN
+        // stays in the sums
 #pragma unroll
         for (int g = 0; g < kGroup; ++g) {
+            Vec<T>::raise(c[g]);
             const unsigned b[4] = {c[g].x, c[g].y, c[g].z, c[g].w};
 #pragma unroll
             for (int i = 0; i < E / 2; ++i) {
-                float2 d = add2(Vec<T>::pair(b, i), make_float2(neg, neg));
-                d.x = max_nan(d.x, -1e30f);
-                d.y = max_nan(d.y, -1e30f);
-                const float2 y = mul2(d, make_float2(kLog2e, kLog2e));
+                float2 y = fma2(Vec<T>::pair(b, i), make_float2(kLog2e, kLog2e), make_float2(-ref, -ref));
+                if (E == 4) { y.x = max_nan(y.x, -1e30f); y.y = max_nan(y.y, -1e30f); }
                 const float2 e = make_float2(ex2(y.x), ex2(y.y));
                 s = add2(s, e);
-                w = fma2(e, d, w);
-            }
-        }
-        if (g_max >= xt) {   // seldom, for a token that is likely
-#pragma unroll
-            for (int g = 0; g < kGroup; ++g) {
-                const unsigned b[4] = {c[g].x, c[g].y, c[g].z, c[g].w};
-                const int vec = base + g * N + tid, j = vec * E - off;
-                if (vec >= v1) break;
-#pragma unroll
-                for (int i = 0; i < E; ++i) {   // (the -inf in front of the row equals a masked token's logit)
-                    const float2 p = Vec<T>::pair(b, i / 2);
-                    const float v = (i & 1) ? p.y : p.x;
-                    before += v > xt || (v == xt && j + i < t && j + i >= 0);
-                }
+                w = fma2(e, y, w);
             }
         }
         if (base + kGroup * N >= v1 && group) slots[(n_slots++ * ROWS + sub) * N + tid] = slot_up(slot);
     }
 
-    // this thread's part, then the warp's, then the CTA's
-    Stat st = warp_join(Stat{m, s.x + s.y, w.x + w.y, before});
+    // this thread's part relative to m itself (ref is a rounded number), then the warp's, then the CTA's
+    const float rest = fabsf(m) < kExtreme ? fmaf(m, kLog2e, -ref) : 0.0f, back = ex2(-rest);
+    const float s1 = s.x + s.y;
+    Stat st = warp_join(Stat{m, s1 * back, kLn2 * back * fmaf(-rest, s1, w.x + w.y), before});
     // T0: the top_k-th greatest of the threads' maxima, so at least top_k elements reach it (-inf: fewer than
     // top_k threads have an element above -inf)
     float T0 = a.top_k ? warp_sort(m) : -INFINITY;
     if constexpr (WARPS > 1) {
         if (lane == 0) sh.stat[warp] = st;
-        if (tid == 0) sh.count = 0;
+        if (tid == 0) sh.count = sh.n_hits = 0;
         if (a.top_k) {
             sh.best_max[warp][lane] = T0;
             for (int h = WARPS / 2; h; h /= 2) {   // the 32 greatest of two lists, again in order
@@ -326,33 +398,72 @@ k_logprobs(const T* __restrict__ logits, Args a) {
         if (a.top_k) T0 = sh.best_max[0][a.top_k - 1];
     } else {
         if (a.top_k) T0 = __shfl_sync(~0u, T0, a.top_k - 1);
-        if (lane == 0) sh.count = 0;
+        if (lane == 0) sh.count = sh.n_hits = 0;
         __syncwarp();
     }
 
+    if (st.m > -INFINITY && (st.m < Vec<T>::kLow || st.m > kExtreme)) {
+        // a maximum near the ends of the type's range: the sums anew, from x - m
+        float ss = 0.0f, sw = 0.0f;
+        auto add = [&](float v) {
+            const float d = max_nan(v - st.m, -1e30f), e = ex2(d * kLog2e);
+            ss += e;
+            sw = fmaf(e, d, sw);
+        };
+        add(edge_x);
+        for (int v = v0 + tid; v < v1; v += N) {
+            const uint4 q = load(v);
+            const unsigned b[4] = {q.x, q.y, q.z, q.w};
+            for (int i = 0; i < E / 2; ++i) {
+                const float2 p = Vec<T>::pair(b, i);
+                add(p.x);
+                add(p.y);
+            }
+        }
+        for (int y = 16; y; y >>= 1) { ss += __shfl_xor_sync(~0u, ss, y); sw += __shfl_xor_sync(~0u, sw, y); }
+        if constexpr (WARPS > 1) {
+            __syncthreads();   // everyone has read the warps' parts
+            if (lane == 0) { sh.stat[warp].s = ss; sh.stat[warp].w = sw; }
+            __syncthreads();
+            ss = sw = 0.0f;
+            for (int i = 0; i < WARPS; ++i) { ss += sh.stat[i].s; sw += sh.stat[i].w; }
+        }
+        st.s = ss;
+        st.w = sw;
+    }
     if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (a.top_k) {
         // the elements that reach T0, from the slots that do (each thread reads its own)
+        if (edge_x >= T0 && edge_x > -INFINITY) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < CAND) sh.cand[at] = order_key(edge_x, edge);
+        }
         for (int k = 0; k < n_slots; ++k) {
             if (!(slot_value(slots[(k * ROWS + sub) * N + tid]) >= T0)) continue;
-            for (int g = 0; g < kGroup * a.slot_groups; ++g) {
-                const int v = v0 + (k * kGroup * a.slot_groups + g) * N + tid;
-                if (v >= v1) break;
+            const int at = atomicAdd(&sh.n_hits, 1);
+            if (at < HITS) sh.hits[at] = (unsigned short)(k * N + tid);
+        }
+        sync();
+        // their vectors, shared out anew: one round trip to L2 for all of them
+        const int n_hits = min(sh.n_hits, HITS) * kGroup;
+        for (int sg = 0; sg < a.slot_groups; ++sg)
+            for (int i = tid; i < n_hits; i += N) {
+                const int hit = sh.hits[i / kGroup];
+                const int v = v0 + ((hit / N * a.slot_groups + sg) * kGroup + i % kGroup) * N + hit % N;
                 const uint4 q = load(v);
                 const unsigned b[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const float2 p = Vec<T>::pair(b, i / 2);
-                    const float y = (i & 1) ? p.y : p.x;
+                for (int e = 0; e < E; ++e) {
+                    const float2 p = Vec<T>::pair(b, e / 2);
+                    const float y = (e & 1) ? p.y : p.x;
                     if (y >= T0 && y > -INFINITY) {
                         const int at = atomicAdd(&sh.count, 1);
-                        if (at < CAND) sh.cand[at] = order_key(y, v * E - off + i);
+                        if (at < CAND) sh.cand[at] = order_key(y, v * E - off + e);
                     }
                 }
             }
-        }
         sync();
-        const int n = sh.count;
+        const int n = sh.n_hits > HITS ? CAND + 1 : sh.count;
         unsigned long long* list = sh.lists[0];
         if (split > 1) {   // in the first CTA of the row
             unsigned long long* mine = sh.lists[part];
@@ -365,6 +476,7 @@ k_logprobs(const T* __restrict__ logits, Args a) {
             for (int i = tid; i < n; i += N) {
                 const unsigned long long key = sh.cand[i];
                 int place = 0;
+#pragma unroll 4
                 for (int j = 0; j < n; ++j) place += sh.cand[j] > key;
                 if (place < a.top_k) list[place] = key;
             }
@@ -372,7 +484,8 @@ k_logprobs(const T* __restrict__ logits, Args a) {
             // more ties than the list of candidates holds: place by place, the greatest key below the last one
             unsigned long long last = ~0ull;
             for (int i = 0; i < a.top_k && last; ++i) {
-                unsigned long long best = 0;
+                unsigned long long best = edge_x > -INFINITY ? order_key(edge_x, edge) : 0;
+                if (best >= last) best = 0;
                 for (int v = v0 + tid; v < v1; v += N) {
                     const uint4 q = load(v);
                     const unsigned b[4] = {q.x, q.y, q.z, q.w};
@@ -420,17 +533,16 @@ k_logprobs(const T* __restrict__ logits, Args a) {
         if (a.entropy) a.entropy[row] = bad ? NAN : st.s > 0.0f ? log_s - st.w / st.s : 0.0f;
         if (a.rank) a.rank[row] = given ? st.before : -1;
     }
-    // the parts' lists, each in order: an entry's place is the number of greater ones
-    const int n = split * a.top_k;
-    for (int i = tid; i < n; i += N) {
-        const unsigned long long key = sh.lists[i / a.top_k][i % a.top_k];
-        int place = i % a.top_k;
-        if (split > 1) {
-            place = 0;
-            for (int j = 0; j < n; ++j) {
-                const unsigned long long o = sh.lists[j / a.top_k][j % a.top_k];
-                place += o > key || (o == key && j < i);   // empty entries are equal
-            }
+    // the parts' lists, each in order: an entry's place is the number of greater ones (empty ones: of earlier ones)
+    for (int i = tid; i < split * kMaxTop; i += N) {
+        const int mine = i / kMaxTop, at = i % kMaxTop;
+        if (at >= a.top_k) continue;
+        const unsigned long long key = sh.lists[mine][at];
+        int place = at;
+        for (int q = 0; q < split; ++q) {
+            if (q == mine) continue;
+#pragma unroll 4
+            for (int j = 0; j < a.top_k; ++j) place += sh.lists[q][j] > key || (key == 0 && q < mine);
         }
         if (place < a.top_k) {
             const unsigned id = 0xFFFFFFFFu - (unsigned)key;
@@ -444,7 +556,7 @@ template <typename T, int WARPS>
 cudaError_t launch(const T* x, Args a, int split, cudaStream_t st) {
     constexpr int N = 32 * WARPS, ROWS = WARPS == 1 ? 4 : 1;
     // slots of 16 bits: at most 32 KB of them, so that a CTA's share of shared memory stays small
-    const long long vecs = ((long long)a.vocab / Vec<T>::E + 2 + split - 1) / split;
+    const long long vecs = ((long long)a.vocab / Vec<T>::E + 1 + split - 1) / split;
     const long long groups = (vecs + (long long)kGroup * N - 1) / ((long long)kGroup * N);
     const int most = (32 << 10) / (2 * N * ROWS);
     a.slot_groups = (int)((groups + most - 1) / most);
@@ -476,7 +588,7 @@ cudaError_t dispatch(const T* x, const Args& a, cudaStream_t st) {
     if (a.vocab <= 2048) return launch<T, 1>(x, a, 1, st);
     int split = 1;
     while (split < kMaxSplit && (long long)a.rows * split * 2 <= 296 && a.vocab / (2 * split) >= 4096) split *= 2;
-    return launch<T, 16>(x, a, split, st);
+    return launch<T, 8>(x, a, split, st);
 }
 
 int bad(const char* m) { return t2sx_set_error(T2SX_ERR_INVALID, m); }

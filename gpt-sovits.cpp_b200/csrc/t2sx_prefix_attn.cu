@@ -25,6 +25,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kWeightExp = 7.0f;   // c above: weights are at most 2^7
 constexpr int kTileRows = 16;        // rows of a warp's tile (the m of mma.m16n8k16)
+constexpr int kMinChunk = 2;         // pages of a split at least
+constexpr int kWarpJoin = 8;         // parts of a token up to which the last item joins them
 
 // A tile of rows against a range of a node's pages.
 struct Item {
@@ -33,33 +35,43 @@ struct Item {
     int32_t pages_at;    // page ids
     int32_t n_pages;
     int32_t pos0;        // position of the first page's first key
-    int32_t part;        // row r's part is number part + r
+    int32_t split;       // which range of the node's pages this is
     int32_t end;         // the node's filled positions end here
+    int32_t new_pos;     // from this position on the keys are the step's own (of one sequence) ...
+    int32_t new_row;     // ... and that one is this row of the step
+    int32_t pad[2];
 };
 
-struct Token {
+// A token as one of a node's: what it is, and where its parts are.  A token's parts are numbers
+// part_at .. part_at + n_parts - 1, those of the node's splits from part0 on.
+struct alignas(16) Token {
+    int32_t row;         // of the step
     int32_t limit;       // positions that it sees; its own is the last of them
     int32_t page;        // page of its own position
-    int32_t part_at;     // its parts' numbers (of its first head) start here in `parts`
+    int32_t part0, part_at;
     int32_t n_parts;     // one: the item writes the result itself
+    int32_t arrivals;    // items that hold some of its heads' parts, for each K/V head
+    int32_t pad;
 };
 
 struct PlanView {
-    const Token* info;       // [rows of the step]
-    const int32_t* tokens;   // nodes' tokens, as rows of the step
+    const Token* tokens;     // nodes' tokens
     const int32_t* pages;
     const Item* items;
-    const int32_t* parts;
-    const int32_t* joins;    // tokens of several parts
-    float* part_o;           // [part][K/V head][dim]
-    float2* part_ml;         // [part][K/V head]
+    const Token* joins;      // tokens of several parts
+    float* part_o;           // [part][query head of the group][K/V head][dim]
+    float2* part_ml;         // [part][query head of the group][K/V head]
+    int32_t* arrived;        // [row][K/V head] items that are done; null: a second kernel joins the parts
     int rows, n_items, n_joins, group, n_kv;
 };
 
 // Strided tensors of one call.
 template <typename T>
 struct Tensors {
-    const T *q, *k, *v;      // k, v: the layer's first page
+    const T* q;
+    T *k, *v;                // the layer's first page
+    const T *k_new, *v_new;  // the rows' own keys and values, or null: they are in the cache
+    long long kv_stride;
     T* out;
     float* lse;
     long long q_stride, out_stride;
@@ -97,8 +109,9 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void cp16(uint32_t smem, const void* gmem) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+// 16 bytes, or as many zeros
+__device__ __forceinline__ void cp16(uint32_t smem, const void* gmem, bool real = true) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(real ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -106,25 +119,10 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 __device__ __forceinline__ void dependents_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// One 16-byte word per thread: the rows' keys and values go to their positions.
-__global__ void __launch_bounds__(256)
-k_write_rows(const Token* __restrict__ info, int rows, const uint4* __restrict__ kn, const uint4* __restrict__ vn,
-             long long stride_vec, uint4* __restrict__ k, uint4* __restrict__ v, int n_kv, int row_vec) {
-    dependents_launch();
-    const int per_row = n_kv * row_vec;
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (long long)rows * per_row) return;
-    const int row = (int)(i / per_row), j = (int)(i - (long long)row * per_row), h = j / row_vec, c = j - h * row_vec;
-    const Token t = info[row];
-    const size_t dst = (((size_t)t.page * n_kv + h) * kPoolPage + (t.limit - 1) % kPoolPage) * row_vec + c;
-    k[dst] = kn[row * stride_vec + j];
-    v[dst] = vn[row * stride_vec + j];
-}
-
 // Tiles of a head dimension: keys per stage of the ring and stages.
 template <int D>
 struct TileShape {
-    static constexpr int KEYS = D == 32 ? 64 : 32, STAGES = 3;
+    static constexpr int KEYS = D == 32 ? 64 : 32, STAGES = D == 32 ? 2 : 3;
     static constexpr int HALF = KEYS * D * 2;   // bytes of a stage's K (or V)
     static constexpr int SMEM = STAGES * 2 * HALF;
 };
@@ -135,6 +133,47 @@ template <int D>
 __device__ __forceinline__ uint32_t tile_at(int row, int c) {
     if constexpr (D == 32) return row * 64 + ((c ^ (row >> 1)) & 3) * 16;
     else return row * (D * 2) + ((c & ~7) | ((c ^ row) & 7)) * 16;
+}
+
+// The parts of one token's query head, in their order whoever joins them: the warp's lanes are D / 4 columns of
+// four dims x 32 / (D / 4) parts.  Parts were written by other SMs in this or the previous launch (L2 loads).
+template <typename T, int D>
+__device__ __forceinline__ void join_row(const PlanView& pv, const Tensors<T>& x, int row, int part_at, int n_parts,
+                                         int head) {
+    constexpr int COLS = D / 4, LANES = 32 / COLS;
+    const int lane = threadIdx.x & 31, kvh = head / pv.group, g = head % pv.group;
+    auto part = [&](int i) { return ((size_t)(part_at + i) * pv.group + g) * pv.n_kv + kvh; };
+    float M = -INFINITY;
+    for (int i = lane; i < n_parts; i += 32) M = fmaxf(M, __ldcg(&pv.part_ml[part(i)]).x);
+    for (int y = 16; y; y >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, y));
+    float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+#pragma unroll 2
+    for (int i = lane / COLS; i < n_parts; i += LANES) {
+        const size_t at = part(i);
+        const float2 ml = __ldcg(&pv.part_ml[at]);
+        const float4 o = __ldcg(reinterpret_cast<const float4*>(pv.part_o + at * D) + lane % COLS);
+        const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+        l = fmaf(f, ml.y, l);
+        acc.x = fmaf(f, o.x, acc.x);
+        acc.y = fmaf(f, o.y, acc.y);
+        acc.z = fmaf(f, o.z, acc.z);
+        acc.w = fmaf(f, o.w, acc.w);
+    }
+#pragma unroll
+    for (int y = COLS; y < 32; y <<= 1) {
+        l += __shfl_xor_sync(~0u, l, y);
+        acc.x += __shfl_xor_sync(~0u, acc.x, y);
+        acc.y += __shfl_xor_sync(~0u, acc.y, y);
+        acc.z += __shfl_xor_sync(~0u, acc.z, y);
+        acc.w += __shfl_xor_sync(~0u, acc.w, y);
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    if (lane < COLS)
+        reinterpret_cast<uint2*>(x.out + row * x.out_stride + head * D)[lane] =
+            make_uint2(pack2(T(), acc.x * inv, acc.y * inv), pack2(T(), acc.z * inv, acc.w * inv));
+    if (x.lse && lane == 0)
+        x.lse[(size_t)row * (pv.n_kv * pv.group) + head] = l > 0.0f ? (M - kWeightExp + log2f(l)) * kLn2 : -INFINITY;
 }
 
 // One warp per (item, K/V head): at most 16 rows, keys streamed through a ring of its own.
@@ -163,29 +202,44 @@ k_attend_tiles(PlanView pv, Tensors<T> x) {
             const size_t at = (((size_t)page * pv.n_kv + kvh) * kPoolPage + sub * S::KEYS) * D;
             const uint32_t dst = ring0 + (t % S::STAGES) * 2 * S::HALF;
             const char *ks = reinterpret_cast<const char*>(x.k + at), *vs = reinterpret_cast<const char*>(x.v + at);
+            const int pos = it.pos0 + t * S::KEYS;
+            const bool plain = pos + S::KEYS <= min(it.end, x.k_new ? it.new_pos : INT32_MAX);
 #pragma unroll
             for (int i = 0; i < S::HALF / 512; ++i) {
                 const int c = i * 32 + lane;
-                const uint32_t d = tile_at<D>(c / (D / 8), c % (D / 8));
-                cp16(dst + d, ks + c * 16);
-                cp16(dst + S::HALF + d, vs + c * 16);
+                const uint32_t d = dst + tile_at<D>(c / (D / 8), c % (D / 8));
+                if (plain) {
+                    cp16(d, ks + c * 16);
+                    cp16(d + S::HALF, vs + c * 16);
+                } else {
+                    // the step's own keys come from the call's tensors; what stands beyond the filled positions may
+                    // be anything, and counts as zeros
+                    const int at_pos = pos + c / (D / 8);
+                    const bool real = at_pos < it.end, own = x.k_new && real && at_pos >= it.new_pos;
+                    const long long off = (it.new_row + at_pos - it.new_pos) * x.kv_stride + kvh * D + (c % (D / 8)) * 8;
+                    cp16(d, own ? reinterpret_cast<const char*>(x.k_new + off) : ks + c * 16, real);
+                    cp16(d + S::HALF, own ? reinterpret_cast<const char*>(x.v_new + off) : vs + c * 16, real);
+                }
             }
         }
         cp_commit();
     };
 
     // rows lane / 4 and lane / 4 + 8
-    int row_of[2], head_of[2], limit[2];
+    int row_of[2], head_of[2], limit[2], n_parts[2];
+    size_t part[2];
     bool live[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int r = lane / 4 + 8 * i, mr = it.row0 + r;
+        const int r = lane / 4 + 8 * i, mr = it.row0 + r, g = mr % group;
         live[i] = r < it.rows;
-        row_of[i] = live[i] ? pv.tokens[it.tokens_at + mr / group] : 0;
-        head_of[i] = kvh * group + mr % group;
-        limit[i] = live[i] ? pv.info[row_of[i]].limit : 0;
+        const Token t = pv.tokens[it.tokens_at + (live[i] ? mr / group : 0)];
+        row_of[i] = t.row;
+        head_of[i] = kvh * group + g;
+        limit[i] = live[i] ? t.limit : 0;
+        n_parts[i] = t.n_parts;
+        part[i] = ((size_t)(t.part0 + it.split) * group + g) * pv.n_kv + kvh;
     }
-    dependents_wait();   // the step's own keys and values
     for (int t = 0; t < S::STAGES - 1; ++t) request(t);
     uint32_t qf[KS][4];
 #pragma unroll
@@ -197,6 +251,23 @@ k_attend_tiles(PlanView pv, Tensors<T> x) {
             qf[k][i + 2] = live[i] ? src[k * 8 + 4 + lane % 4] : 0;
         }
     }
+    // The item with a token's own position writes its key and value to the cache: read here, written after
+    // the tiles for the first token (a decode step's only one).
+    auto own = [&](int r) -> const Token* {
+        const Token* t = pv.tokens + it.tokens_at + (it.row0 + r) / group;
+        return x.k_new && r < it.rows && (it.row0 + r) % group == 0 && t->limit > it.pos0 &&
+               t->limit <= it.pos0 + it.n_pages * kPoolPage && lane < D / 4 ? t : nullptr;
+    };
+    auto own_src = [&](const Token* t) {
+        return reinterpret_cast<const uint4*>((lane >= D / 8 ? x.v_new : x.k_new) + t->row * x.kv_stride + kvh * D) + lane % (D / 8);
+    };
+    auto own_dst = [&](const Token* t) {
+        return reinterpret_cast<uint4*>((lane >= D / 8 ? x.v : x.k) +
+                                        (((size_t)t->page * pv.n_kv + kvh) * kPoolPage + (t->limit - 1) % kPoolPage) * D) + lane % (D / 8);
+    };
+    const Token* own0 = own(0);
+    uint4 own_word = make_uint4(0, 0, 0, 0);
+    if (own0) own_word = *own_src(own0);
     // the smallest limit of the rows: keys below it need no mask
     int free_to = min(live[0] ? limit[0] : INT32_MAX, live[1] ? limit[1] : INT32_MAX);
     for (int y = 16; y; y >>= 1) free_to = min(free_to, __shfl_xor_sync(~0u, free_to, y));
@@ -208,11 +279,6 @@ k_attend_tiles(PlanView pv, Tensors<T> x) {
         __syncwarp();
         const uint32_t kt = ring0 + (t % S::STAGES) * 2 * S::HALF, vt = kt + S::HALF;
         const int pos = it.pos0 + t * S::KEYS;
-        if (pos + S::KEYS > it.end) {   // what stands beyond the filled positions may be NaN: as values it counts 0
-            for (int c = max(0, it.end - pos) * (D / 8) + lane; c < S::KEYS * (D / 8); c += 32)
-                *reinterpret_cast<uint4*>(ring + (vt - ring0) + tile_at<D>(c / (D / 8), c % (D / 8))) = make_uint4(0, 0, 0, 0);
-            __syncwarp();
-        }
         float s[NT][4] = {};
 #pragma unroll
         for (int n = 0; n < NT; n += 2)
@@ -284,13 +350,16 @@ k_attend_tiles(PlanView pv, Tensors<T> x) {
     }
     cp_wait<0>();
     dependents_launch();
+    if (own0) *own_dst(own0) = own_word;
+    for (int r = 1; r < it.rows; ++r)
+        if (const Token* t = own(r)) *own_dst(t) = *own_src(t);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         float sum = l[i];
         sum += __shfl_xor_sync(~0u, sum, 1);
         sum += __shfl_xor_sync(~0u, sum, 2);
         if (!live[i] || limit[i] <= it.pos0) continue;   // such a row has no part here
-        if (pv.info[row_of[i]].n_parts == 1) {
+        if (n_parts[i] == 1) {
             const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
             uint32_t* dst = reinterpret_cast<uint32_t*>(x.out + row_of[i] * x.out_stride + head_of[i] * D);
 #pragma unroll
@@ -299,44 +368,85 @@ k_attend_tiles(PlanView pv, Tensors<T> x) {
                 x.lse[(size_t)row_of[i] * (pv.n_kv * group) + head_of[i]] =
                     sum > 0.0f ? (m[i] - kWeightExp + log2f(sum)) * kLn2 : -INFINITY;
         } else {
-            const size_t at = (size_t)(it.part + it.row0 + lane / 4 + 8 * i) * pv.n_kv + kvh;
+            const size_t at = part[i];
             float2* dst = reinterpret_cast<float2*>(pv.part_o + at * D);
 #pragma unroll
             for (int d = 0; d < DT; ++d) dst[d * 4 + lane % 4] = make_float2(o[d][2 * i], o[d][2 * i + 1]);
             if (lane % 4 == 0) pv.part_ml[at] = make_float2(m[i], sum);
         }
     }
+    if (!pv.arrived) return;
+    // the item that completes a token's parts joins them
+    __threadfence();
+    __syncwarp();
+    bool last = false;
+    Token t = {};
+    if (lane < it.rows && (lane == 0 || (it.row0 + lane) % group == 0)) {
+        t = pv.tokens[it.tokens_at + (it.row0 + lane) / group];
+        if (t.n_parts > 1 && t.limit > it.pos0) {
+            int32_t* n = &pv.arrived[(size_t)t.row * pv.n_kv + kvh];
+            last = atomicAdd(n, 1) == t.arrivals - 1;
+            if (last) *n = 0;   // for the next call
+        }
+    }
+    __threadfence();
+    for (unsigned todo = __ballot_sync(~0u, last); todo; todo &= todo - 1) {
+        const int from = __ffs(todo) - 1, row = __shfl_sync(~0u, t.row, from), part_at = __shfl_sync(~0u, t.part_at, from),
+                  n = __shfl_sync(~0u, t.n_parts, from);
+        for (int g = 0; g < group; ++g) join_row<T, D>(pv, x, row, part_at, n, kvh * group + g);
+    }
 }
 
-// One warp per (token of several parts, query head): the parts in order.
+// One CTA of four warps per (token of several parts, query head), for tokens of many parts: each warp joins every
+// fourth part, then the first one the four results.
 template <typename T, int D>
 __global__ void __launch_bounds__(128)
 k_join_parts(PlanView pv, Tensors<T> x) {
+    constexpr int COLS = D / 4, LANES = 128 / COLS;
+    __shared__ float4 so[128];
+    __shared__ float sl[LANES], sm[4];
     dependents_wait();
-    const int lane = threadIdx.x & 31, heads = pv.n_kv * pv.group;
-    const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (w >= (long long)pv.n_joins * heads) return;
-    const int row = pv.joins[w / heads], head = (int)(w % heads), kvh = head / pv.group, g = head % pv.group;
-    const Token t = pv.info[row];
+    const int tid = threadIdx.x, lane = tid & 31, heads = pv.n_kv * pv.group;
+    const int head = (int)(blockIdx.x % heads), kvh = head / pv.group, g = head % pv.group;
+    const Token t = pv.joins[blockIdx.x / heads];
+    const int row = t.row;
+    auto part = [&](int i) { return ((size_t)(t.part_at + i) * pv.group + g) * pv.n_kv + kvh; };
     float M = -INFINITY;
-    for (int i = lane; i < t.n_parts; i += 32) M = fmaxf(M, pv.part_ml[(size_t)(pv.parts[t.part_at + i] + g) * pv.n_kv + kvh].x);
+    for (int i = tid; i < t.n_parts; i += 128)
+        M = fmaxf(M, __ldcg(&pv.part_ml[part(i)]).x);
     for (int y = 16; y; y >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, y));
-    float acc[D / 32] = {}, l = 0.0f;
-    for (int i = 0; i < t.n_parts; ++i) {
-        const size_t at = (size_t)(pv.parts[t.part_at + i] + g) * pv.n_kv + kvh;
-        const float2 ml = pv.part_ml[at];
+    if (lane == 0) sm[tid >> 5] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+#pragma unroll 4
+    for (int i = tid / COLS; i < t.n_parts; i += LANES) {
+        const size_t at = part(i);
+        const float2 ml = __ldcg(&pv.part_ml[at]);
+        const float4 o = __ldcg(reinterpret_cast<const float4*>(pv.part_o + at * D) + tid % COLS);
         const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
         l = fmaf(f, ml.y, l);
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) acc[j] = fmaf(f, pv.part_o[at * D + j * 32 + lane], acc[j]);
+        acc.x = fmaf(f, o.x, acc.x);
+        acc.y = fmaf(f, o.y, acc.y);
+        acc.z = fmaf(f, o.z, acc.z);
+        acc.w = fmaf(f, o.w, acc.w);
+    }
+    so[tid] = acc;
+    if (tid % COLS == 0) sl[tid / COLS] = l;
+    __syncthreads();
+    if (tid >= COLS) return;
+    acc = so[tid];
+    l = sl[0];
+    for (int j = 1; j < LANES; ++j) {
+        const float4 o = so[j * COLS + tid];
+        acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
+        l += sl[j];
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-        const uint32_t h = pack2(T(), acc[j] * inv, 0.0f);
-        reinterpret_cast<uint16_t*>(x.out + row * x.out_stride + head * D)[j * 32 + lane] = (uint16_t)h;
-    }
-    if (x.lse && lane == 0) x.lse[(size_t)row * heads + head] = l > 0.0f ? (M - kWeightExp + log2f(l)) * kLn2 : -INFINITY;
+    reinterpret_cast<uint2*>(x.out + row * x.out_stride + head * D)[tid] =
+        make_uint2(pack2(T(), acc.x * inv, acc.y * inv), pack2(T(), acc.z * inv, acc.w * inv));
+    if (x.lse && tid == 0) x.lse[(size_t)row * heads + head] = l > 0.0f ? (M - kWeightExp + log2f(l)) * kLn2 : -INFINITY;
 }
 
 int bad(const char* m) { return t2sx_set_error(T2SX_ERR_INVALID, m); }
@@ -346,6 +456,7 @@ struct Node {
     int32_t tokens_at, n_tokens;
     int32_t pages_at, n_pages;
     int32_t pos0, end;
+    int32_t new_pos, new_row;
 };
 
 int sm_count(int device) {
@@ -360,6 +471,7 @@ struct t2sx_plan {
     t2sx_pool* pool = nullptr;
     int n_heads = 0, n_sm = 148;
     bool ready = false, shared_rows = false;
+    int32_t most_parts = 0;
     uint64_t version = 0;          // of the pool at the update
     // host copy of what the device gets, in pinned memory: two buffers, so that an update need not
     // wait for the previous one's upload
@@ -371,9 +483,9 @@ struct t2sx_plan {
     size_t dev_bytes = 0, work_bytes = 0;
     PlanView view = {};
     // scratch of an update
-    std::vector<int32_t> order, next_order, group_of, count, group_page, tokens, pages, parts, joins;
+    std::vector<int32_t> order, next_order, group_of, count, group_page, node_rows, pages;
     std::vector<int32_t> stamp, stamp_group, row0;
-    std::vector<Token> info;
+    std::vector<Token> info, tokens, joins;   // the step's rows; nodes' tokens; those of several parts
     std::vector<Node> nodes;
     std::vector<Item> items;
 };
@@ -420,7 +532,7 @@ extern "C" void t2sx_plan_free(t2sx_plan* a) {
 // split by the page that follows their common run, keeping their order.
 static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int32_t* n_new) {
     t2sx_pool* p = a->pool;
-    a->nodes.clear(); a->tokens.clear(); a->pages.clear();
+    a->nodes.clear(); a->node_rows.clear(); a->pages.clear();
     a->order.clear();
     for (int32_t i = 0; i < n; ++i)
         if (n_new[i] > 0) a->order.push_back(i);
@@ -432,12 +544,12 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
     std::fill(a->stamp.begin(), a->stamp.end(), -1);
     auto emit = [&](const Set& s, int32_t to) {
         Node nd;
-        nd.tokens_at = (int32_t)a->tokens.size();
+        nd.tokens_at = (int32_t)a->node_rows.size();
         for (int32_t j = s.lo; j < s.hi; ++j) {
             const int32_t i = a->order[j];
-            for (int32_t k = 0; k < n_new[i]; ++k) a->tokens.push_back(a->row0[i] + k);
+            for (int32_t k = 0; k < n_new[i]; ++k) a->node_rows.push_back(a->row0[i] + k);
         }
-        nd.n_tokens = (int32_t)a->tokens.size() - nd.tokens_at;
+        nd.n_tokens = (int32_t)a->node_rows.size() - nd.tokens_at;
         const std::vector<int32_t>& t = p->table[seqs[a->order[s.lo]]];
         nd.pages_at = (int32_t)a->pages.size();
         a->pages.insert(a->pages.end(), t.begin() + s.depth, t.begin() + to);
@@ -445,6 +557,10 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
         nd.pos0 = s.depth * kPoolPage;
         // pages of several sequences are full; a sequence's own ones end with it
         nd.end = s.hi - s.lo > 1 ? to * kPoolPage : (int32_t)std::min<int64_t>((int64_t)to * kPoolPage, p->len[seqs[a->order[s.lo]]]);
+        // rows of several sequences have no position in the node's pages (or the step writes nothing)
+        const int32_t i0 = a->order[s.lo];
+        nd.new_pos = s.hi - s.lo > 1 ? INT32_MAX : (int32_t)(p->len[seqs[i0]] - n_new[i0]);
+        nd.new_row = a->row0[i0];
         a->nodes.push_back(nd);
     };
     while (!todo.empty()) {
@@ -492,66 +608,66 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
     }
 }
 
-// Items and parts from the nodes.  A node's pages are split so that there are several items for each warp
-// that the device holds, and each part's result is small against the keys that it stands for.
-static void build_items(t2sx_plan* a) {
+// Items and parts from the nodes; returns the number of parts.  A node's pages are split so that there are
+// several items for each warp that the device holds, and each part's result is small against the keys that
+// it stands for.
+static int64_t build_items(t2sx_plan* a) {
     const int group = a->n_heads / a->pool->n_kv, n_kv = a->pool->n_kv;
-    a->items.clear(); a->parts.clear(); a->joins.clear();
+    a->items.clear(); a->joins.clear();
     int64_t work = 0;
     for (const Node& nd : a->nodes) work += (int64_t)nd.n_pages * ((nd.n_tokens * (int64_t)group + kTileRows - 1) / kTileRows);
-    const int64_t warps = (int64_t)a->n_sm * 9;
-    const int64_t chunk = std::max<int64_t>(2, work * n_kv / (warps * 3));
-    struct Split { int32_t node, page, n_pages; int64_t part; };
-    std::vector<Split> splits;
-    int64_t part = 0;
-    for (size_t i = 0; i < a->nodes.size(); ++i) {
-        const Node& nd = a->nodes[i];
-        const int32_t n = (int32_t)((nd.n_pages + chunk - 1) / chunk), per = (nd.n_pages + n - 1) / n;
-        for (int32_t pg = 0; pg < nd.n_pages; pg += per) {
-            splits.push_back({(int32_t)i, pg, std::min(per, nd.n_pages - pg), part});
-            part += (int64_t)nd.n_tokens * group;
-        }
-    }
-    for (const Split& s : splits) {
-        const Node& nd = a->nodes[s.node];
-        const int32_t start = nd.pos0 + s.page * kPoolPage;
-        const int32_t* tok = a->tokens.data() + nd.tokens_at;
-        for (int32_t j = 0; j < nd.n_tokens; ++j)
-            if (a->info[tok[j]].limit > start) ++a->info[tok[j]].n_parts;
-        const int64_t rows = (int64_t)nd.n_tokens * group;
-        for (int64_t r = 0; r < rows; r += kTileRows) {
-            const int32_t n = (int32_t)std::min<int64_t>(kTileRows, rows - r);
-            int32_t sees = 0;
-            for (int64_t j = r / group; j <= (r + n - 1) / group; ++j) sees = std::max(sees, a->info[tok[j]].limit);
-            const int32_t pages = std::min(s.n_pages, pages_of(sees) - start / kPoolPage);
-            if (pages <= 0) continue;
-            a->items.push_back({nd.tokens_at, (int32_t)r, n, nd.pages_at + s.page, pages, start, (int32_t)s.part, nd.end});
-        }
-    }
-    std::stable_sort(a->items.begin(), a->items.end(), [](const Item& x, const Item& y) { return x.n_pages > y.n_pages; });
-    int32_t at = 0;
-    for (size_t r = 0; r < a->info.size(); ++r) {
-        Token& t = a->info[r];
-        t.part_at = at;
-        at += t.n_parts;
-        if (t.n_parts > 1) a->joins.push_back((int32_t)r);
-        t.n_parts = 0;
-    }
-    a->parts.resize(at);
-    for (const Split& s : splits) {
-        const Node& nd = a->nodes[s.node];
-        const int32_t start = nd.pos0 + s.page * kPoolPage;
+    const int64_t warps = (int64_t)a->n_sm * (a->pool->dim == 128 ? 4 : 9);
+    const int64_t chunk = std::max<int64_t>(kMinChunk, work * n_kv / (warps * 2));
+    a->tokens.resize(a->node_rows.size());
+    for (const Node& nd : a->nodes) {
+        const int32_t n_splits = (int32_t)((nd.n_pages + chunk - 1) / chunk), per = (nd.n_pages + n_splits - 1) / n_splits;
+        const int32_t* rows_of = a->node_rows.data() + nd.tokens_at;
+        // a token has parts for the splits that begin below its limit, the first ones
         for (int32_t j = 0; j < nd.n_tokens; ++j) {
-            Token& t = a->info[a->tokens[nd.tokens_at + j]];
-            if (t.limit > start) a->parts[t.part_at + t.n_parts++] = (int32_t)(s.part + (int64_t)j * group);
+            Token& t = a->info[rows_of[j]];
+            a->tokens[nd.tokens_at + j].part0 = t.n_parts;   // among the token's; its own number is added below
+            const int32_t seen = pages_of(t.limit) - nd.pos0 / kPoolPage;
+            if (seen > 0) t.n_parts += std::min((nd.n_pages + per - 1) / per, (seen + per - 1) / per);
         }
+        const int64_t rows = (int64_t)nd.n_tokens * group;
+        for (int32_t split = 0, pg = 0; pg < nd.n_pages; ++split, pg += per) {
+            const int32_t start = nd.pos0 + pg * kPoolPage;
+            for (int64_t r = 0; r < rows; r += kTileRows) {
+                const int32_t n = (int32_t)std::min<int64_t>(kTileRows, rows - r);
+                int32_t sees = 0;
+                for (int64_t j = r / group; j <= (r + n - 1) / group; ++j) sees = std::max(sees, a->info[rows_of[j]].limit);
+                const int32_t pages = std::min(std::min(per, nd.n_pages - pg), pages_of(sees) - start / kPoolPage);
+                if (pages <= 0) continue;
+                for (int64_t j = r / group; j <= (r + n - 1) / group; ++j)
+                    if (a->info[rows_of[j]].limit > start) ++a->info[rows_of[j]].arrivals;
+                a->items.push_back({nd.tokens_at, (int32_t)r, n, nd.pages_at + pg, pages, start, split, nd.end, nd.new_pos, nd.new_row, {}});
+            }
+        }
+    }
+    // the longest items first; pages of several sequences before all, so that a token's own pages come last and
+    // its join falls to an item of that token alone
+    std::stable_sort(a->items.begin(), a->items.end(), [](const Item& x, const Item& y) {
+        const bool sx = x.new_pos == INT32_MAX, sy = y.new_pos == INT32_MAX;
+        return sx != sy ? sx : x.n_pages > y.n_pages;
+    });
+    int64_t parts = 0;
+    a->most_parts = 0;
+    for (Token& t : a->info) {
+        t.part_at = (int32_t)std::min<int64_t>(parts, INT32_MAX);
+        if (t.n_parts > 1) { a->joins.push_back(t); parts += t.n_parts; }
+        a->most_parts = std::max(a->most_parts, t.n_parts);
+    }
+    for (size_t i = 0; i < a->tokens.size(); ++i) {
+        const int32_t ordinal = a->tokens[i].part0;
+        a->tokens[i] = a->info[a->node_rows[i]];
+        a->tokens[i].part0 = a->tokens[i].part_at + ordinal;
     }
     a->view.n_items = (int)a->items.size();
     a->view.n_joins = (int)a->joins.size();
     a->view.group = group;
     a->view.n_kv = n_kv;
     a->view.rows = (int)a->info.size();
-    a->view.part_ml = reinterpret_cast<float2*>((uintptr_t)part);   // their number; the caller places the arrays
+    return parts;
 }
 
 extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, const int32_t* n_new, void* stream) {
@@ -583,13 +699,12 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
                 const int32_t limit = (int32_t)(p->len[seqs[i]] - n_new[i] + j + 1);
                 const int32_t page = p->table[seqs[i]][(limit - 1) / kPoolPage];
                 a->shared_rows |= p->users[page] > 1;
-                a->info[r] = Token{limit, page, 0, 0};
+                a->info[r] = Token{r, limit, page, 0, 0, 0, 0, 0};
             }
         }
         build_nodes(a, n, seqs, n_new);
-        build_items(a);
-        const int64_t n_parts = (int64_t)(uintptr_t)a->view.part_ml;
-        if (n_parts > INT32_MAX || a->parts.size() > (size_t)INT32_MAX || a->items.size() * p->n_kv > (size_t)INT32_MAX ||
+        const int64_t n_parts = build_items(a);
+        if (n_parts >= INT32_MAX || a->items.size() * p->n_kv > (size_t)INT32_MAX ||
             a->joins.size() * (size_t)a->n_heads > (size_t)INT32_MAX)
             return bad("t2sx_plan_update: too many rows");
 
@@ -597,8 +712,7 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
         POOL_CK(dg.set(p->device));
         size_t bytes = 0;
         auto place = [&](auto const& v) { const size_t at = bytes; bytes = (bytes + v.size() * sizeof(v[0]) + 15) & ~(size_t)15; return at; };
-        const size_t o_info = place(a->info), o_items = place(a->items), o_tokens = place(a->tokens), o_pages = place(a->pages),
-                     o_parts = place(a->parts), o_joins = place(a->joins);
+        const size_t o_items = place(a->items), o_tokens = place(a->tokens), o_pages = place(a->pages), o_joins = place(a->joins);
         const int b = a->turn ^= 1;
         POOL_CK(cudaEventSynchronize(a->sent[b]));
         if (a->host_bytes[b] < bytes) {
@@ -622,23 +736,23 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
         };
         POOL_CK(grow(a->dev, a->dev_bytes, bytes));
         // results of parts, where tokens have several
-        const size_t part_rows = a->joins.empty() ? 0 : (size_t)n_parts * p->n_kv, o_bytes = part_rows * p->dim * 4;
-        POOL_CK(grow(a->work, a->work_bytes, o_bytes + part_rows * 8));
+        const size_t part_rows = (size_t)n_parts * a->n_heads, o_bytes = part_rows * p->dim * 4;
+        const size_t n_arrived = !a->joins.empty() && a->most_parts <= kWarpJoin ? (size_t)rows * p->n_kv : 0;
+        POOL_CK(grow(a->work, a->work_bytes, o_bytes + part_rows * 8 + n_arrived * 4));
+        if (n_arrived) POOL_CK(cudaMemsetAsync(a->work + o_bytes + part_rows * 8, 0, n_arrived * 4, st));
         auto put = [&](size_t at, auto const& v) { if (!v.empty()) memcpy(a->host[b] + at, v.data(), v.size() * sizeof(v[0])); };
-        put(o_info, a->info); put(o_items, a->items); put(o_tokens, a->tokens); put(o_pages, a->pages); put(o_parts, a->parts);
-        put(o_joins, a->joins);
+        put(o_items, a->items); put(o_tokens, a->tokens); put(o_pages, a->pages); put(o_joins, a->joins);
         if (bytes) POOL_CK(cudaMemcpyAsync(a->dev, a->host[b], bytes, cudaMemcpyHostToDevice, st));
         POOL_CK(cudaEventRecord(a->sent[b], st));
         POOL_CK(p->end(st));
         PlanView& w = a->view;
-        w.info = (const Token*)(a->dev + o_info);
         w.items = (const Item*)(a->dev + o_items);
-        w.tokens = (const int32_t*)(a->dev + o_tokens);
+        w.tokens = (const Token*)(a->dev + o_tokens);
         w.pages = (const int32_t*)(a->dev + o_pages);
-        w.parts = (const int32_t*)(a->dev + o_parts);
-        w.joins = (const int32_t*)(a->dev + o_joins);
+        w.joins = (const Token*)(a->dev + o_joins);
         w.part_o = (float*)a->work;
         w.part_ml = (float2*)(a->work + o_bytes);
+        w.arrived = n_arrived ? (int32_t*)(a->work + o_bytes + part_rows * 8) : nullptr;
         a->version = p->version;
         a->ready = true;
         return T2SX_OK;
@@ -662,27 +776,28 @@ static cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t s
 }
 
 template <typename T, int D>
-static cudaError_t launch_attend(t2sx_plan* a, const Tensors<T>& x, bool wrote, cudaStream_t st) {
+static cudaError_t launch_attend(t2sx_plan* a, const Tensors<T>& x, cudaStream_t st) {
     const PlanView& w = a->view;
     using S = TileShape<D>;
     static std::once_flag once[64];
     std::call_once(once[a->pool->device & 63],
                    [] { cudaFuncSetAttribute(k_attend_tiles<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
-    cudaError_t e = launch(k_attend_tiles<T, D>, dim3((unsigned)(w.n_items * w.n_kv)), 32, S::SMEM, st, wrote, w, x);
-    if (e == cudaSuccess && w.n_joins)
-        e = launch(k_join_parts<T, D>, dim3((unsigned)(((long long)w.n_joins * a->n_heads + 3) / 4)), 128, 0, st, true, w, x);
+    cudaError_t e = launch(k_attend_tiles<T, D>, dim3((unsigned)(w.n_items * w.n_kv)), 32, S::SMEM, st, false, w, x);
+    if (e == cudaSuccess && w.n_joins && !w.arrived)
+        e = launch(k_join_parts<T, D>, dim3((unsigned)(w.n_joins * a->n_heads)), 128, 0, st, true, w, x);
     return e;
 }
 
 template <typename T>
-static cudaError_t attend(t2sx_plan* a, size_t page0, const void* q, int64_t q_stride, float scale, void* out, int64_t out_stride,
-                          float* lse, bool wrote, cudaStream_t st) {
+static cudaError_t attend(t2sx_plan* a, int32_t layer, const void* q, int64_t q_stride, const void* k_new, const void* v_new,
+                          int64_t kv_stride, float scale, void* out, int64_t out_stride, float* lse, cudaStream_t st) {
     t2sx_pool* p = a->pool;
-    const size_t first = page0 * p->n_kv * kPoolPage * p->dim;
-    const Tensors<T> x = {(const T*)q, (const T*)p->k + first, (const T*)p->v + first, (T*)out, lse, q_stride, out_stride, scale * kLog2e};
-    if (p->dim == 32) return launch_attend<T, 32>(a, x, wrote, st);
-    if (p->dim == 64) return launch_attend<T, 64>(a, x, wrote, st);
-    return launch_attend<T, 128>(a, x, wrote, st);
+    const size_t first = (size_t)layer * p->n_pages * p->n_kv * kPoolPage * p->dim;
+    const Tensors<T> x = {(const T*)q, (T*)p->k + first, (T*)p->v + first, (const T*)k_new, (const T*)v_new, kv_stride,
+                          (T*)out, lse, q_stride, out_stride, scale * kLog2e};
+    if (p->dim == 32) return launch_attend<T, 32>(a, x, st);
+    if (p->dim == 64) return launch_attend<T, 64>(a, x, st);
+    return launch_attend<T, 128>(a, x, st);
 }
 
 extern "C" int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, int64_t q_stride, const void* k_new_dev,
@@ -708,19 +823,8 @@ extern "C" int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, 
     DeviceGuard dg;
     POOL_CK(dg.set(p->device));
     POOL_CK(p->begin(st));
-    const size_t page0 = (size_t)layer * p->n_pages;
-    if (k_new_dev) {
-        const int row_vec = p->dim * 2 / 16;
-        const int64_t vecs = (int64_t)a->view.rows * p->n_kv * row_vec;
-        const size_t first = page0 * p->n_kv * kPoolPage * row_vec;
-        k_write_rows<<<(unsigned)((vecs + 255) / 256), 256, 0, st>>>(a->view.info, a->view.rows, (const uint4*)k_new_dev,
-                                                                    (const uint4*)v_new_dev, kv_stride / 8, (uint4*)p->k + first,
-                                                                    (uint4*)p->v + first, p->n_kv, row_vec);
-        POOL_CK(cudaGetLastError());
-    }
-    const bool wrote = k_new_dev != nullptr;
-    if (p->type == T2SX_TYPE_F16) POOL_CK(attend<__half>(a, page0, q_dev, q_stride, scale, out_dev, out_stride, lse_dev, wrote, st));
-    else POOL_CK(attend<__nv_bfloat16>(a, page0, q_dev, q_stride, scale, out_dev, out_stride, lse_dev, wrote, st));
+    auto go = p->type == T2SX_TYPE_F16 ? attend<__half> : attend<__nv_bfloat16>;
+    POOL_CK(go(a, layer, q_dev, q_stride, k_new_dev, v_new_dev, kv_stride, scale, out_dev, out_stride, lse_dev, st));
     POOL_CK(p->end(st));
     return T2SX_OK;
 }

@@ -520,6 +520,42 @@ def test_logprobs_empty_rows_and_padding(t2sx_mod, dtype, rows, vocab):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [0, 1, 30])
+@pytest.mark.parametrize("vocab", [900, 40000])
+def test_logprobs_ends_of_the_range(t2sx_mod, dtype, vocab):
+    """Tokens masked with the type's lowest value: some, all, all but masked ones, beside -inf; values near the
+    greatest one; values around -10000, whose differences count."""
+    _need_gpu()
+    low = torch.finfo(TORCH[dtype]).min
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    x = (torch.randn((7, vocab), generator=gen, device="cuda") * 2).to(TORCH[dtype])
+    x[0, ::2] = low
+    x[1] = low
+    x[2] = low
+    x[2, 1::3] = float("-inf")
+    x[3, : vocab - 9] = low
+    x[4] = -low
+    x[4, ::2] = -low * 0.5
+    x[5] = -10000 + x[5] * 8
+    x[6] = low
+    x[6, vocab // 3 :] = low * 0.998
+    tokens = torch.tensor([1, 7, 0, vocab - 1, 3, 2, vocab // 2], device="cuda", dtype=torch.int32)
+    got = [a.cpu() for a in _scores(t2sx_mod, x, tokens, 8)]
+    ref = x.double().log_softmax(-1).cpu()
+    lp, h, rank, ids, tl = got
+    # (differences of up to twice the type's range: compared where the weight is not 0)
+    want = ref.gather(1, tokens.cpu().long()[:, None])[:, 0]
+    near = want > -1e3
+    assert near.sum() >= 5 and ((lp.double() - want).abs()[near] <= 2.0 ** -17 * want.abs().clamp(min=1)[near]).all()
+    href = -torch.special.xlogy(ref.exp(), ref.exp()).sum(-1)
+    assert ((h.double() - href).abs() <= 2.0 ** -17 * 16).all(), (h, href)
+    order = torch.sort(x.double().cpu(), dim=1, descending=True, stable=True)
+    assert torch.equal(ids.long(), order.indices[:, :8])
+    tref = ref.gather(1, order.indices[:, :8])
+    assert ((tl.double() - tref).abs()[tref > -1e3] <= 2.0 ** -17 * 16).all()
+
+
+@gpu
 def test_logprobs_optional_outputs(t2sx_mod):
     _need_gpu()
     x = torch.randn((4, 50), device="cuda")
