@@ -21,10 +21,8 @@ inline int32_t pages_of(int64_t len) { return (int32_t)((len + kPoolPage - 1) / 
 
 // One page copy: the first `fill` positions of every layer and head.
 struct PageMove {
-    int32_t src;
-    uint32_t dst_fill;   // dst | (fill - 1) << 26
+    int32_t src, dst, fill;
 };
-inline PageMove page_move(int32_t src, int32_t dst, int fill) { return PageMove{src, (uint32_t)dst | (uint32_t)(fill - 1) << 26}; }
 
 }  // namespace t2sx
 

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from array import array
 
 import numpy as np
 
@@ -73,7 +74,7 @@ SIGNATURES = {
     "t2sx_pool_free": (None, [_P]),
     "t2sx_pool_available": (C.c_int, [_P, _P]),
     "t2sx_pool_length": (_I64, [_P, _I]),
-    "t2sx_pool_table": (C.c_int, [_P, _I, _P, _I, _P]),
+    "t2sx_pool_table": (C.c_int, [_P, _I, _P, _I, _P, _P]),
     "t2sx_pool_extend": (C.c_int, [_P, _I, _P, _P]),
     "t2sx_pool_fork": (C.c_int, [_P, _I, _P, _P, _P]),
     "t2sx_pool_copy": (C.c_int, [_P, _I, _P, _P, _P]),
@@ -438,8 +439,14 @@ class KVCache:
             pass
 
 
-def _i32(a):
-    return np.ascontiguousarray(np.atleast_1d(a), dtype=np.int32)
+def _ids(a, kind="i"):
+    """(address, number, what keeps them alive) of ids or counts ("q": 64 bits); lists and tuples of Python
+    integers take the short way."""
+    if isinstance(a, (list, tuple)):
+        a = array(kind, a)
+        return a.buffer_info()[0], len(a), a
+    a = np.ascontiguousarray(np.atleast_1d(a), dtype=np.int32 if kind == "i" else np.int64)
+    return a.__array_interface__["data"][0], a.size, a
 
 
 class PagePool:
@@ -472,25 +479,25 @@ class PagePool:
 
     def table(self, seqs) -> np.ndarray:
         """Page ids of the sequences, int32 [n][most pages of one], filled up with -1."""
-        seqs = _i32(seqs)
-        width = max((-(-self.length(int(s)) // self.PAGE) for s in seqs), default=0)
-        out = np.empty((seqs.size, width), dtype=np.int32)
-        _ck(lib().t2sx_pool_table(self.h, seqs.size, _p(seqs), width, _p(out)))
+        ids, n, _keep = _ids(seqs)
+        width = C.c_int32(0)
+        _ck(lib().t2sx_pool_table(self.h, n, ids, 0, None, C.byref(width)))
+        out = np.empty((n, width.value), dtype=np.int32)
+        _ck(lib().t2sx_pool_table(self.h, n, ids, width.value, out.__array_interface__["data"][0], None))
         return out
 
     def _pairs(self, fn, srcs, dsts, stream):
-        srcs, dsts = _i32(srcs), _i32(dsts)
-        if srcs.size != dsts.size:
+        (a, n, _a), (b, m, _b) = _ids(srcs), _ids(dsts)
+        if n != m:
             raise ValueError("as many sources as destinations are needed")
-        _ck(fn(self.h, srcs.size, _p(srcs), _p(dsts), stream))
+        _ck(fn(self.h, n, a, b, stream))
 
     def extend(self, seqs, counts):
         """counts[i] more positions for seqs[i]."""
-        seqs = _i32(seqs)
-        counts = np.ascontiguousarray(np.atleast_1d(counts), dtype=np.int64)
-        if seqs.size != counts.size:
+        (a, n, _a), (b, m, _b) = _ids(seqs), _ids(counts, "q")
+        if n != m:
             raise ValueError("as many counts as sequences are needed")
-        _ck(lib().t2sx_pool_extend(self.h, seqs.size, _p(seqs), _p(counts)))
+        _ck(lib().t2sx_pool_extend(self.h, n, a, b))
 
     def fork(self, srcs, dsts, stream: int = 0):
         """dsts[i] := a continuation of srcs[i] that shares its full pages."""
@@ -501,8 +508,8 @@ class PagePool:
         self._pairs(lib().t2sx_pool_copy, srcs, dsts, stream)
 
     def release(self, seqs):
-        seqs = _i32(seqs)
-        _ck(lib().t2sx_pool_release(self.h, seqs.size, _p(seqs)))
+        ids, n, _keep = _ids(seqs)
+        _ck(lib().t2sx_pool_release(self.h, n, ids))
 
     def compact(self, stream: int = 0) -> int:
         """Moves the pages in use to the lowest ids; how many moved."""
@@ -537,11 +544,11 @@ class AttnPlan:
 
     def update(self, seqs, n_new, stream: int = 0):
         """The step's sequences and how many of their last positions are rows of the step."""
-        seqs, n_new = _i32(seqs), _i32(n_new)
-        if seqs.size != n_new.size:
+        (a, n, _a), (b, m, rows) = _ids(seqs), _ids(n_new)
+        if n != m:
             raise ValueError("as many row counts as sequences are needed")
-        _ck(lib().t2sx_plan_update(self.h, seqs.size, _p(seqs), _p(n_new), stream))
-        self.rows = int(n_new.sum())
+        _ck(lib().t2sx_plan_update(self.h, n, a, b, stream))
+        self.rows = int(sum(rows))
 
     def attend(self, layer: int, q_ptr: int, out_ptr: int, scale: float, k_new_ptr: int | None = None,
                v_new_ptr: int | None = None, lse_ptr: int | None = None, q_stride: int | None = None,

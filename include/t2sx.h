@@ -275,8 +275,9 @@ T2SX_API void t2sx_pool_free(t2sx_pool* p);
 T2SX_API int t2sx_pool_available(t2sx_pool* p, int32_t* n_pages);
 /* Positions of a sequence; -1 for a bad argument. */
 T2SX_API int64_t t2sx_pool_length(t2sx_pool* p, int32_t seq);
-/* Page ids of n sequences: out [n][width], rows filled up with -1; width >= the longest's pages. */
-T2SX_API int t2sx_pool_table(t2sx_pool* p, int32_t n, const int32_t* seqs, int32_t width, int32_t* out);
+/* Page ids of n sequences: out [n][width], rows filled up with -1, width at least the longest's pages.
+ * *longest (may be null) = the longest's pages; with out null that alone. */
+T2SX_API int t2sx_pool_table(t2sx_pool* p, int32_t n, const int32_t* seqs, int32_t width, int32_t* out, int32_t* longest);
 /* counts[i] (>= 0) positions more for sequence seqs[i] (distinct), in order; their values are
  * undefined until written.  T2SX_ERR_OOM if the pool has not enough pages. */
 T2SX_API int t2sx_pool_extend(t2sx_pool* p, int32_t n, const int32_t* seqs, const int64_t* counts);
