@@ -17,16 +17,22 @@
 #include <cstring>
 #include <memory>
 #include <mutex>
+#include <type_traits>
 
 using namespace t2sx;
 
+#ifndef C32
+#define C32 32,3,16
+#define C64 32,3,9
+#define C128 32,3,4
+#endif
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kWeightExp = 7.0f;   // c above: weights are at most 2^7
 constexpr int kTileRows = 16;        // rows of a warp's tile (the m of mma.m16n8k16)
 constexpr int kMinChunk = 2;         // pages of a split at least
-constexpr int kWarpJoin = 8;         // parts of a token up to which the last item joins them
+constexpr int kSmallPages = 32;      // pages of a sequence in a small step at most
 
 // A tile of rows against a range of a node's pages.
 struct Item {
@@ -50,7 +56,8 @@ struct alignas(16) Token {
     int32_t page;        // page of its own position
     int32_t part0, part_at;
     int32_t n_parts;     // one: the item writes the result itself
-    int32_t arrivals;    // items that hold some of its heads' parts, for each K/V head
+    int32_t ends_here;   // the node's item completes the token: its own part is the last one, and the others are
+                         // those of the launch before
     int32_t pad;
 };
 
@@ -61,8 +68,7 @@ struct PlanView {
     const Token* joins;      // tokens of several parts
     float* part_o;           // [part][query head of the group][K/V head][dim]
     float2* part_ml;         // [part][query head of the group][K/V head]
-    int32_t* arrived;        // [row][K/V head] items that are done; null: a second kernel joins the parts
-    int rows, n_items, n_joins, group, n_kv;
+    int rows, n_shared, n_items, n_joins, group, n_kv;   // items: first the n_shared of several sequences
 };
 
 // Strided tensors of one call.
@@ -119,12 +125,17 @@ __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0
 __device__ __forceinline__ void dependents_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// Tiles of a head dimension: keys per stage of the ring and stages.
+// Tiles of a head dimension: keys per stage of a warp's ring, its stages, the warps of an SM that this leaves
+// room for, and the warps of a CTA that shares out one item.
+template <int KEYS_, int STAGES_, int RESIDENT_>
+struct Cfg { static constexpr int KEYS = KEYS_, STAGES = STAGES_, RESIDENT = RESIDENT_; };
 template <int D>
 struct TileShape {
-    static constexpr int KEYS = D == 32 ? 64 : 32, STAGES = D == 32 ? 2 : 3;
+    using C = std::conditional_t<D == 32, Cfg<C32>, std::conditional_t<D == 64, Cfg<C64>, Cfg<C128>>>;
+    static constexpr int KEYS = C::KEYS, STAGES = C::STAGES, RESIDENT = C::RESIDENT, TEAM = D == 128 ? 4 : 8;
     static constexpr int HALF = KEYS * D * 2;   // bytes of a stage's K (or V)
-    static constexpr int SMEM = STAGES * 2 * HALF;
+    static constexpr int RING = STAGES * 2 * HALF;
+    static_assert(RING >= 16 * D * 4, "a warp's results take the place of its ring");
 };
 
 // 16-byte chunk `c` of key `row` in a tile: chunks are exchanged within 128 bytes so that the eight rows
@@ -135,62 +146,23 @@ __device__ __forceinline__ uint32_t tile_at(int row, int c) {
     else return row * (D * 2) + ((c & ~7) | ((c ^ row) & 7)) * 16;
 }
 
-// The parts of one token's query head, in their order whoever joins them: the warp's lanes are D / 4 columns of
-// four dims x 32 / (D / 4) parts.  Parts were written by other SMs in this or the previous launch (L2 loads).
-template <typename T, int D>
-__device__ __forceinline__ void join_row(const PlanView& pv, const Tensors<T>& x, int row, int part_at, int n_parts,
-                                         int head) {
-    constexpr int COLS = D / 4, LANES = 32 / COLS;
-    const int lane = threadIdx.x & 31, kvh = head / pv.group, g = head % pv.group;
-    auto part = [&](int i) { return ((size_t)(part_at + i) * pv.group + g) * pv.n_kv + kvh; };
-    float M = -INFINITY;
-    for (int i = lane; i < n_parts; i += 32) M = fmaxf(M, __ldcg(&pv.part_ml[part(i)]).x);
-    for (int y = 16; y; y >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, y));
-    float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
-#pragma unroll 2
-    for (int i = lane / COLS; i < n_parts; i += LANES) {
-        const size_t at = part(i);
-        const float2 ml = __ldcg(&pv.part_ml[at]);
-        const float4 o = __ldcg(reinterpret_cast<const float4*>(pv.part_o + at * D) + lane % COLS);
-        const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
-        l = fmaf(f, ml.y, l);
-        acc.x = fmaf(f, o.x, acc.x);
-        acc.y = fmaf(f, o.y, acc.y);
-        acc.z = fmaf(f, o.z, acc.z);
-        acc.w = fmaf(f, o.w, acc.w);
-    }
-#pragma unroll
-    for (int y = COLS; y < 32; y <<= 1) {
-        l += __shfl_xor_sync(~0u, l, y);
-        acc.x += __shfl_xor_sync(~0u, acc.x, y);
-        acc.y += __shfl_xor_sync(~0u, acc.y, y);
-        acc.z += __shfl_xor_sync(~0u, acc.z, y);
-        acc.w += __shfl_xor_sync(~0u, acc.w, y);
-    }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    if (lane < COLS)
-        reinterpret_cast<uint2*>(x.out + row * x.out_stride + head * D)[lane] =
-            make_uint2(pack2(T(), acc.x * inv, acc.y * inv), pack2(T(), acc.z * inv, acc.w * inv));
-    if (x.lse && lane == 0)
-        x.lse[(size_t)row * (pv.n_kv * pv.group) + head] = l > 0.0f ? (M - kWeightExp + log2f(l)) * kLn2 : -INFINITY;
-}
-
-// One warp per (item, K/V head): at most 16 rows, keys streamed through a ring of its own.
-template <typename T, int D>
-__global__ void __launch_bounds__(32)
-k_attend_tiles(PlanView pv, Tensors<T> x) {
+// One CTA per (item, K/V head): at most 16 rows.  Its W warps share out the item's tiles, each with a ring of
+// its own, and join their results in shared memory.
+template <typename T, int D, int W>
+__global__ void __launch_bounds__(32 * W, W == 1 ? TileShape<D>::RESIDENT : 1)
+k_attend_tiles(PlanView pv, Tensors<T> x, int item0) {
     using S = TileShape<D>;
     constexpr int NT = S::KEYS / 8, DT = D / 8, KS = D / 16;   // key tiles, dim tiles, steps along the dims
     extern __shared__ __align__(1024) unsigned char ring[];
-    const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring);
-    const int lane = threadIdx.x, kvh = blockIdx.x % pv.n_kv;   // neighbours read one page
-    const Item it = pv.items[blockIdx.x / pv.n_kv];
+    const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5;
+    const int kvh = blockIdx.x % pv.n_kv;   // neighbours read one page
+    const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring) + warp * S::RING;
+    const Item it = pv.items[item0 + blockIdx.x / pv.n_kv];
     const int group = pv.group;
 
-    const int tiles = it.n_pages * (kPoolPage / S::KEYS);
-    int page_id = it.pages_at >= 0 && lane < it.n_pages ? pv.pages[it.pages_at + lane] : 0;
-    int page_base = 0;                                // pages [page_base, page_base + 32) are in the lanes
+    const int all = it.n_pages * (kPoolPage / S::KEYS), first = all * warp / W, tiles = all * (warp + 1) / W;
+    int page_base = first / (kPoolPage / S::KEYS);    // pages [page_base, page_base + 32) are in the lanes
+    int page_id = page_base + lane < it.n_pages ? pv.pages[it.pages_at + page_base + lane] : 0;
     auto request = [&](int t) {
         if (t < tiles) {
             const int pg = t / (kPoolPage / S::KEYS), sub = t % (kPoolPage / S::KEYS);
@@ -200,7 +172,7 @@ k_attend_tiles(PlanView pv, Tensors<T> x) {
             }
             const int page = __shfl_sync(~0u, page_id, pg - page_base);
             const size_t at = (((size_t)page * pv.n_kv + kvh) * kPoolPage + sub * S::KEYS) * D;
-            const uint32_t dst = ring0 + (t % S::STAGES) * 2 * S::HALF;
+            const uint32_t dst = ring0 + ((t - first) % S::STAGES) * 2 * S::HALF;
             const char *ks = reinterpret_cast<const char*>(x.k + at), *vs = reinterpret_cast<const char*>(x.v + at);
             const int pos = it.pos0 + t * S::KEYS;
             const bool plain = pos + S::KEYS <= min(it.end, x.k_new ? it.new_pos : INT32_MAX);
@@ -226,9 +198,8 @@ k_attend_tiles(PlanView pv, Tensors<T> x) {
     };
 
     // rows lane / 4 and lane / 4 + 8
-    int row_of[2], head_of[2], limit[2], n_parts[2];
-    size_t part[2];
-    bool live[2];
+    int row_of[2], head_of[2], limit[2], n_parts[2], part[2];
+    bool live[2], ends[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int r = lane / 4 + 8 * i, mr = it.row0 + r, g = mr % group;
@@ -238,9 +209,11 @@ k_attend_tiles(PlanView pv, Tensors<T> x) {
         head_of[i] = kvh * group + g;
         limit[i] = live[i] ? t.limit : 0;
         n_parts[i] = t.n_parts;
-        part[i] = ((size_t)(t.part0 + it.split) * group + g) * pv.n_kv + kvh;
+        ends[i] = t.ends_here;
+        part[i] = t.part0 + it.split;
     }
-    for (int t = 0; t < S::STAGES - 1; ++t) request(t);
+    auto part_index = [&](int i, int part) { return ((size_t)part * group + head_of[i] - kvh * group) * pv.n_kv + kvh; };
+    for (int t = first; t < first + S::STAGES - 1; ++t) request(t);
     uint32_t qf[KS][4];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -256,7 +229,7 @@ k_attend_tiles(PlanView pv, Tensors<T> x) {
     auto own = [&](int r) -> const Token* {
         const Token* t = pv.tokens + it.tokens_at + (it.row0 + r) / group;
         return x.k_new && r < it.rows && (it.row0 + r) % group == 0 && t->limit > it.pos0 &&
-               t->limit <= it.pos0 + it.n_pages * kPoolPage && lane < D / 4 ? t : nullptr;
+               t->limit <= it.pos0 + it.n_pages * kPoolPage && lane < D / 4 && warp == 0 ? t : nullptr;
     };
     auto own_src = [&](const Token* t) {
         return reinterpret_cast<const uint4*>((lane >= D / 8 ? x.v_new : x.k_new) + t->row * x.kv_stride + kvh * D) + lane % (D / 8);
@@ -274,10 +247,10 @@ k_attend_tiles(PlanView pv, Tensors<T> x) {
 
     const bool upper = it.rows > 8;
     float o[DT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    for (int t = 0; t < tiles; ++t) {
+    for (int t = first; t < tiles; ++t) {
         cp_wait<S::STAGES - 2>();
         __syncwarp();
-        const uint32_t kt = ring0 + (t % S::STAGES) * 2 * S::HALF, vt = kt + S::HALF;
+        const uint32_t kt = ring0 + ((t - first) % S::STAGES) * 2 * S::HALF, vt = kt + S::HALF;
         const int pos = it.pos0 + t * S::KEYS;
         float s[NT][4] = {};
 #pragma unroll
@@ -349,51 +322,91 @@ k_attend_tiles(PlanView pv, Tensors<T> x) {
         request(t + S::STAGES - 1);
     }
     cp_wait<0>();
-    dependents_launch();
     if (own0) *own_dst(own0) = own_word;
     for (int r = 1; r < it.rows; ++r)
         if (const Token* t = own(r)) *own_dst(t) = *own_src(t);
+    dependents_launch();
+    float sum[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        float sum = l[i];
-        sum += __shfl_xor_sync(~0u, sum, 1);
-        sum += __shfl_xor_sync(~0u, sum, 2);
-        if (!live[i] || limit[i] <= it.pos0) continue;   // such a row has no part here
-        if (n_parts[i] == 1) {
-            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-            uint32_t* dst = reinterpret_cast<uint32_t*>(x.out + row_of[i] * x.out_stride + head_of[i] * D);
+        sum[i] = l[i];
+        sum[i] += __shfl_xor_sync(~0u, sum[i], 1);
+        sum[i] += __shfl_xor_sync(~0u, sum[i], 2);
+    }
+    if constexpr (W > 1) {
+        // the warps' results in the place of their rings; then each warp joins the dim tiles warp, warp + W, ...
+        __shared__ float2 ml[W][16];
+        __syncthreads();
+        float2* all_o = reinterpret_cast<float2*>(ring);
 #pragma unroll
-            for (int d = 0; d < DT; ++d) dst[d * 4 + lane % 4] = pack2(T(), o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
-            if (x.lse && lane % 4 == 0)
-                x.lse[(size_t)row_of[i] * (pv.n_kv * group) + head_of[i]] =
-                    sum > 0.0f ? (m[i] - kWeightExp + log2f(sum)) * kLn2 : -INFINITY;
-        } else {
-            const size_t at = part[i];
+        for (int i = 0; i < 2; ++i) {
+            if (lane % 4 == 0) ml[warp][lane / 4 + 8 * i] = make_float2(m[i], sum[i]);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) all_o[((warp * 2 + i) * DT + d) * 32 + lane] = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float M = -INFINITY;
+            for (int j = 0; j < W; ++j) M = fmaxf(M, ml[j][lane / 4 + 8 * i].x);
+            m[i] = M;
+            sum[i] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d][2 * i] = o[d][2 * i + 1] = 0.0f;
+            for (int j = 0; j < W; ++j) {
+                const float2 part = ml[j][lane / 4 + 8 * i];
+                const float f = part.x == -INFINITY ? 0.0f : ex2(part.x - M);
+                sum[i] = fmaf(part.y, f, sum[i]);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    if (d % W != warp) continue;
+                    const float2 y = all_o[((j * 2 + i) * DT + d) * 32 + lane];
+                    o[d][2 * i] = fmaf(y.x, f, o[d][2 * i]);
+                    o[d][2 * i + 1] = fmaf(y.y, f, o[d][2 * i + 1]);
+                }
+            }
+        }
+    }
+    auto mine = [&](int d) { return W == 1 || d % W == warp; };
+    dependents_wait();   // the parts of the launch before
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (!live[i] || limit[i] <= it.pos0) continue;   // such a row has no part here
+        if (n_parts[i] > 1 && !ends[i]) {
+            const size_t at = part_index(i, part[i]);
             float2* dst = reinterpret_cast<float2*>(pv.part_o + at * D);
 #pragma unroll
-            for (int d = 0; d < DT; ++d) dst[d * 4 + lane % 4] = make_float2(o[d][2 * i], o[d][2 * i + 1]);
-            if (lane % 4 == 0) pv.part_ml[at] = make_float2(m[i], sum);
+            for (int d = 0; d < DT; ++d)
+                if (mine(d)) dst[d * 4 + lane % 4] = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+            if (lane % 4 == 0 && warp == 0) pv.part_ml[at] = make_float2(m[i], sum[i]);
+            continue;
         }
-    }
-    if (!pv.arrived) return;
-    // the item that completes a token's parts joins them
-    __threadfence();
-    __syncwarp();
-    bool last = false;
-    Token t = {};
-    if (lane < it.rows && (lane == 0 || (it.row0 + lane) % group == 0)) {
-        t = pv.tokens[it.tokens_at + (it.row0 + lane) / group];
-        if (t.n_parts > 1 && t.limit > it.pos0) {
-            int32_t* n = &pv.arrived[(size_t)t.row * pv.n_kv + kvh];
-            last = atomicAdd(n, 1) == t.arrivals - 1;
-            if (last) *n = 0;   // for the next call
+        if constexpr (W == 1) {
+            for (int j = n_parts[i] - 1; j-- > 0;) {   // the other parts, if any
+                const size_t at = part_index(i, part[i] - n_parts[i] + 1 + j);
+                const float2 ml = __ldcg(&pv.part_ml[at]);
+                const float2* src = reinterpret_cast<const float2*>(pv.part_o + at * D);
+                float2 y[DT];
+#pragma unroll
+                for (int d = 0; d < DT; ++d) y[d] = __ldcg(&src[d * 4 + lane % 4]);
+                const float M = fmaxf(m[i], ml.x), f = m[i] == -INFINITY ? 0.0f : ex2(m[i] - M), g = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+                m[i] = M;
+                sum[i] = fmaf(sum[i], f, ml.y * g);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    o[d][2 * i] = fmaf(o[d][2 * i], f, y[d].x * g);
+                    o[d][2 * i + 1] = fmaf(o[d][2 * i + 1], f, y[d].y * g);
+                }
+            }
         }
-    }
-    __threadfence();
-    for (unsigned todo = __ballot_sync(~0u, last); todo; todo &= todo - 1) {
-        const int from = __ffs(todo) - 1, row = __shfl_sync(~0u, t.row, from), part_at = __shfl_sync(~0u, t.part_at, from),
-                  n = __shfl_sync(~0u, t.n_parts, from);
-        for (int g = 0; g < group; ++g) join_row<T, D>(pv, x, row, part_at, n, kvh * group + g);
+        const float inv = sum[i] > 0.0f ? 1.0f / sum[i] : 0.0f;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(x.out + row_of[i] * x.out_stride + head_of[i] * D);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+            if (mine(d)) dst[d * 4 + lane % 4] = pack2(T(), o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
+        if (x.lse && lane % 4 == 0 && warp == 0)
+            x.lse[(size_t)row_of[i] * (pv.n_kv * group) + head_of[i]] =
+                sum[i] > 0.0f ? (m[i] - kWeightExp + log2f(sum[i])) * kLn2 : -INFINITY;
     }
 }
 
@@ -459,6 +472,10 @@ struct Node {
     int32_t new_pos, new_row;
 };
 
+int resident_warps(int dim) {
+    return dim == 32 ? TileShape<32>::RESIDENT : dim == 64 ? TileShape<64>::RESIDENT : TileShape<128>::RESIDENT;
+}
+
 int sm_count(int device) {
     int n = 0;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) return 148;
@@ -470,8 +487,7 @@ int sm_count(int device) {
 struct t2sx_plan {
     t2sx_pool* pool = nullptr;
     int n_heads = 0, n_sm = 148;
-    bool ready = false, shared_rows = false;
-    int32_t most_parts = 0;
+    bool ready = false, shared_rows = false, small = false;
     uint64_t version = 0;          // of the pool at the update
     // host copy of what the device gets, in pinned memory: two buffers, so that an update need not
     // wait for the previous one's upload
@@ -563,6 +579,10 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
         nd.new_row = a->row0[i0];
         a->nodes.push_back(nd);
     };
+    if (a->small) {   // nothing is shared: one node for each sequence
+        for (int32_t j = 0; j < (int32_t)a->order.size(); ++j) emit({j, j + 1, 0}, (int32_t)p->table[seqs[a->order[j]]].size());
+        return;
+    }
     while (!todo.empty()) {
         const Set s = todo.back();
         todo.pop_back();
@@ -616,8 +636,8 @@ static int64_t build_items(t2sx_plan* a) {
     a->items.clear(); a->joins.clear();
     int64_t work = 0;
     for (const Node& nd : a->nodes) work += (int64_t)nd.n_pages * ((nd.n_tokens * (int64_t)group + kTileRows - 1) / kTileRows);
-    const int64_t warps = (int64_t)a->n_sm * (a->pool->dim == 128 ? 4 : 9);
-    const int64_t chunk = std::max<int64_t>(kMinChunk, work * n_kv / (warps * 2));
+    const int64_t warps = (int64_t)a->n_sm * resident_warps(a->pool->dim);
+    const int64_t chunk = a->small ? kSmallPages : std::max<int64_t>(kMinChunk, (work * n_kv + warps - 1) / warps);
     a->tokens.resize(a->node_rows.size());
     for (const Node& nd : a->nodes) {
         const int32_t n_splits = (int32_t)((nd.n_pages + chunk - 1) / chunk), per = (nd.n_pages + n_splits - 1) / n_splits;
@@ -628,6 +648,7 @@ static int64_t build_items(t2sx_plan* a) {
             a->tokens[nd.tokens_at + j].part0 = t.n_parts;   // among the token's; its own number is added below
             const int32_t seen = pages_of(t.limit) - nd.pos0 / kPoolPage;
             if (seen > 0) t.n_parts += std::min((nd.n_pages + per - 1) / per, (seen + per - 1) / per);
+            if (nd.new_pos != INT32_MAX) t.ends_here = seen > 0 && n_splits == 1;
         }
         const int64_t rows = (int64_t)nd.n_tokens * group;
         for (int32_t split = 0, pg = 0; pg < nd.n_pages; ++split, pg += per) {
@@ -638,29 +659,28 @@ static int64_t build_items(t2sx_plan* a) {
                 for (int64_t j = r / group; j <= (r + n - 1) / group; ++j) sees = std::max(sees, a->info[rows_of[j]].limit);
                 const int32_t pages = std::min(std::min(per, nd.n_pages - pg), pages_of(sees) - start / kPoolPage);
                 if (pages <= 0) continue;
-                for (int64_t j = r / group; j <= (r + n - 1) / group; ++j)
-                    if (a->info[rows_of[j]].limit > start) ++a->info[rows_of[j]].arrivals;
                 a->items.push_back({nd.tokens_at, (int32_t)r, n, nd.pages_at + pg, pages, start, split, nd.end, nd.new_pos, nd.new_row, {}});
             }
         }
     }
-    // the longest items first; pages of several sequences before all, so that a token's own pages come last and
-    // its join falls to an item of that token alone
+    // pages of several sequences first (a launch of their own), then the longest items first
     std::stable_sort(a->items.begin(), a->items.end(), [](const Item& x, const Item& y) {
         const bool sx = x.new_pos == INT32_MAX, sy = y.new_pos == INT32_MAX;
         return sx != sy ? sx : x.n_pages > y.n_pages;
     });
+    a->view.n_shared = (int)(std::find_if(a->items.begin(), a->items.end(), [](const Item& x) { return x.new_pos != INT32_MAX; }) -
+                             a->items.begin());
     int64_t parts = 0;
-    a->most_parts = 0;
     for (Token& t : a->info) {
         t.part_at = (int32_t)std::min<int64_t>(parts, INT32_MAX);
-        if (t.n_parts > 1) { a->joins.push_back(t); parts += t.n_parts; }
-        a->most_parts = std::max(a->most_parts, t.n_parts);
+        if (t.n_parts > 1) parts += t.n_parts;
+        if (t.n_parts > 1 && !t.ends_here) a->joins.push_back(t);
     }
     for (size_t i = 0; i < a->tokens.size(); ++i) {
         const int32_t ordinal = a->tokens[i].part0;
         a->tokens[i] = a->info[a->node_rows[i]];
         a->tokens[i].part0 = a->tokens[i].part_at + ordinal;
+        a->tokens[i].ends_here &= ordinal == a->tokens[i].n_parts - 1;
     }
     a->view.n_items = (int)a->items.size();
     a->view.n_joins = (int)a->joins.size();
@@ -702,6 +722,15 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
                 a->info[r] = Token{r, limit, page, 0, 0, 0, 0, 0};
             }
         }
+        // A small step: a CTA for each (tile of rows, K/V head), all at one time, with no parts to join; its shared pages
+        // come from L2 however often they are read.
+        int64_t row_tiles = 0;
+        a->small = true;
+        for (int32_t i = 0; i < n; ++i) {
+            row_tiles += ((int64_t)n_new[i] * (a->n_heads / p->n_kv) + kTileRows - 1) / kTileRows;
+            a->small &= n_new[i] == 0 || p->table[seqs[i]].size() <= (size_t)kSmallPages;
+        }
+        a->small &= row_tiles * p->n_kv <= 2 * a->n_sm;
         build_nodes(a, n, seqs, n_new);
         const int64_t n_parts = build_items(a);
         if (n_parts >= INT32_MAX || a->items.size() * p->n_kv > (size_t)INT32_MAX ||
@@ -737,9 +766,7 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
         POOL_CK(grow(a->dev, a->dev_bytes, bytes));
         // results of parts, where tokens have several
         const size_t part_rows = (size_t)n_parts * a->n_heads, o_bytes = part_rows * p->dim * 4;
-        const size_t n_arrived = !a->joins.empty() && a->most_parts <= kWarpJoin ? (size_t)rows * p->n_kv : 0;
-        POOL_CK(grow(a->work, a->work_bytes, o_bytes + part_rows * 8 + n_arrived * 4));
-        if (n_arrived) POOL_CK(cudaMemsetAsync(a->work + o_bytes + part_rows * 8, 0, n_arrived * 4, st));
+        POOL_CK(grow(a->work, a->work_bytes, o_bytes + part_rows * 8));
         auto put = [&](size_t at, auto const& v) { if (!v.empty()) memcpy(a->host[b] + at, v.data(), v.size() * sizeof(v[0])); };
         put(o_items, a->items); put(o_tokens, a->tokens); put(o_pages, a->pages); put(o_joins, a->joins);
         if (bytes) POOL_CK(cudaMemcpyAsync(a->dev, a->host[b], bytes, cudaMemcpyHostToDevice, st));
@@ -752,7 +779,6 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
         w.joins = (const Token*)(a->dev + o_joins);
         w.part_o = (float*)a->work;
         w.part_ml = (float2*)(a->work + o_bytes);
-        w.arrived = n_arrived ? (int32_t*)(a->work + o_bytes + part_rows * 8) : nullptr;
         a->version = p->version;
         a->ready = true;
         return T2SX_OK;
@@ -780,10 +806,18 @@ static cudaError_t launch_attend(t2sx_plan* a, const Tensors<T>& x, cudaStream_t
     const PlanView& w = a->view;
     using S = TileShape<D>;
     static std::once_flag once[64];
-    std::call_once(once[a->pool->device & 63],
-                   [] { cudaFuncSetAttribute(k_attend_tiles<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
-    cudaError_t e = launch(k_attend_tiles<T, D>, dim3((unsigned)(w.n_items * w.n_kv)), 32, S::SMEM, st, false, w, x);
-    if (e == cudaSuccess && w.n_joins && !w.arrived)
+    std::call_once(once[a->pool->device & 63], [] {
+        cudaFuncSetAttribute(k_attend_tiles<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::RING);
+        cudaFuncSetAttribute(k_attend_tiles<T, D, S::TEAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TEAM * S::RING);
+    });
+    if (a->small)
+        return launch(k_attend_tiles<T, D, S::TEAM>, dim3((unsigned)w.n_items * w.n_kv), 32 * S::TEAM, S::TEAM * S::RING, st, false, w, x, 0);
+    auto tiles = [&](int item0, int n, bool early) {
+        return n ? launch(k_attend_tiles<T, D, 1>, dim3((unsigned)n * w.n_kv), 32, S::RING, st, early, w, x, item0) : cudaSuccess;
+    };
+    cudaError_t e = tiles(0, w.n_shared, false);
+    if (e == cudaSuccess) e = tiles(w.n_shared, w.n_items - w.n_shared, w.n_shared > 0);
+    if (e == cudaSuccess && w.n_joins)
         e = launch(k_join_parts<T, D>, dim3((unsigned)(w.n_joins * a->n_heads)), 128, 0, st, true, w, x);
     return e;
 }
