@@ -7,10 +7,7 @@
 // and a token's result follows from its parts: M = max m_i, out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
 // The constant c keeps small weights above the subnormal numbers of f16 (and is harmless for bf16).
 // A row is a (token, query head of the K/V head's group); `group` heads of a token are neighbours.
-#include "t2sx_pool.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include "t2sx_prefix_attn.cuh"
 
 #include <algorithm>
 #include <cmath>
@@ -20,83 +17,22 @@
 #include <type_traits>
 
 using namespace t2sx;
+using namespace t2sx::attn;
+
+namespace {
 
 #ifndef C32
 #define C32 32,3,16
 #define C64 32,3,9
 #define C128 32,3,4
 #endif
-namespace {
-
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kWeightExp = 7.0f;   // c above: weights are at most 2^7
 constexpr int kTileRows = 16;        // rows of a warp's tile (the m of mma.m16n8k16)
 constexpr int kMinChunk = 2;         // pages of a split at least
+constexpr int kSplitCost = 4, kJoinCost = 4;   // in pages: what a split costs beside its pages, and joining parts
+constexpr int kTcMinRows = 64;       // rows of a node from which tiles of 128 take it
+constexpr int kTcMinChunk = 4;       // pages of a split of such a node at least
 constexpr int kSmallPages = 32;      // pages of a sequence in a small step at most
 
-// A tile of rows against a range of a node's pages.
-struct Item {
-    int32_t tokens_at;   // the node's tokens start here in `tokens`
-    int32_t row0, rows;  // rows of the node: token row / group, head row % group
-    int32_t pages_at;    // page ids
-    int32_t n_pages;
-    int32_t pos0;        // position of the first page's first key
-    int32_t split;       // which range of the node's pages this is
-    int32_t end;         // the node's filled positions end here
-    int32_t new_pos;     // from this position on the keys are the step's own (of one sequence) ...
-    int32_t new_row;     // ... and that one is this row of the step
-    int32_t pad[2];
-};
-
-// A token as one of a node's: what it is, and where its parts are.  A token's parts are numbers
-// part_at .. part_at + n_parts - 1, those of the node's splits from part0 on.
-struct alignas(16) Token {
-    int32_t row;         // of the step
-    int32_t limit;       // positions that it sees; its own is the last of them
-    int32_t page;        // page of its own position
-    int32_t part0, part_at;
-    int32_t n_parts;     // one: the item writes the result itself
-    int32_t ends_here;   // the node's item completes the token: its own part is the last one, and the others are
-                         // those of the launch before
-    int32_t pad;
-};
-
-struct PlanView {
-    const Token* tokens;     // nodes' tokens
-    const int32_t* pages;
-    const Item* items;
-    const Token* joins;      // tokens of several parts
-    float* part_o;           // [part][query head of the group][K/V head][dim]
-    float2* part_ml;         // [part][query head of the group][K/V head]
-    int rows, n_shared, n_items, n_joins, group, n_kv;   // items: first the n_shared of several sequences
-};
-
-// Strided tensors of one call.
-template <typename T>
-struct Tensors {
-    const T* q;
-    T *k, *v;                // the layer's first page
-    const T *k_new, *v_new;  // the rows' own keys and values, or null: they are in the cache
-    long long kv_stride;
-    T* out;
-    float* lse;
-    long long q_stride, out_stride;
-    float scale2;            // scale * log2(e)
-};
-
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint32_t pack2(__half, float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ void mma16816(__half, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -122,8 +58,22 @@ __device__ __forceinline__ void cp16(uint32_t smem, const void* gmem, bool real 
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void dependents_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// One 16-byte word per thread: the rows' keys and values go to their positions (for tiles of 128 rows of one
+// sequence, which read them from the cache by tensor copies).
+__global__ void __launch_bounds__(256)
+k_write_rows(const Token* __restrict__ rows_of, int rows, const uint4* __restrict__ kn, const uint4* __restrict__ vn,
+             long long stride_vec, uint4* __restrict__ k, uint4* __restrict__ v, int n_kv, int row_vec) {
+    dependents_launch();
+    const int per_row = n_kv * row_vec;
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= (long long)rows * per_row) return;
+    const int row = (int)(i / per_row), j = (int)(i - (long long)row * per_row), h = j / row_vec, c = j - h * row_vec;
+    const Token t = rows_of[row];
+    const size_t dst = (((size_t)t.page * n_kv + h) * kPoolPage + (t.limit - 1) % kPoolPage) * row_vec + c;
+    k[dst] = kn[row * stride_vec + j];
+    v[dst] = vn[row * stride_vec + j];
+}
 
 // Tiles of a head dimension: keys per stage of a warp's ring, its stages, the warps of an SM that this leaves
 // room for, and the warps of a CTA that shares out one item.
@@ -159,6 +109,7 @@ k_attend_tiles(PlanView pv, Tensors<T> x, int item0) {
     const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring) + warp * S::RING;
     const Item it = pv.items[item0 + blockIdx.x / pv.n_kv];
     const int group = pv.group;
+    dependents_launch();   // the next launch fills what this one leaves free
 
     const int all = it.n_pages * (kPoolPage / S::KEYS), first = all * warp / W, tiles = all * (warp + 1) / W;
     int page_base = first / (kPoolPage / S::KEYS);    // pages [page_base, page_base + 32) are in the lanes
@@ -325,7 +276,6 @@ k_attend_tiles(PlanView pv, Tensors<T> x, int item0) {
     if (own0) *own_dst(own0) = own_word;
     for (int r = 1; r < it.rows; ++r)
         if (const Token* t = own(r)) *own_dst(t) = *own_src(t);
-    dependents_launch();
     float sum[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -470,6 +420,7 @@ struct Node {
     int32_t pages_at, n_pages;
     int32_t pos0, end;
     int32_t new_pos, new_row;
+    bool tc;             // tiles of 128 rows
 };
 
 int resident_warps(int dim) {
@@ -487,7 +438,9 @@ int sm_count(int device) {
 struct t2sx_plan {
     t2sx_pool* pool = nullptr;
     int n_heads = 0, n_sm = 148;
-    bool ready = false, shared_rows = false, small = false;
+    bool ready = false, shared_rows = false, small = false, tc_writes = false;
+    CUtensorMap map_k, map_v;
+    int32_t *err = nullptr, *err_dev = nullptr;   // pinned: what a kernel that gave up a wait reports
     uint64_t version = 0;          // of the pool at the update
     // host copy of what the device gets, in pinned memory: two buffers, so that an update need not
     // wait for the previous one's upload
@@ -517,6 +470,7 @@ static void plan_release(t2sx_plan* a) {
     }
     if (a->dev) cudaFree(a->dev);
     if (a->work) cudaFree(a->work);
+    if (a->err) cudaFreeHost(a->err);
     delete a;
     if (--p->n_plans == 0 && p->closed) t2sx_pool_release_object(p);
 }
@@ -534,6 +488,10 @@ extern "C" int t2sx_plan_create(t2sx_pool* p, int32_t n_heads, t2sx_plan** out) 
         a->n_heads = n_heads;
         ++p->n_plans;
         a->n_sm = sm_count(p->device);
+        if (!tc_maps(p, &a->map_k, &a->map_v)) return t2sx_set_error(T2SX_ERR_CUDA, "t2sx_plan_create: the driver gives no tensor maps");
+        POOL_CK(cudaHostAlloc(&a->err, 4, cudaHostAllocMapped));
+        *a->err = 0;
+        POOL_CK(cudaHostGetDevicePointer(&a->err_dev, a->err, 0));
         for (int i = 0; i < 2; ++i) POOL_CK(cudaEventCreateWithFlags(&a->sent[i], cudaEventDisableTiming));
         *out = a.release();
         return T2SX_OK;
@@ -628,18 +586,47 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
     }
 }
 
+// Pages of a split, for the nodes of one kind: of the even divisions of the longest node, the one that ends first,
+// where a split costs its pages and as much again as kSplitCost of them, `slots` of them run at a time, and
+// they start the longest first.
+static int64_t best_chunk(const t2sx_plan* a, bool tc, int64_t slots) {
+    const int group = a->n_heads / a->pool->n_kv, tile = tc ? kTcRows : kTileRows;
+    const int64_t least = tc ? kTcMinChunk : kMinChunk;
+    int64_t longest = 0;
+    for (const Node& nd : a->nodes)
+        if (nd.tc == tc) longest = std::max<int64_t>(longest, nd.n_pages);
+    int64_t best = std::max<int64_t>(longest, 1);
+    double best_cost = 1e300;
+    for (int64_t parts = 1; parts <= 512 && (parts == 1 || (longest + parts - 1) / parts >= least); parts += parts < 32 ? 1 : parts / 16) {
+        const int64_t chunk = (longest + parts - 1) / parts;
+        int64_t items = 0, pages = 0;
+        for (const Node& nd : a->nodes) {
+            if (nd.tc != tc) continue;
+            const int64_t tiles = (nd.n_tokens * (int64_t)group + tile - 1) / tile * a->pool->n_kv;
+            items += tiles * ((nd.n_pages + chunk - 1) / chunk);
+            pages += tiles * nd.n_pages;
+        }
+        const double waves = (double)((items + slots - 1) / slots) * (chunk + kSplitCost);
+        const double even = (double)(pages + items * kSplitCost) / slots + (items > slots ? chunk : 0);
+        const double cost = std::min(waves, std::max(even, (double)(chunk + kSplitCost))) + (parts > 1 ? kJoinCost : 0);
+        if (cost < best_cost) { best_cost = cost; best = chunk; }
+    }
+    return best;
+}
+
 // Items and parts from the nodes; returns the number of parts.  A node's pages are split so that there are
 // several items for each warp that the device holds, and each part's result is small against the keys that
 // it stands for.
 static int64_t build_items(t2sx_plan* a) {
     const int group = a->n_heads / a->pool->n_kv, n_kv = a->pool->n_kv;
     a->items.clear(); a->joins.clear();
-    int64_t work = 0;
-    for (const Node& nd : a->nodes) work += (int64_t)nd.n_pages * ((nd.n_tokens * (int64_t)group + kTileRows - 1) / kTileRows);
-    const int64_t warps = (int64_t)a->n_sm * resident_warps(a->pool->dim);
-    const int64_t chunk = a->small ? kSmallPages : std::max<int64_t>(kMinChunk, (work * n_kv + warps - 1) / warps);
+    for (Node& nd : a->nodes) nd.tc = !a->small && (int64_t)nd.n_tokens * group >= kTcMinRows;
+    const int64_t warp_chunk = a->small ? kSmallPages : best_chunk(a, false, (int64_t)a->n_sm * resident_warps(a->pool->dim));
+    const int64_t tc_chunk = best_chunk(a, true, (int64_t)a->n_sm * 2);
     a->tokens.resize(a->node_rows.size());
     for (const Node& nd : a->nodes) {
+        const int64_t chunk = nd.tc ? tc_chunk : warp_chunk;
+        const int tile = nd.tc ? kTcRows : kTileRows;
         const int32_t n_splits = (int32_t)((nd.n_pages + chunk - 1) / chunk), per = (nd.n_pages + n_splits - 1) / n_splits;
         const int32_t* rows_of = a->node_rows.data() + nd.tokens_at;
         // a token has parts for the splits that begin below its limit, the first ones
@@ -648,28 +635,32 @@ static int64_t build_items(t2sx_plan* a) {
             a->tokens[nd.tokens_at + j].part0 = t.n_parts;   // among the token's; its own number is added below
             const int32_t seen = pages_of(t.limit) - nd.pos0 / kPoolPage;
             if (seen > 0) t.n_parts += std::min((nd.n_pages + per - 1) / per, (seen + per - 1) / per);
-            if (nd.new_pos != INT32_MAX) t.ends_here = seen > 0 && n_splits == 1;
+            if (nd.new_pos != INT32_MAX) t.ends_here = seen > 0 && n_splits == 1 && !nd.tc;
         }
         const int64_t rows = (int64_t)nd.n_tokens * group;
         for (int32_t split = 0, pg = 0; pg < nd.n_pages; ++split, pg += per) {
             const int32_t start = nd.pos0 + pg * kPoolPage;
-            for (int64_t r = 0; r < rows; r += kTileRows) {
-                const int32_t n = (int32_t)std::min<int64_t>(kTileRows, rows - r);
+            for (int64_t r = 0; r < rows; r += tile) {
+                const int32_t n = (int32_t)std::min<int64_t>(tile, rows - r);
                 int32_t sees = 0;
                 for (int64_t j = r / group; j <= (r + n - 1) / group; ++j) sees = std::max(sees, a->info[rows_of[j]].limit);
                 const int32_t pages = std::min(std::min(per, nd.n_pages - pg), pages_of(sees) - start / kPoolPage);
                 if (pages <= 0) continue;
-                a->items.push_back({nd.tokens_at, (int32_t)r, n, nd.pages_at + pg, pages, start, split, nd.end, nd.new_pos, nd.new_row, {}});
+                a->items.push_back({nd.tokens_at, (int32_t)r, n, nd.pages_at + pg, pages, start, split, nd.end, nd.new_pos, nd.new_row,
+                                    nd.tc ? 0 : nd.new_pos == INT32_MAX ? 1 : 2, 0});
             }
         }
     }
-    // pages of several sequences first (a launch of their own), then the longest items first
+    // by launch, the longest items first
     std::stable_sort(a->items.begin(), a->items.end(), [](const Item& x, const Item& y) {
-        const bool sx = x.new_pos == INT32_MAX, sy = y.new_pos == INT32_MAX;
-        return sx != sy ? sx : x.n_pages > y.n_pages;
+        return x.launch != y.launch ? x.launch < y.launch : x.n_pages > y.n_pages;
     });
-    a->view.n_shared = (int)(std::find_if(a->items.begin(), a->items.end(), [](const Item& x) { return x.new_pos != INT32_MAX; }) -
-                             a->items.begin());
+    int32_t n_launch[3] = {0, 0, 0};
+    a->tc_writes = false;
+    for (const Item& it : a->items) {
+        ++n_launch[it.launch];
+        a->tc_writes |= it.launch == 0 && it.new_pos != INT32_MAX;
+    }
     int64_t parts = 0;
     for (Token& t : a->info) {
         t.part_at = (int32_t)std::min<int64_t>(parts, INT32_MAX);
@@ -682,7 +673,9 @@ static int64_t build_items(t2sx_plan* a) {
         a->tokens[i].part0 = a->tokens[i].part_at + ordinal;
         a->tokens[i].ends_here &= ordinal == a->tokens[i].n_parts - 1;
     }
-    a->view.n_items = (int)a->items.size();
+    a->view.n_tc = n_launch[0];
+    a->view.n_shared = n_launch[1];
+    a->view.n_own = n_launch[2];
     a->view.n_joins = (int)a->joins.size();
     a->view.group = group;
     a->view.n_kv = n_kv;
@@ -741,7 +734,8 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
         POOL_CK(dg.set(p->device));
         size_t bytes = 0;
         auto place = [&](auto const& v) { const size_t at = bytes; bytes = (bytes + v.size() * sizeof(v[0]) + 15) & ~(size_t)15; return at; };
-        const size_t o_items = place(a->items), o_tokens = place(a->tokens), o_pages = place(a->pages), o_joins = place(a->joins);
+        if (!a->tc_writes) a->info.clear();   // the rows by themselves are needed on the device where a launch writes them
+        const size_t o_info = place(a->info), o_items = place(a->items), o_tokens = place(a->tokens), o_pages = place(a->pages), o_joins = place(a->joins);
         const int b = a->turn ^= 1;
         POOL_CK(cudaEventSynchronize(a->sent[b]));
         if (a->host_bytes[b] < bytes) {
@@ -768,11 +762,12 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
         const size_t part_rows = (size_t)n_parts * a->n_heads, o_bytes = part_rows * p->dim * 4;
         POOL_CK(grow(a->work, a->work_bytes, o_bytes + part_rows * 8));
         auto put = [&](size_t at, auto const& v) { if (!v.empty()) memcpy(a->host[b] + at, v.data(), v.size() * sizeof(v[0])); };
-        put(o_items, a->items); put(o_tokens, a->tokens); put(o_pages, a->pages); put(o_joins, a->joins);
+        put(o_info, a->info); put(o_items, a->items); put(o_tokens, a->tokens); put(o_pages, a->pages); put(o_joins, a->joins);
         if (bytes) POOL_CK(cudaMemcpyAsync(a->dev, a->host[b], bytes, cudaMemcpyHostToDevice, st));
         POOL_CK(cudaEventRecord(a->sent[b], st));
         POOL_CK(p->end(st));
         PlanView& w = a->view;
+        w.rows_of = (const Token*)(a->dev + o_info);
         w.items = (const Item*)(a->dev + o_items);
         w.tokens = (const Token*)(a->dev + o_tokens);
         w.pages = (const int32_t*)(a->dev + o_pages);
@@ -785,24 +780,8 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
     });
 }
 
-// With `early` the kernel may start while the one before it runs (it waits for it itself).
-template <typename... P, typename... A>
-static cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, bool early, A&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = threads;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = early ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
-}
-
 template <typename T, int D>
-static cudaError_t launch_attend(t2sx_plan* a, const Tensors<T>& x, cudaStream_t st) {
+static cudaError_t launch_attend(t2sx_plan* a, Tensors<T> x, int layer, cudaStream_t st) {
     const PlanView& w = a->view;
     using S = TileShape<D>;
     static std::once_flag once[64];
@@ -811,12 +790,28 @@ static cudaError_t launch_attend(t2sx_plan* a, const Tensors<T>& x, cudaStream_t
         cudaFuncSetAttribute(k_attend_tiles<T, D, S::TEAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TEAM * S::RING);
     });
     if (a->small)
-        return launch(k_attend_tiles<T, D, S::TEAM>, dim3((unsigned)w.n_items * w.n_kv), 32 * S::TEAM, S::TEAM * S::RING, st, false, w, x, 0);
+        return launch(k_attend_tiles<T, D, S::TEAM>, dim3((unsigned)w.n_own * w.n_kv), 32 * S::TEAM, S::TEAM * S::RING, st, false, w, x, 0);
     auto tiles = [&](int item0, int n, bool early) {
         return n ? launch(k_attend_tiles<T, D, 1>, dim3((unsigned)n * w.n_kv), 32, S::RING, st, early, w, x, item0) : cudaSuccess;
     };
-    cudaError_t e = tiles(0, w.n_shared, false);
-    if (e == cudaSuccess) e = tiles(w.n_shared, w.n_items - w.n_shared, w.n_shared > 0);
+    cudaError_t e = cudaSuccess;
+    bool early = false;   // a launch of this call comes before
+    if (w.n_tc) {
+        if (x.k_new && a->tc_writes) {
+            const int row_vec = D * 2 / 16;
+            const int64_t vecs = (int64_t)w.rows * w.n_kv * row_vec;
+            k_write_rows<<<(unsigned)((vecs + 255) / 256), 256, 0, st>>>(w.rows_of, w.rows, (const uint4*)x.k_new, (const uint4*)x.v_new,
+                                                                        x.kv_stride / 8, (uint4*)x.k, (uint4*)x.v, w.n_kv, row_vec);
+            e = cudaGetLastError();
+            x.k_new = x.v_new = nullptr;
+            early = true;
+        }
+        if (e == cudaSuccess) e = launch_tc(w, x, a->pool, a->map_k, a->map_v, layer * a->pool->n_pages, a->err_dev, early, st);
+        early = true;
+    }
+    if (e == cudaSuccess) e = tiles(w.n_tc, w.n_shared, early);
+    early |= w.n_shared > 0;
+    if (e == cudaSuccess) e = tiles(w.n_tc + w.n_shared, w.n_own, early);
     if (e == cudaSuccess && w.n_joins)
         e = launch(k_join_parts<T, D>, dim3((unsigned)(w.n_joins * a->n_heads)), 128, 0, st, true, w, x);
     return e;
@@ -829,9 +824,24 @@ static cudaError_t attend(t2sx_plan* a, int32_t layer, const void* q, int64_t q_
     const size_t first = (size_t)layer * p->n_pages * p->n_kv * kPoolPage * p->dim;
     const Tensors<T> x = {(const T*)q, (T*)p->k + first, (T*)p->v + first, (const T*)k_new, (const T*)v_new, kv_stride,
                           (T*)out, lse, q_stride, out_stride, scale * kLog2e};
-    if (p->dim == 32) return launch_attend<T, 32>(a, x, st);
-    if (p->dim == 64) return launch_attend<T, 64>(a, x, st);
-    return launch_attend<T, 128>(a, x, st);
+    if (p->dim == 32) return launch_attend<T, 32>(a, x, layer, st);
+    if (p->dim == 64) return launch_attend<T, 64>(a, x, layer, st);
+    return launch_attend<T, 128>(a, x, layer, st);
+}
+
+static int plan_error(t2sx_plan* a) {
+    volatile int32_t* e = a->err;
+    if (!*e) return T2SX_OK;
+    *e = 0;
+    return t2sx_set_error(T2SX_ERR_TIMEOUT, "a tensor-core attention of this plan gave up waiting; its outputs are NaN");
+}
+
+extern "C" int t2sx_plan_sync(t2sx_plan* a) {
+    if (!a) return bad("t2sx_plan_sync: null plan");
+    DeviceGuard dg;
+    POOL_CK(dg.set(a->pool->device));
+    if (a->pool->worked) POOL_CK(cudaEventSynchronize(a->pool->done));
+    return plan_error(a);
 }
 
 extern "C" int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, int64_t q_stride, const void* k_new_dev,
@@ -853,6 +863,7 @@ extern "C" int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, 
         return bad("t2sx_plan_attend: tensors must be 16-byte aligned");
     if (k_new_dev && a->shared_rows)
         return t2sx_set_error(T2SX_ERR_STATE, "t2sx_plan_attend: a row's position is in a page of several sequences, which is not written");
+    if (int rc = plan_error(a)) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     DeviceGuard dg;
     POOL_CK(dg.set(p->device));

@@ -32,6 +32,7 @@
 #include "t2sx_kernels.cuh"
 #include "t2sx_math.cuh"
 #include "t2sx_kv.cuh"
+#include "t2sx_tcgen.cuh"
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -72,52 +73,6 @@ constexpr int SMEM = 1024 + NS * STAGE + OUT_BYTES + DX_BYTES + KVB_BYTES + BAR_
 // result, read as a float, is 12582912 + S exactly (|S| < 2^22), so float(S) is one subtraction.
 constexpr int kMagic = 0x4B400000;
 constexpr float kMagicF = 12582912.0f;
-constexpr long long kSpinCycles = 2000000000LL;   // bound of one wait (~1 s at 1.9 GHz)
-// Value the kernel stores into its error word when a CTA gave up waiting (the session's bounds
-// checks store 1 into the same word).
-constexpr int kErrTimeout = 3;
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Wait for the phase of the given parity; false when the CTA aborted or the wait ran out after
-// `limit` cycles (kSpinCycles unless a test shortened it).
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit) {
-    long long t0 = 0;
-    for (uint32_t it = 0;; ++it) {
-        if (bar_try(bar, parity)) return true;
-        if ((it & 31) == 31) {
-            if (*abort_flag) return false;
-            const long long now = clock64();
-            if (t0 == 0) t0 = now;
-            else if (now - t0 > limit) { *abort_flag = 1; return false; }
-        }
-    }
-}
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
-        ::"r"(dst), "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
 
 // barrier of the 8 epilogue warps only (named barrier 1)
 // tensor store of one box from shared memory (x, y >= 0; x * element size a multiple of 16 bytes;
@@ -127,13 +82,6 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int 
                  "r"(y), "r"(smem_u32(ssrc))
                  : "memory");
 }
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
-// this thread's tensor stores have read their shared-memory source
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory"); }
-// this thread's tensor stores have completed
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
-// shared-memory writes of this thread become visible to the tensor-store (async) proxy
-__device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;\n" ::"n"(32 * EPI_WARPS) : "memory"); }
 // the same barrier, returning the OR of v over the 8 warps (one decision for all of them)
 __device__ __forceinline__ bool epi_sync_or(bool v) {
@@ -143,11 +91,6 @@ __device__ __forceinline__ bool epi_sync_or(bool v) {
                  : "r"((uint32_t)v), "n"(32 * EPI_WARPS)
                  : "memory");
     return r != 0;
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
 }
 // D[tmem] (=|+=) A[smem] . B[smem]^T, s8 x s8 -> s32
 __device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {

@@ -84,6 +84,7 @@ SIGNATURES = {
     "t2sx_plan_free": (None, [_P]),
     "t2sx_plan_update": (C.c_int, [_P, _I, _P, _P, _P]),
     "t2sx_plan_attend": (C.c_int, [_P, _I, _P, _I64, _P, _P, _I64, _F, _P, _I64, _P, _P]),
+    "t2sx_plan_sync": (C.c_int, [_P]),
     "t2sx_token_logprobs": (C.c_int, [_I, _I, _I64, _I64, _P, _I64, _P, _I, _P, _P, _P, _P, _P, _P]),
 }
 NOALLOC_MAX_ELEMS = 1 << 21
@@ -560,6 +561,11 @@ class AttnPlan:
         _ck(lib().t2sx_plan_attend(self.h, layer, q_ptr, row if q_stride is None else q_stride, k_new_ptr, v_new_ptr,
                                    self.pool.n_kv_heads * dim if kv_stride is None else kv_stride, scale, out_ptr,
                                    row if out_stride is None else out_stride, lse_ptr, stream))
+
+    def sync(self):
+        """Waits for the pool's device work; raises T2SXError(ERR_TIMEOUT) if an attend() gave up a bounded
+        wait since the last report (its outputs are then NaN)."""
+        _ck(lib().t2sx_plan_sync(self.h))
 
     def close(self):
         if self.h:

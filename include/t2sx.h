@@ -196,7 +196,7 @@ T2SX_API int t2sx_matmul(t2sx_weight* w, const float* x_dev, int64_t M, const fl
  * bounded wait (T2SX_ERR_TIMEOUT; its outputs are NaN); clears that state.  The reference has no
  * counterpart (ggml's CPU kernels do not wait on anything). */
 T2SX_API int t2sx_weight_sync(t2sx_weight* w, void* stream);
-/* Test hook, no counterpart in the reference.  cycles > 0: tensor-core matmuls launched (or
+/* Test hook, no counterpart in the reference.  cycles > 0: tensor-core kernels launched (or
  * graphs captured) from now on first wait on a barrier that nothing completes, and every wait of
  * theirs is bounded by `cycles` clock cycles, so the wait runs out and the error path is taken
  * (outputs NaN, T2SX_ERR_TIMEOUT); 0 restores normal operation with the built-in bound of about
@@ -317,6 +317,11 @@ T2SX_API int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, cons
 T2SX_API int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, int64_t q_stride, const void* k_new_dev,
                               const void* v_new_dev, int64_t kv_stride, float scale, void* out_dev, int64_t out_stride,
                               float* lse_dev, void* stream);
+
+/* Waits for the pool's device work and reports whether a tensor-core attention of this plan since the last
+ * report gave up a bounded wait (T2SX_ERR_TIMEOUT; its outputs are NaN).  attend reports it too, if it
+ * is known by then. */
+T2SX_API int t2sx_plan_sync(t2sx_plan* a);
 
 /* Scores of given tokens under rows of logits (f32, f16 or bf16; stride elements apart):
  * logprob [rows]: log softmax of the row at tokens[r]; entropy [rows] (nats); rank [rows]: how many

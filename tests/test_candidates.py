@@ -424,6 +424,71 @@ def test_plan_outlives_pool_and_updates_grow(t2sx_mod):
     plan.close()
 
 
+@gpu
+@pytest.mark.parametrize("dtype,heads,kv,dim", SHAPES)
+def test_attend_again_and_again(t2sx_mod, dtype, heads, kv, dim):
+    """Many rows of shared and of own pages, one to three pages to a tile: every call gives the same bits, also
+    with other work between the calls."""
+    _need_gpu()
+    c = Cache(t2sx_mod, dtype, 1, 400, kv, dim, 90)
+    c.extend(0, 190)
+    c.derive("fork", [0] * 80, list(range(1, 81)))
+    for s in range(1, 81):
+        c.extend(s, 1 + s * 7 % 90)
+    c.extend(85, 170)
+    seqs, new = list(range(1, 81)) + [85], [1] * 80 + [130]
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q = torch.randn((sum(new), heads, dim), generator=gen, device="cuda").to(TORCH[dtype])
+    plan = c.pool.plan(heads)
+    plan.update(seqs, new, _stream())
+    outs = []
+    for i in range(12):
+        out = torch.full_like(q, 7.0)
+        plan.attend(0, q.data_ptr(), out.data_ptr(), 0.2, stream=_stream())
+        outs.append(out)
+        if i % 3 == 0:
+            torch.empty(1 << 26, device="cuda").fill_(1.0)   # what the caches held is gone
+    ref, mag, _ = _reference(c, 0, seqs, new, q, heads, 0.2)
+    u = UNIT[dtype]
+    for out in outs:
+        assert torch.equal(out.view(torch.int16), outs[0].view(torch.int16))
+        assert ((out.double() - ref).abs() <= u * (mag + ref.abs()) + 2.0 ** -14 * mag + 2.0 ** -24).all()
+    plan.sync()
+
+
+@gpu
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_attend_wait_timeout_reported_and_recovered(t2sx_mod, dim):
+    """A wait that nothing ends runs out: NaN outputs and a status, and the next calls are right again."""
+    _need_gpu()
+    c = Cache(t2sx_mod, 1, 1, 40, 8, dim, 3)
+    c.extend(0, 700)
+    q = torch.randn((300, 16, dim), device="cuda").half()
+    out = torch.zeros_like(q)
+    plan = c.pool.plan(16)
+    plan.update([0], [300], _stream())
+    call = lambda: plan.attend(0, q.data_ptr(), out.data_ptr(), 0.1, stream=_stream())
+    try:
+        t2sx_mod.test_set_tc_wait_cycles(100_000)
+        call()
+        with pytest.raises(t2sx_mod.T2SXError) as e:
+            plan.sync()
+        assert e.value.code == t2sx_mod.ERR_TIMEOUT
+        assert out.isnan().any()
+        call()
+        torch.cuda.synchronize()
+        with pytest.raises(t2sx_mod.T2SXError) as e:
+            call()
+        assert e.value.code == t2sx_mod.ERR_TIMEOUT
+    finally:
+        t2sx_mod.test_set_tc_wait_cycles(0)
+    for _ in range(2):
+        call()
+        plan.sync()
+        ref, mag, _ = _reference(c, 0, [0], [300], q, 16, 0.1)
+        assert ((out.double() - ref).abs() <= 2.0 ** -11 * (mag + ref.abs()) + 2.0 ** -14 * mag + 2.0 ** -24).all()
+
+
 # ---- log probabilities -----------------------------------------------------------------------------------
 
 def _scores(t2sx, x, tokens, top, stream=None):
