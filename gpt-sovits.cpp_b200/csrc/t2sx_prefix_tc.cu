@@ -277,7 +277,7 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
             }
             __syncwarp();
         }
-        if (lane == 0) {   // MMAs under way read shared memory and write TMEM: the CTA ends after them
+        if (lane == 0) {   // all MMAs: the output is whole, and nothing reads shared memory any more
             tc_commit(end_bar);
             const long long t0 = clock64();
             while (!bar_try(end_bar, 0) && clock64() - t0 < kSpinCycles) {}
@@ -347,11 +347,10 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
             tc_fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(p_full(b));
+            __syncwarp();
         }
-        // The last score tile came after the output of page n - 3, so two phases may be outstanding: a wait by parity
-        // tells only neighbouring ones apart, and they are waited for one after the other.
-        if (!gone && n > 1 && !warp_wait(o_done, n & 1, abort_flag, spin)) gone = true;
-        if (!gone && !warp_wait(o_done, (n - 1) & 1, abort_flag, spin)) gone = true;
+        // (not o_done: two of its phases may be outstanding here, which a wait by parity does not tell apart)
+        if (!gone && !warp_wait(end_bar, 0, abort_flag, spin)) gone = true;
         tc_fence_after();
         gone = __any_sync(~0u, gone);
         const bool counts = live && tok.limit > it.pos0, whole = tok.n_parts == 1;
