@@ -29,7 +29,7 @@ namespace {
 constexpr int kTileRows = 16;        // rows of a warp's tile (the m of mma.m16n8k16)
 constexpr int kMinChunk = 2;         // pages of a split at least
 constexpr int kSplitCost = 4, kJoinCost = 4;   // in pages: what a split costs beside its pages, and joining parts
-constexpr int kTcMinRows = 64;       // rows of a node from which tiles of 128 take it
+constexpr int kTcMinRows = 64;       // rows of a node from which the tcgen05 kernel takes it
 constexpr int kTcMinChunk = 4;       // pages of a split of such a node at least
 constexpr int kSmallPages = 32;      // pages of a sequence in a small step at most
 
@@ -59,8 +59,8 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// One 16-byte word per thread: the rows' keys and values go to their positions (for tiles of 128 rows of one
-// sequence, which read them from the cache by tensor copies).
+// One 16-byte word per thread: the rows' keys and values go to their positions (for the tcgen05 kernel on pages of one
+// sequence, which reads them from the cache by tensor copies).
 __global__ void __launch_bounds__(256)
 k_write_rows(const Token* __restrict__ rows_of, int rows, const uint4* __restrict__ kn, const uint4* __restrict__ vn,
              long long stride_vec, uint4* __restrict__ k, uint4* __restrict__ v, int n_kv, int row_vec) {
@@ -349,14 +349,13 @@ k_attend_tiles(PlanView pv, Tensors<T> x, int item0) {
                 }
             }
         }
-        const float inv = sum[i] > 0.0f ? 1.0f / sum[i] : 0.0f;
+        const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
         uint32_t* dst = reinterpret_cast<uint32_t*>(x.out + row_of[i] * x.out_stride + head_of[i] * D);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
             if (mine(d)) dst[d * 4 + lane % 4] = pack2(T(), o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
         if (x.lse && lane % 4 == 0 && warp == 0)
-            x.lse[(size_t)row_of[i] * (pv.n_kv * group) + head_of[i]] =
-                sum[i] > 0.0f ? (m[i] - kWeightExp + log2f(sum[i])) * kLn2 : -INFINITY;
+            x.lse[(size_t)row_of[i] * (pv.n_kv * group) + head_of[i]] = (m[i] - kWeightExp + log2f(sum[i])) * kLn2;
     }
 }
 
@@ -406,10 +405,10 @@ k_join_parts(PlanView pv, Tensors<T> x) {
         acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
         l += sl[j];
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     reinterpret_cast<uint2*>(x.out + row * x.out_stride + head * D)[tid] =
         make_uint2(pack2(T(), acc.x * inv, acc.y * inv), pack2(T(), acc.z * inv, acc.w * inv));
-    if (x.lse && tid == 0) x.lse[(size_t)row * heads + head] = l > 0.0f ? (M - kWeightExp + log2f(l)) * kLn2 : -INFINITY;
+    if (x.lse && tid == 0) x.lse[(size_t)row * heads + head] = (M - kWeightExp + log2f(l)) * kLn2;
 }
 
 int bad(const char* m) { return t2sx_set_error(T2SX_ERR_INVALID, m); }
@@ -420,7 +419,7 @@ struct Node {
     int32_t pages_at, n_pages;
     int32_t pos0, end;
     int32_t new_pos, new_row;
-    bool tc;             // tiles of 128 rows
+    bool tc;             // for the tcgen05 kernel
 };
 
 int resident_warps(int dim) {
@@ -622,7 +621,7 @@ static int64_t build_items(t2sx_plan* a) {
     a->items.clear(); a->joins.clear();
     for (Node& nd : a->nodes) nd.tc = !a->small && (int64_t)nd.n_tokens * group >= kTcMinRows;
     const int64_t warp_chunk = a->small ? kSmallPages : best_chunk(a, false, (int64_t)a->n_sm * resident_warps(a->pool->dim));
-    const int64_t tc_chunk = best_chunk(a, true, (int64_t)a->n_sm * 2);
+    const int64_t tc_chunk = best_chunk(a, true, a->n_sm);
     a->tokens.resize(a->node_rows.size());
     for (const Node& nd : a->nodes) {
         const int64_t chunk = nd.tc ? tc_chunk : warp_chunk;

@@ -25,7 +25,7 @@ struct Item {
     int32_t end;         // the node's filled positions end here
     int32_t new_pos;     // from this position on the keys are the step's own (of one sequence) ...
     int32_t new_row;     // ... and that one is this row of the step
-    int32_t launch;      // 0: tiles of 128 rows, 1: pages of several sequences, 2: the others
+    int32_t launch;      // 0: tcgen05, 1: pages of several sequences, 2: the others
     int32_t pad;
 };
 
@@ -50,7 +50,7 @@ struct PlanView {
     float* part_o;           // [part][query head of the group][K/V head][dim]
     float2* part_ml;         // [part][query head of the group][K/V head]
     const Token* rows_of;    // the step's rows (for a launch that writes their keys and values)
-    // items: n_tc tiles of 128 rows, then n_shared of pages of several sequences, then n_own others
+    // items: n_tc of up to kTcRows rows, then n_shared of pages of several sequences, then n_own others
     int rows, n_tc, n_shared, n_own, n_joins, group, n_kv;
 };
 
@@ -99,8 +99,8 @@ cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cu
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
 }
 
-// Tiles of kTcRows rows on the tcgen05 tensor cores (t2sx_prefix_tc.cu).
-constexpr int kTcRows = 128;
+// Items of up to kTcRows rows on the tcgen05 tensor cores (t2sx_prefix_tc.cu).
+constexpr int kTcRows = 256;
 bool tc_maps(const t2sx_pool* p, CUtensorMap* k, CUtensorMap* v);
 template <typename T>
 cudaError_t launch_tc(const PlanView& w, const Tensors<T>& x, const t2sx_pool* p, const CUtensorMap& k, const CUtensorMap& v, int layer_page,

@@ -1,16 +1,19 @@
 // Attention over shared pages for many rows: tiles of 128 rows on the tcgen05 tensor cores.
 //
-// A CTA takes 128 rows (tokens x query heads of one K/V head's group) against a range of pages, one page
-// (64 keys) at a time:
-//   warps 0-3  the softmax, one row per thread: scores from TMEM, running maximum and sum, weights back to
+// A CTA, one per SM, has two tiles of 128 rows (tokens x query heads of one K/V head's group) and a range of
+// pages, and takes one page (64 keys) at a time.  An item of more than 128 rows fills both tiles, and each
+// page's K and V serve both; a smaller one is in both, with every second page, and the two results are joined
+// at the end.
+//   warps 0-7  the softmax, one row per thread: scores from TMEM, running maximum and sum, weights back to
 //              TMEM in 16 bits.  The accumulated output is rescaled only when the maximum grows by more than
 //              2^8 (the weights then stay below 2^15, in the range of f16);
-//   warp 4     TMA: the K and V tiles of a page, in two rings;
-//   warp 5     the MMAs: S = Q K^T (M 128, N 64) into one of two score buffers, then O += P V with P from TMEM
-//              (M 128, N head dim).  S of the next page is issued before O of this one, so that the tensor
-//              cores work while the softmax does.
-// Two CTAs share an SM (96 KB of shared memory and 256 TMEM columns each), one's softmax over the other's MMAs.
-// TMEM columns: scores and weights 2 x 64, output from column 128 on.
+//   warp 8     TMA: the K and V tiles of the pages, in two rings;
+//   warps 9-10 the MMAs, one thread for each tile: S = Q K^T (M 128, N 64) into one of two score buffers of a tile, then O += P V with P from
+//              TMEM (M 128, N head dim).  S is issued two pages ahead, so that the tensor cores work while
+//              the softmax does.
+// TMEM columns of a tile: scores and weights 2 x 64, output from column 128 on.
+// Two tiles to a CTA because the L2 cache bounds the traffic: with one tile each and two CTAs per SM a tile
+// waited 600 cycles of 1700 for its keys.
 //
 // Every wait is bounded; a CTA whose wait runs out raises its abort flag, lets its copies and MMAs land, writes
 // NaN and sets the plan's error word.
@@ -26,18 +29,20 @@ namespace {
 using namespace tc;
 
 constexpr int kKeys = kPoolPage;      // keys of a tile
-constexpr int kSoftWarps = 4, kTmaWarp = 4, kMmaWarp = 5, kThreads = 192;
-constexpr int kTmemCols = 256, kOutCol = 2 * kKeys;
+constexpr int kTileM = kTcRows / 2;   // rows of a tile
+constexpr int kSoftWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kThreads = 352;   // one MMA warp per tile
+constexpr int kTileCols = 256, kTmemCols = 2 * kTileCols, kOutCol = 2 * kKeys;
 constexpr float kHeadroom = 8.0f;     // log2 of how far weights may pass those of the reference maximum
 
 template <int D>
 struct TcShape {
-    static constexpr int STAGES = D == 128 ? 2 : 4;
+    static constexpr int STAGES = D == 128 ? 5 : 8;
     static constexpr int PITCH = D == 32 ? 64 : 128;               // bytes of a row of a swizzled block
     static constexpr int HALVES = D == 128 ? 2 : 1;                // blocks of 64 dims
-    static constexpr int TILE = kKeys * D * 2, Q = kTcRows * D * 2;
-    static constexpr int BARS = 4 * STAGES + 2 + 2 + 3;            // K, V full and empty; scores; weights; output, end, stall
-    static constexpr int SMEM = 1024 + Q + 2 * STAGES * TILE + BARS * 8 + 16;
+    static constexpr int TILE = kKeys * D * 2, Q = kTileM * D * 2;
+    static constexpr int BARS = 4 * STAGES + 2 * (2 + 2 + 1) + 4;  // K, V full and empty; a tile's scores, weights, output; end, stall, tail, zero
+    static constexpr int SMEM = 1024 + 2 * Q + 2 * STAGES * TILE + BARS * 8 + kTileM * 8 + 16;
+    static_assert(2 * STAGES * TILE >= 2 * kTileM * (D + 4) * 4, "the tiles' outputs take the place of the rings");
 };
 
 // Shared-memory descriptor of an operand whose rows are PITCH bytes, swizzled within them; groups of eight rows
@@ -53,7 +58,7 @@ __device__ __forceinline__ uint64_t operand(uint32_t saddr, uint32_t lead) {
 template <typename T>
 constexpr uint32_t instr(int n, bool b_mn) {
     const uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
-    return (1u << 4) | (type << 7) | (type << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTcRows >> 4) << 24);
+    return (1u << 4) | (type << 7) | (type << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
 }
 
 // D[tmem] (=|+=) A[smem] . B[smem]
@@ -114,41 +119,60 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     return *reinterpret_cast<float2*>(&r);
 }
 
+// True in one lane of the warp, the leader.  The compiler knows that only one thread passes, and needs no loop around
+// the instructions that take their operands from uniform registers.
+__device__ __forceinline__ bool elect_one(uint32_t& leader) {
+    uint32_t r;
+    asm volatile("{\n.reg .pred p;\nelect.sync %1|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r), "=r"(leader));
+    return r != 0;
+}
 // bar_wait of a whole warp: one answer for all of its lanes
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit) {
     return __all_sync(~0u, bar_wait(bar, parity, abort_flag, limit));
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, 1)
 k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, PlanView pv, Tensors<T> x, int layer_page,
             int32_t* err, long long spin, int stall) {
     using S = TcShape<D>;
     constexpr int NS = S::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    const uint32_t sq = smem_u32(smem), sk = sq + S::Q, sv = sk + NS * S::TILE, bars = sv + NS * S::TILE;
-    uint8_t* tail = smem + S::Q + 2 * NS * S::TILE + S::BARS * 8;
-    uint32_t* tmem_holder = (uint32_t*)tail;
-    volatile int* abort_flag = (volatile int*)(tail + 4);
+    uint8_t* rings = smem + 2 * S::Q;
+    const uint32_t sq = smem_u32(smem), sk = smem_u32(rings), sv = sk + NS * S::TILE, bars = sv + NS * S::TILE;
+    float2* tile1_ml = (float2*)(rings + 2 * NS * S::TILE + S::BARS * 8);
+    uint32_t* tmem_holder = (uint32_t*)(tile1_ml + kTileM);
+    volatile int* abort_flag = (volatile int*)(tmem_holder + 1);
     auto k_full = [&](int s) { return bars + 8 * s; };
     auto k_empty = [&](int s) { return bars + 8 * (NS + s); };
     auto v_full = [&](int s) { return bars + 8 * (2 * NS + s); };
     auto v_empty = [&](int s) { return bars + 8 * (3 * NS + s); };
-    auto s_full = [&](int b) { return bars + 8 * (4 * NS + b); };
-    auto p_full = [&](int b) { return bars + 8 * (4 * NS + 2 + b); };
-    const uint32_t o_done = bars + 8 * (4 * NS + 4), end_bar = o_done + 8, stall_bar = o_done + 16;
+    auto s_full = [&](int tile, int b) { return bars + 8 * (4 * NS + tile * 5 + b); };
+    auto p_full = [&](int tile, int b) { return bars + 8 * (4 * NS + tile * 5 + 2 + b); };
+    auto o_done = [&](int tile) { return bars + 8 * (4 * NS + tile * 5 + 4); };
+    const uint32_t end_bar = bars + 8 * (4 * NS + 10), stall_bar = end_bar + 8, tail_bar = end_bar + 16, zero_bar = end_bar + 24;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int kvh = blockIdx.x % pv.n_kv, group = pv.group;
     const Item it = pv.items[blockIdx.x / pv.n_kv];
-    const int n = it.n_pages, soft_warps = (it.rows + 31) / 32;
+    const bool alternate = it.rows <= kTileM;   // both tiles have the item's rows, and every second page
+    const int n = it.n_pages;
+    // a tile's pages are numbers 0 .. pages_of_tile - 1: which one of the item's
+    auto tile_pages = [&](int tile) { return alternate ? (n - tile + 1) / 2 : n; };
+    auto tile_rows = [&](int tile) { return alternate ? it.rows : min(kTileM, it.rows - tile * kTileM); };
+    auto nth = [&](int tile, int k) { return alternate ? 2 * k + tile : k; };
     if (tid == 0) {
-        for (int s = 0; s < NS; ++s) { bar_init(k_full(s), 1); bar_init(k_empty(s), 1); bar_init(v_full(s), 1); bar_init(v_empty(s), 1); }
-        for (int b = 0; b < 2; ++b) { bar_init(s_full(b), 1); bar_init(p_full(b), soft_warps); }
-        bar_init(o_done, 1);
-        bar_init(end_bar, 1);
+        const int users = alternate ? 1 : 2;   // tiles that read a page
+        for (int s = 0; s < NS; ++s) { bar_init(k_full(s), 1); bar_init(k_empty(s), users); bar_init(v_full(s), 1); bar_init(v_empty(s), users); }
+        for (int tile = 0; tile < 2; ++tile) {
+            for (int b = 0; b < 2; ++b) { bar_init(s_full(tile, b), 1); bar_init(p_full(tile, b), (tile_rows(tile) + 31) / 32); }
+            bar_init(o_done(tile), 1);
+        }
+        bar_init(end_bar, 2);
         bar_init(stall_bar, 1);   // no thread ever arrives on it
+        bar_init(tail_bar, 1);
+        bar_init(zero_bar, 31);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -157,22 +181,28 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     // Q, row by row: a negative scale goes into its signs, a zero one makes it zero
-    const int mr = it.row0 + tid, g = mr % group;
-    const bool live = warp < kSoftWarps && tid < it.rows;
+    const int tile = (warp >> 2) & 1, r = tid & (kTileM - 1);   // of a softmax thread
+    const int mr = it.row0 + r + (alternate ? 0 : tile * kTileM), g = mr % group;
+    const bool live = warp < kSoftWarps && r < tile_rows(tile);
     Token tok = {};
     if (live) tok = pv.tokens[it.tokens_at + mr / group];
     const int head = kvh * group + g;
     dependents_wait();     // the step's own keys and values
     dependents_launch();   // not before: the launch after this one reads them, too
-    if (warp < kSoftWarps) {
-        const uint4* src = reinterpret_cast<const uint4*>(x.q + tok.row * x.q_stride + head * D);
+    if (warp < kSoftWarps && !(alternate && tile == 1)) {
+        // a warp's 32 rows, neighbouring lanes on neighbouring 16-byte words of a row
+        constexpr int W = D / 8, R = 32 / W;
         const uint32_t flip = x.scale2 < 0.0f ? 0x80008000u : 0u, keep = x.scale2 != 0.0f ? 0xFFFFFFFFu : 0u;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-            uint4 w = live ? src[c] : make_uint4(0, 0, 0, 0);
+        const int c = lane % W;
+        const T* mine = x.q + tok.row * x.q_stride + head * D;
+#pragma unroll 8
+        for (int i = 0; i < 32; i += R) {
+            const int from = i + lane / W, rr = (warp & 3) * 32 + from;
+            const uint4* src = reinterpret_cast<const uint4*>(__shfl_sync(~0u, (unsigned long long)mine, from));
+            uint4 w = rr < tile_rows(tile) ? src[c] : make_uint4(0, 0, 0, 0);
             w.x = (w.x ^ flip) & keep; w.y = (w.y ^ flip) & keep; w.z = (w.z ^ flip) & keep; w.w = (w.w ^ flip) & keep;
-            const int at = D == 32 ? tid * 64 + ((c ^ (tid >> 1)) & 3) * 16 : (c >> 3) * (kTcRows * 128) + tid * 128 + ((c ^ tid) & 7) * 16;
-            *reinterpret_cast<uint4*>(smem + at) = w;
+            const int at = D == 32 ? rr * 64 + ((c ^ (rr >> 1)) & 3) * 16 : (c >> 3) * (kTileM * 128) + rr * 128 + ((c ^ rr) & 7) * 16;
+            *reinterpret_cast<uint4*>(smem + tile * S::Q + at) = w;
         }
         fence_proxy_async_smem();
     }
@@ -182,7 +212,6 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     const uint32_t tmem = *tmem_holder;
     const float scale = x.scale2 == 0.0f ? 1.0f : fabsf(x.scale2);
 
-    float m = -INFINITY, l = 0.0f;
     bool gone = false;
     if (warp == kTmaWarp) {
         // ---- copies ----
@@ -230,68 +259,80 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
             }
         }
         __syncwarp();
-    } else if (warp == kMmaWarp) {
-        // ---- MMAs ----
+    } else if (warp >= kMmaWarp) {
+        // ---- MMAs: one thread for each tile ----
         constexpr uint32_t idesc_s = instr<T>(kKeys, false), idesc_o = instr<T>(D, true);
-        auto scores = [&](int j) {   // S(j) = Q K(j)^T
-            const int s = j % NS;
-            if (!warp_wait(k_full(s), (j / NS) & 1, abort_flag, spin)) return false;
-            tc_fence_after();
-            if (lane == 0) {
+        const int tile = warp - kMmaWarp, nt = tile_pages(tile);
+        const int filled = it.end - (it.pos0 + (n - 1) * kKeys), last = (n - 1) % NS;
+        const bool clears = filled < kKeys && (alternate ? tile == ((n - 1) & 1) : tile == 0);   // this warp's lanes see to the rest
+        uint32_t leader;
+        if (elect_one(leader)) {
+            const uint64_t q_desc = operand<S::PITCH>(sq + (alternate ? 0 : tile * S::Q), 16), k_desc = operand<S::PITCH>(sk, 16),
+                           v_desc = operand<S::PITCH>(sv, kKeys * 128);
+            const uint32_t cols = tmem + tile * kTileCols;
+            auto scores = [&](int k) {   // S = Q K^T of the tile's k-th page
+                const int j = nth(tile, k), s = j % NS;
+                if (!bar_wait(k_full(s), (j / NS) & 1, abort_flag, spin)) return false;
+                const uint64_t kd = k_desc + s * (S::TILE >> 4);
+                const uint32_t d = cols + (k & 1) * kKeys;
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t qa = sq + (k / 4) * (D == 32 ? 0 : kTcRows * 128) + (k % 4) * 32;
-                    const uint32_t ka = sk + s * S::TILE + (k / 4) * (D == 32 ? 0 : kKeys * 128) + (k % 4) * 32;
-                    mma_ss(tmem + (j & 1) * kKeys, operand<S::PITCH>(qa, 16), operand<S::PITCH>(ka, 16), idesc_s, k > 0);
-                }
+                for (int i = 0; i < D / 16; ++i)
+                    mma_ss(d, q_desc + (((i / 4) * (kTileM * 128) + (i % 4) * 32) >> 4), kd + (((i / 4) * (kKeys * 128) + (i % 4) * 32) >> 4), idesc_s,
+                           i > 0);
+                tc_commit(s_full(tile, k & 1));
                 tc_commit(k_empty(s));
-                tc_commit(s_full(j & 1));
-            }
-            __syncwarp();
-            return true;
-        };
-        gone = !scores(0);
-        for (int j = 0; j < n && !gone; ++j) {
-            if (j + 1 < n && !scores(j + 1)) { gone = true; break; }
-            const int s = j % NS;
-            if (!warp_wait(v_full(s), (j / NS) & 1, abort_flag, spin)) { gone = true; break; }
-            const int filled = it.end - (it.pos0 + j * kKeys);
-            if (filled < kKeys) {
-                // what stands beyond the filled positions may be NaN: as values (times the weight 0) it counts 0
-                uint8_t* vt = smem + S::Q + NS * S::TILE + s * S::TILE;
-                for (int h = 0; h < S::HALVES; ++h)
-                    for (int b = filled * S::PITCH + lane * 16; b < kKeys * S::PITCH; b += 512)
-                        *reinterpret_cast<uint4*>(vt + h * (kKeys * 128) + b) = make_uint4(0, 0, 0, 0);
-                fence_proxy_async_smem();
-                __syncwarp();
-            }
-            if (!warp_wait(p_full(j & 1), (j >> 1) & 1, abort_flag, spin)) { gone = true; break; }
-            tc_fence_after();
-            if (lane == 0) {
+                return true;
+            };
+            auto outputs = [&](int k) {   // O += P V
+                const int j = nth(tile, k), s = j % NS;
+                if (!bar_wait(v_full(s), (j / NS) & 1, abort_flag, spin)) return false;
+                if (filled < kKeys && j == n - 1) {
+                    if (clears) bar_arrive(tail_bar);
+                    if (!bar_wait(zero_bar, 0, abort_flag, spin)) return false;
+                }
+                if (!bar_wait(p_full(tile, k & 1), (k >> 1) & 1, abort_flag, spin)) return false;
+                tc_fence_after();
+                const uint64_t vd = v_desc + s * (S::TILE >> 4);
+                const uint32_t d = cols + kOutCol, pa = cols + (k & 1) * kKeys;
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                    mma_ts(tmem + kOutCol, tmem + (j & 1) * kKeys + k * 8, operand<S::PITCH>(sv + s * S::TILE + k * 16 * S::PITCH, kKeys * 128),
-                           idesc_o, j > 0 || k > 0);
+                for (int i = 0; i < kKeys / 16; ++i) mma_ts(d, pa + i * 8, vd + ((i * 16 * S::PITCH) >> 4), idesc_o, i > 0 ? 1u : (uint32_t)(k > 0));
+                tc_commit(o_done(tile));
                 tc_commit(v_empty(s));
-                tc_commit(o_done);
-            }
-            __syncwarp();
-        }
-        if (lane == 0) {   // all MMAs: the output is whole, and nothing reads shared memory any more
+                return true;
+            };
+            // Two pages' scores ahead: S(k + 2) follows O(k), whose weights were in the same score buffer (MMAs of
+            // a thread run in order).
+            gone = (nt > 0 && !scores(0)) || (nt > 1 && !scores(1));
+            for (int k = 0; k < nt && !gone; ++k) gone = !outputs(k) || (k + 2 < nt && !scores(k + 2));
+            // all MMAs: the output is whole, and nothing reads shared memory any more
             tc_commit(end_bar);
             const long long t0 = clock64();
             while (!bar_try(end_bar, 0) && clock64() - t0 < kSpinCycles) {}
+        } else if (clears) {
+            // The other lanes: what stands beyond the filled positions of the last page may be NaN; as values (times
+            // the weight 0) it counts 0.
+            if (bar_wait(tail_bar, 0, abort_flag, spin)) {
+                uint8_t* vt = rings + NS * S::TILE + last * S::TILE;
+                const int words = (kKeys - filled) * (S::PITCH / 16);
+                const int rank = (lane - (int)leader - 1) & 31;   // 0 .. 30
+                for (int h = 0; h < S::HALVES; ++h)
+                    for (int i = rank; i < words; i += 31)
+                        *reinterpret_cast<uint4*>(vt + h * (kKeys * 128) + filled * S::PITCH + i * 16) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+                bar_arrive(zero_bar);
+            }
         }
         __syncwarp();
-    } else if (warp < soft_warps) {
+    } else if (warp < kSoftWarps && (warp & 3) < (tile_rows(tile) + 31) / 32 && tile_pages(tile) > 0) {
         // ---- softmax: one row per thread ----
-        const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-        const int limit = live ? tok.limit : INT32_MAX;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + tile * kTileCols;
+        const int limit = live ? tok.limit : INT32_MAX, nt = tile_pages(tile);
+        float m = -INFINITY, l = 0.0f;
         int free_to = limit;
         for (int y = 16; y; y >>= 1) free_to = min(free_to, __shfl_xor_sync(~0u, free_to, y));
-        for (int j = 0; j < n; ++j) {
-            const int b = j & 1, pos = it.pos0 + j * kKeys;
-            if ((stall && j == 0 && !warp_wait(stall_bar, 0, abort_flag, spin)) || !warp_wait(s_full(b), (j >> 1) & 1, abort_flag, spin)) {
+        for (int k = 0; k < nt; ++k) {
+            const int b = k & 1, pos = it.pos0 + nth(tile, k) * kKeys;
+            if ((stall && k == 0 && !warp_wait(stall_bar, 0, abort_flag, spin)) || !warp_wait(s_full(tile, b), (k >> 1) & 1, abort_flag, spin)) {
                 gone = true;
                 break;
             }
@@ -317,8 +358,8 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
                 const float f = grew ? (m == -INFINITY ? 0.0f : ex2(m - top)) : 1.0f;
                 if (grew) m = top;
                 l *= f;
-                if (j > 0) {   // (the scores of j came after the output of page j - 2)
-                    if (!warp_wait(o_done, (j - 1) & 1, abort_flag, spin)) { gone = true; break; }
+                if (k > 0) {   // (the scores of k came after the output of page k - 2)
+                    if (!warp_wait(o_done(tile), (k - 1) & 1, abort_flag, spin)) { gone = true; break; }
                     tc_fence_after();
 #pragma unroll
                     for (int c = 0; c < D; c += 32) {
@@ -346,48 +387,78 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) bar_arrive(p_full(b));
+            if (lane == 0) bar_arrive(p_full(tile, b));
             __syncwarp();
         }
         // (not o_done: two of its phases may be outstanding here, which a wait by parity does not tell apart)
         if (!gone && !warp_wait(end_bar, 0, abort_flag, spin)) gone = true;
         tc_fence_after();
-        gone = __any_sync(~0u, gone);
-        const bool counts = live && tok.limit > it.pos0, whole = tok.n_parts == 1;
-        const size_t part = ((size_t)(tok.part0 + it.split) * group + g) * pv.n_kv + kvh;
-        const float inv = gone ? NAN : l > 0.0f ? 1.0f / l : 0.0f;
+        // The output goes through shared memory (the rings' place), row by row, so that neighbouring lanes write
+        // neighbouring words of a row; rows are four words apart in the banks.
+        constexpr int ROW = D + 4;
+        float* stage = reinterpret_cast<float*>(rings) + (size_t)(tile * kTileM + r) * ROW;
+        const bool two = alternate && n > 1;   // this row's other half is in the other tile
+        const bool writes = !two || tile == 0;
+        float f0 = 1.0f, f1 = 0.0f;
+        if (two) {
+            if (tile == 1) {
+                tile1_ml[r] = make_float2(m, gone ? NAN : l);
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            if (!gone) {
-                tmem_ld32(lanes + kOutCol + c, o);
-                tmem_wait_ld(o);
-            } else {
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(lanes + kOutCol + c, o);
+                    tmem_wait_ld(o);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = 0x7FC00000u;
-            }
-            if (!counts) continue;
-            if (whole) {
-                uint4* dst = reinterpret_cast<uint4*>(x.out + tok.row * x.out_stride + head * D + c);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        w[e] = pack2(T(), __uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-                    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(stage + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 }
-            } else {
-                uint4* dst = reinterpret_cast<uint4*>(pv.part_o + part * D + c);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+            asm volatile("bar.sync 1, %0;" ::"r"(64 * ((it.rows + 31) / 32)) : "memory");
+            if (tile == 0) {
+                const float2 o = tile1_ml[r];
+                const float M = fmaxf(m, o.x);
+                f0 = m == -INFINITY ? 0.0f : ex2(m - M);
+                f1 = o.x == -INFINITY ? 0.0f : ex2(o.x - M);
+                m = M;
+                l = fmaf(l, f0, o.y * f1);
+                gone |= !(o.y == o.y);
             }
         }
-        if (counts) {
-            if (gone) l = NAN;
-            if (!whole) pv.part_ml[part] = make_float2(gone ? 0.0f : m, l);
-            else if (x.lse)
-                x.lse[(size_t)tok.row * (pv.n_kv * group) + head] = gone ? NAN : l > 0.0f ? (m - kWeightExp + log2f(l)) * kLn2 : -INFINITY;
+        if (writes) {
+            const bool counts = live && tok.limit > it.pos0, whole = tok.n_parts == 1;
+            const size_t part = ((size_t)(tok.part0 + it.split) * group + g) * pv.n_kv + kvh;
+            const float inv = gone ? NAN : !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(lanes + kOutCol + c, o);
+                tmem_wait_ld(o);
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    float4 y = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+                    if (two) {
+                        const float4 z = *reinterpret_cast<const float4*>(stage + kTileM * ROW + c + i);
+                        y = make_float4(fmaf(y.x, f0, z.x * f1), fmaf(y.y, f0, z.y * f1), fmaf(y.z, f0, z.z * f1), fmaf(y.w, f0, z.w * f1));
+                    }
+                    *reinterpret_cast<float4*>(stage + c + i) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+                }
+            }
+            __syncwarp();
+            constexpr int W = D / 4, R = 32 / W;   // lanes of a row, rows of the warp at a time
+            const char* to = reinterpret_cast<const char*>(whole ? (const void*)(x.out + tok.row * x.out_stride + head * D) : (const void*)(pv.part_o + part * D));
+            const int kind = !counts ? 0 : whole ? 1 : 2;
+#pragma unroll 4
+            for (int i = 0; i < 32; i += R) {
+                const int from = i + lane / W, c = lane % W;
+                const int what = __shfl_sync(~0u, kind, from);
+                char* dst = reinterpret_cast<char*>(__shfl_sync(~0u, (unsigned long long)to, from));
+                const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(rings) + (size_t)(tile * kTileM + (warp & 3) * 32 + from) * ROW + 4 * c);
+                if (what == 1) reinterpret_cast<uint2*>(dst)[c] = make_uint2(pack2(T(), y.x, y.y), pack2(T(), y.z, y.w));
+                else if (what == 2) reinterpret_cast<float4*>(dst)[c] = y;
+            }
+            if (counts) {
+                if (!whole) pv.part_ml[part] = gone ? make_float2(0.0f, NAN) : make_float2(m, l);
+                else if (x.lse) x.lse[(size_t)tok.row * (pv.n_kv * group) + head] = gone ? NAN : (m - kWeightExp + log2f(l)) * kLn2;
+            }
         }
     }
     tc_fence_before();
