@@ -597,7 +597,8 @@ static int64_t best_chunk(const t2sx_plan* a, bool tc, int64_t slots) {
     int64_t best = std::max<int64_t>(longest, 1);
     double best_cost = 1e300;
     for (int64_t parts = 1; parts <= 512 && (parts == 1 || (longest + parts - 1) / parts >= least); parts += parts < 32 ? 1 : parts / 16) {
-        const int64_t chunk = (longest + parts - 1) / parts;
+        int64_t chunk = (longest + parts - 1) / parts;
+        if (tc) chunk += chunk & 1;   // it takes two pages at a time
         int64_t items = 0, pages = 0;
         for (const Node& nd : a->nodes) {
             if (nd.tc != tc) continue;
@@ -626,7 +627,9 @@ static int64_t build_items(t2sx_plan* a) {
     for (const Node& nd : a->nodes) {
         const int64_t chunk = nd.tc ? tc_chunk : warp_chunk;
         const int tile = nd.tc ? kTcRows : kTileRows;
-        const int32_t n_splits = (int32_t)((nd.n_pages + chunk - 1) / chunk), per = (nd.n_pages + n_splits - 1) / n_splits;
+        const int32_t n_splits = (int32_t)((nd.n_pages + chunk - 1) / chunk);
+        int32_t per = (nd.n_pages + n_splits - 1) / n_splits;
+        if (nd.tc) per += per & 1;
         const int32_t* rows_of = a->node_rows.data() + nd.tokens_at;
         // a token has parts for the splits that begin below its limit, the first ones
         for (int32_t j = 0; j < nd.n_tokens; ++j) {

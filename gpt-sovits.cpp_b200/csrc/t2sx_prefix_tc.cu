@@ -4,9 +4,9 @@
 // pages, and takes one page (64 keys) at a time.  An item of more than 128 rows fills both tiles, and each
 // page's K and V serve both; a smaller one is in both, with every second page, and the two results are joined
 // at the end.
-//   warps 0-7  the softmax, one row per thread: scores from TMEM, running maximum and sum, weights back to
-//              TMEM in 16 bits.  The accumulated output is rescaled only when the maximum grows by more than
-//              2^8 (the weights then stay below 2^15, in the range of f16);
+//   warps 0-7  the softmax, one row per thread: scores from TMEM, weights back to TMEM in 16 bits, their sum.
+//              The maximum that the weights refer to is looked for, and the output rescaled, only when a
+//              tile's weights add up to 2^15 (f16 ends at 2^16);
 //   warp 8     TMA: the K and V tiles of the pages, in two rings;
 //   warps 9-10 the MMAs, one thread for each tile: S = Q K^T (M 128, N 64) into one of two score buffers of a tile, then O += P V with P from
 //              TMEM (M 128, N head dim).  S is issued two pages ahead, so that the tensor cores work while
@@ -32,7 +32,9 @@ constexpr int kKeys = kPoolPage;      // keys of a tile
 constexpr int kTileM = kTcRows / 2;   // rows of a tile
 constexpr int kSoftWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kThreads = 352;   // one MMA warp per tile
 constexpr int kTileCols = 256, kTmemCols = 2 * kTileCols, kOutCol = 2 * kKeys;
-constexpr float kHeadroom = 8.0f;     // log2 of how far weights may pass those of the reference maximum
+// A tile's weights against the reference maximum add up to less than this, or the reference is moved: f16 ends at
+// 2^16, and 64 weights at the reference itself make 2^13.
+constexpr float kSumLimit = 32768.0f;
 
 template <int D>
 struct TcShape {
@@ -106,19 +108,6 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[N]) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
-    return *reinterpret_cast<float2*>(&r);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(r)
-        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
-    return *reinterpret_cast<float2*>(&r);
-}
-
 // True in one lane of the warp, the leader.  The compiler knows that only one thread passes, and needs no loop around
 // the instructions that take their operands from uniform registers.
 __device__ __forceinline__ bool elect_one(uint32_t& leader) {
@@ -126,9 +115,47 @@ __device__ __forceinline__ bool elect_one(uint32_t& leader) {
     asm volatile("{\n.reg .pred p;\nelect.sync %1|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r), "=r"(leader));
     return r != 0;
 }
-// bar_wait of a whole warp: one answer for all of its lanes
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit) {
-    return __all_sync(~0u, bar_wait(bar, parity, abort_flag, limit));
+// The steps of weights(), volatile so that they stay in its order.
+__device__ __forceinline__ void v_fma2(float2& d, float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm volatile("fma.rn.f32x2 %0, %1, %2, %3;"
+                 : "=l"(r)
+                 : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+    d = *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ void v_add2(float2& d, float2 a) {
+    uint64_t r;
+    asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<uint64_t*>(&d)), "l"(*reinterpret_cast<uint64_t*>(&a)));
+    d = *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ void v_ex2(float& x) { asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x)); }
+__device__ __forceinline__ void v_pack2(__half, uint32_t& d, float2 a) { asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(a.y), "f"(a.x)); }
+__device__ __forceinline__ void v_pack2(__nv_bfloat16, uint32_t& d, float2 a) {
+    asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(a.y), "f"(a.x));
+}
+
+// The softmax weights of a row's scores in 16 bits, two to a word, and their sum: 2^(scale s - m + kWeightExp).
+// The exponential unit takes a warp's instruction every 8 cycles, and a warp issues in order: the multiplications of
+// later scores and the additions and conversions of earlier ones stand between the exponentials, which then follow
+// one another without a pause (left to the compiler the 64 of them took 1000 cycles instead of 560).
+template <typename T>
+__device__ __forceinline__ float weights(const uint32_t (&sc)[kKeys], uint32_t (&p)[kKeys / 2], float scale, float m) {
+    constexpr int N = kKeys / 2, AHEAD = 4, LAG = 3;
+    const float base = m == -INFINITY ? 0.0f : kWeightExp - m;
+    const float2 scale2 = make_float2(scale, scale), base2 = make_float2(base, base);
+    float2 y[N], sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+    auto multiply = [&](int c) { v_fma2(y[c], make_float2(__uint_as_float(sc[2 * c]), __uint_as_float(sc[2 * c + 1])), scale2, base2); };
+#pragma unroll
+    for (int c = 0; c < AHEAD; ++c) multiply(c);
+#pragma unroll
+    for (int c = 0; c < N + LAG; ++c) {
+        if (c < N) v_ex2(y[c].x);
+        if (c + AHEAD < N) multiply(c + AHEAD);
+        if (c >= LAG) v_add2(sum[c & 1], y[c - LAG]);
+        if (c < N) v_ex2(y[c].y);
+        if (c >= LAG) v_pack2(T(), p[c - LAG], y[c - LAG]);
+    }
+    return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
 }
 
 template <typename T, int D>
@@ -330,12 +357,12 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         float m = -INFINITY, l = 0.0f;
         int free_to = limit;
         for (int y = 16; y; y >>= 1) free_to = min(free_to, __shfl_xor_sync(~0u, free_to, y));
+        // In this loop a wait that is given up changes nothing in what the warp does: it goes on with whatever it finds,
+        // and its results are replaced at the end.
+        if (stall) gone = !bar_wait(stall_bar, 0, abort_flag, spin);
         for (int k = 0; k < nt; ++k) {
             const int b = k & 1, pos = it.pos0 + nth(tile, k) * kKeys;
-            if ((stall && k == 0 && !warp_wait(stall_bar, 0, abort_flag, spin)) || !warp_wait(s_full(tile, b), (k >> 1) & 1, abort_flag, spin)) {
-                gone = true;
-                break;
-            }
+            gone |= !bar_wait(s_full(tile, b), (k >> 1) & 1, abort_flag, spin);
             tc_fence_after();
             uint32_t sc[kKeys];
             tmem_ld32(lanes + b * kKeys, sc);
@@ -347,19 +374,22 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
                 for (int c = 0; c < kKeys; ++c)
                     if (c >= seen) sc[c] = 0xFF800000u;
             }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < kKeys; c += 8)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(sc[c + 2 * e]), __uint_as_float(sc[c + 2 * e + 1])));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-            const bool grew = top > m + kHeadroom;   // also when there was none before
+            // Weights against the reference maximum so far; they are right unless one passes 2^15, and then the sum does.
+            uint32_t p[kKeys / 2];
+            float sum = weights<T>(sc, p, scale, m);
+            const bool grew = !(sum < kSumLimit) || m == -INFINITY;
             if (__any_sync(~0u, grew)) {
-                const float f = grew ? (m == -INFINITY ? 0.0f : ex2(m - top)) : 1.0f;
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < kKeys; c += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(sc[c + 2 * e]), __uint_as_float(sc[c + 2 * e + 1])));
+                const float top = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale);
+                const float f = !grew ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
                 if (grew) m = top;
                 l *= f;
                 if (k > 0) {   // (the scores of k came after the output of page k - 2)
-                    if (!warp_wait(o_done(tile), (k - 1) & 1, abort_flag, spin)) { gone = true; break; }
+                    gone |= !bar_wait(o_done(tile), (k - 1) & 1, abort_flag, spin);
                     tc_fence_after();
 #pragma unroll
                     for (int c = 0; c < D; c += 32) {
@@ -371,18 +401,9 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
                         tmem_st32(lanes + kOutCol + c, o);
                     }
                 }
+                sum = weights<T>(sc, p, scale, m);
             }
-            const float base = m == -INFINITY ? 0.0f : kWeightExp - m;
-            float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-            uint32_t p[kKeys / 2];
-#pragma unroll
-            for (int c = 0; c < kKeys / 2; ++c) {
-                const float2 y = fma2(make_float2(__uint_as_float(sc[2 * c]), __uint_as_float(sc[2 * c + 1])), make_float2(scale, scale), make_float2(base, base));
-                const float2 e = make_float2(ex2(y.x), ex2(y.y));
-                sum[c & 1] = add2(sum[c & 1], e);
-                p[c] = pack2(T(), e.x, e.y);
-            }
-            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            l += sum;
             tmem_st32(lanes + b * kKeys, p);
             tmem_wait_st();
             tc_fence_before();
@@ -391,7 +412,8 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
             __syncwarp();
         }
         // (not o_done: two of its phases may be outstanding here, which a wait by parity does not tell apart)
-        if (!gone && !warp_wait(end_bar, 0, abort_flag, spin)) gone = true;
+        gone |= !bar_wait(end_bar, 0, abort_flag, spin);
+        gone = __any_sync(~0u, gone);
         tc_fence_after();
         // The output goes through shared memory (the rings' place), row by row, so that neighbouring lanes write
         // neighbouring words of a row; rows are four words apart in the banks.
