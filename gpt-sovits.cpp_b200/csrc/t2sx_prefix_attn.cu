@@ -27,6 +27,8 @@ namespace {
 #define C128 32,3,4
 #endif
 constexpr int kTileRows = 16;        // rows of a warp's tile (the m of mma.m16n8k16)
+constexpr int kWarpsPerPlace = 3;    // warps of a launch for each one that the device holds at a time, where items are many
+constexpr int kLongItem = 256;       // keys
 constexpr int kMinChunk = 2;         // pages of a split at least
 constexpr int kSplitCost = 4, kJoinCost = 4;   // in pages: what a split costs beside its pages, and joining parts
 constexpr int kTcMinRows = 64;       // rows of a node from which the tcgen05 kernel takes it
@@ -85,7 +87,7 @@ struct TileShape {
     static constexpr int KEYS = C::KEYS, STAGES = C::STAGES, RESIDENT = C::RESIDENT, TEAM = D == 128 ? 4 : 8;
     static constexpr int HALF = KEYS * D * 2;   // bytes of a stage's K (or V)
     static constexpr int RING = STAGES * 2 * HALF;
-    static_assert(RING >= 16 * D * 4, "a warp's results take the place of its ring");
+    static_assert(RING >= kTileRows * D * 4, "a warp's results take the place of its ring");
 };
 
 // 16-byte chunk `c` of key `row` in a tile: chunks are exchanged within 128 bytes so that the eight rows
@@ -96,34 +98,57 @@ __device__ __forceinline__ uint32_t tile_at(int row, int c) {
     else return row * (D * 2) + ((c & ~7) | ((c ^ row) & 7)) * 16;
 }
 
-// One CTA per (item, K/V head): at most 16 rows.  Its W warps share out the item's tiles, each with a ring of
-// its own, and join their results in shared memory.
+// At most 16 rows per item.  W = 1: a warp takes `heads_per` K/V heads of an item one after the other, its ring
+// running on from one to the next, so that a short item's start is paid once.  W > 1: a
+// CTA per (item, K/V head), whose warps share out the item's tiles, each with a ring of its own, and join their
+// results in shared memory.
 template <typename T, int D, int W>
 __global__ void __launch_bounds__(32 * W, W == 1 ? TileShape<D>::RESIDENT : 1)
-k_attend_tiles(PlanView pv, Tensors<T> x, int item0) {
+k_attend_tiles(PlanView pv, Tensors<T> x, int item0, int heads_per) {
     using S = TileShape<D>;
     constexpr int NT = S::KEYS / 8, DT = D / 8, KS = D / 16;   // key tiles, dim tiles, steps along the dims
     extern __shared__ __align__(1024) unsigned char ring[];
     const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5;
-    const int kvh = blockIdx.x % pv.n_kv;   // neighbours read one page
+    const int ways = (pv.n_kv + heads_per - 1) / heads_per;
+    const int kv0 = (int)(blockIdx.x % ways) * heads_per, kv1 = min(pv.n_kv, kv0 + heads_per);   // neighbours read one page
     const uint32_t ring0 = (uint32_t)__cvta_generic_to_shared(ring) + warp * S::RING;
-    const Item it = pv.items[item0 + blockIdx.x / pv.n_kv];
+    const Item it = pv.items[item0 + blockIdx.x / ways];
     const int group = pv.group;
     dependents_launch();   // the next launch fills what this one leaves free
 
-    const int all = it.n_pages * (kPoolPage / S::KEYS), first = all * warp / W, tiles = all * (warp + 1) / W;
-    int page_base = first / (kPoolPage / S::KEYS);    // pages [page_base, page_base + 32) are in the lanes
-    int page_id = page_base + lane < it.n_pages ? pv.pages[it.pages_at + page_base + lane] : 0;
-    auto request = [&](int t) {
-        if (t < tiles) {
+    // rows lane / 4 and lane / 4 + 8
+    int row_of[2], g_of[2], limit[2], n_parts[2], part[2];
+    long long q_at[2];
+    bool live[2], ends[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = lane / 4 + 8 * i, mr = it.row0 + r, g = mr % group;
+        live[i] = r < it.rows;
+        const Token t = pv.tokens[it.tokens_at + (live[i] ? mr / group : 0)];
+        row_of[i] = t.row;
+        g_of[i] = g;
+        q_at[i] = t.row * x.q_stride + g * D;
+        limit[i] = live[i] ? t.limit : 0;
+        n_parts[i] = t.n_parts;
+        ends[i] = t.ends_here;
+        part[i] = t.part0 + it.split;
+    }
+    const int all = (it.keys + S::KEYS - 1) / S::KEYS, first = all * warp / W, tiles = all * (warp + 1) / W;
+    int page_base = 0;                                // pages [page_base, page_base + 32) are in the lanes
+    int page_id = lane < it.n_pages ? pv.pages[it.pages_at + lane] : 0;
+    // tiles of one K/V head after those of another
+    int next_t = first, next_kv = first < tiles ? kv0 : kv1, stage_in = 0;
+    auto request = [&]() {
+        if (next_kv < kv1) {
+            const int t = next_t, kvh = next_kv;
             const int pg = t / (kPoolPage / S::KEYS), sub = t % (kPoolPage / S::KEYS);
-            if (pg - page_base >= 32) {
-                page_base += 32;
+            if (pg < page_base || pg >= page_base + 32) {
+                page_base = pg;
                 page_id = page_base + lane < it.n_pages ? pv.pages[it.pages_at + page_base + lane] : 0;
             }
             const int page = __shfl_sync(~0u, page_id, pg - page_base);
             const size_t at = (((size_t)page * pv.n_kv + kvh) * kPoolPage + sub * S::KEYS) * D;
-            const uint32_t dst = ring0 + ((t - first) % S::STAGES) * 2 * S::HALF;
+            const uint32_t dst = ring0 + stage_in * 2 * S::HALF;
             const char *ks = reinterpret_cast<const char*>(x.k + at), *vs = reinterpret_cast<const char*>(x.v + at);
             const int pos = it.pos0 + t * S::KEYS;
             const bool plain = pos + S::KEYS <= min(it.end, x.k_new ? it.new_pos : INT32_MAX);
@@ -144,37 +169,12 @@ k_attend_tiles(PlanView pv, Tensors<T> x, int item0) {
                     cp16(d + S::HALF, own ? reinterpret_cast<const char*>(x.v_new + off) : vs + c * 16, real);
                 }
             }
+            if (++next_t == tiles) { next_t = first; ++next_kv; }
+            stage_in = stage_in + 1 == S::STAGES ? 0 : stage_in + 1;
         }
         cp_commit();
     };
-
-    // rows lane / 4 and lane / 4 + 8
-    int row_of[2], head_of[2], limit[2], n_parts[2], part[2];
-    bool live[2], ends[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = lane / 4 + 8 * i, mr = it.row0 + r, g = mr % group;
-        live[i] = r < it.rows;
-        const Token t = pv.tokens[it.tokens_at + (live[i] ? mr / group : 0)];
-        row_of[i] = t.row;
-        head_of[i] = kvh * group + g;
-        limit[i] = live[i] ? t.limit : 0;
-        n_parts[i] = t.n_parts;
-        ends[i] = t.ends_here;
-        part[i] = t.part0 + it.split;
-    }
-    auto part_index = [&](int i, int part) { return ((size_t)part * group + head_of[i] - kvh * group) * pv.n_kv + kvh; };
-    for (int t = first; t < first + S::STAGES - 1; ++t) request(t);
-    uint32_t qf[KS][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(x.q + row_of[i] * x.q_stride + head_of[i] * D);
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            qf[k][i] = live[i] ? src[k * 8 + lane % 4] : 0;
-            qf[k][i + 2] = live[i] ? src[k * 8 + 4 + lane % 4] : 0;
-        }
-    }
+    for (int i = 0; i < S::STAGES - 1; ++i) request();
     // The item with a token's own position writes its key and value to the cache: read here, written after
     // the tiles for the first token (a decode step's only one).
     auto own = [&](int r) -> const Token* {
@@ -182,26 +182,65 @@ k_attend_tiles(PlanView pv, Tensors<T> x, int item0) {
         return x.k_new && r < it.rows && (it.row0 + r) % group == 0 && t->limit > it.pos0 &&
                t->limit <= it.pos0 + it.n_pages * kPoolPage && lane < D / 4 && warp == 0 ? t : nullptr;
     };
-    auto own_src = [&](const Token* t) {
+    auto own_src = [&](const Token* t, int kvh) {
         return reinterpret_cast<const uint4*>((lane >= D / 8 ? x.v_new : x.k_new) + t->row * x.kv_stride + kvh * D) + lane % (D / 8);
     };
-    auto own_dst = [&](const Token* t) {
+    auto own_dst = [&](const Token* t, int kvh) {
         return reinterpret_cast<uint4*>((lane >= D / 8 ? x.v : x.k) +
                                         (((size_t)t->page * pv.n_kv + kvh) * kPoolPage + (t->limit - 1) % kPoolPage) * D) + lane % (D / 8);
     };
     const Token* own0 = own(0);
-    uint4 own_word = make_uint4(0, 0, 0, 0);
-    if (own0) own_word = *own_src(own0);
     // the smallest limit of the rows: keys below it need no mask
     int free_to = min(live[0] ? limit[0] : INT32_MAX, live[1] ? limit[1] : INT32_MAX);
     for (int y = 16; y; y >>= 1) free_to = min(free_to, __shfl_xor_sync(~0u, free_to, y));
 
     const bool upper = it.rows > 8;
+    int stage = 0;
+    for (int kvh = kv0; kvh < kv1; ++kvh) {
+    int head_of[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) head_of[i] = kvh * group + g_of[i];
+    auto part_index = [&](int i, int part) { return ((size_t)part * group + g_of[i]) * pv.n_kv + kvh; };
+    uint4 own_word = make_uint4(0, 0, 0, 0);
+    if (own0) own_word = *own_src(own0, kvh);
+    uint32_t qf[KS][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(x.q + q_at[i] + (long long)kvh * group * D);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            qf[k][i] = live[i] ? src[k * 8 + lane % 4] : 0;
+            qf[k][i + 2] = live[i] ? src[k * 8 + 4 + lane % 4] : 0;
+        }
+    }
     float o[DT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    // The parts of the launch before: the first head's are folded in at its end (they may not be there yet), those
+    // of the others are what the head starts from.
+    const bool start_from = W == 1 && kvh > kv0;
+    int folded[2] = {0, 0};
+    if (start_from) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (!live[i] || !ends[i] || n_parts[i] < 2 || limit[i] <= it.pos0) continue;
+            const size_t at = part_index(i, part[i] - 1);
+            const float2 ml = __ldcg(&pv.part_ml[at]);
+            m[i] = ml.x;
+            l[i] = lane % 4 == 0 ? ml.y : 0.0f;
+            const float2* src = reinterpret_cast<const float2*>(pv.part_o + at * D);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const float2 y = __ldcg(&src[d * 4 + lane % 4]);
+                o[d][2 * i] = y.x;
+                o[d][2 * i + 1] = y.y;
+            }
+            folded[i] = 1;
+        }
+    }
     for (int t = first; t < tiles; ++t) {
         cp_wait<S::STAGES - 2>();
         __syncwarp();
-        const uint32_t kt = ring0 + ((t - first) % S::STAGES) * 2 * S::HALF, vt = kt + S::HALF;
+        const uint32_t kt = ring0 + stage * 2 * S::HALF, vt = kt + S::HALF;
+        stage = stage + 1 == S::STAGES ? 0 : stage + 1;
         const int pos = it.pos0 + t * S::KEYS;
         float s[NT][4] = {};
 #pragma unroll
@@ -270,12 +309,11 @@ k_attend_tiles(PlanView pv, Tensors<T> x, int item0) {
             }
         }
         __syncwarp();
-        request(t + S::STAGES - 1);
+        request();
     }
-    cp_wait<0>();
-    if (own0) *own_dst(own0) = own_word;
+    if (own0) *own_dst(own0, kvh) = own_word;
     for (int r = 1; r < it.rows; ++r)
-        if (const Token* t = own(r)) *own_dst(t) = *own_src(t);
+        if (const Token* t = own(r)) *own_dst(t, kvh) = *own_src(t, kvh);
     float sum[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -286,6 +324,7 @@ k_attend_tiles(PlanView pv, Tensors<T> x, int item0) {
     if constexpr (W > 1) {
         // the warps' results in the place of their rings; then each warp joins the dim tiles warp, warp + W, ...
         __shared__ float2 ml[W][16];
+        cp_wait<0>();
         __syncthreads();
         float2* all_o = reinterpret_cast<float2*>(ring);
 #pragma unroll
@@ -332,7 +371,7 @@ k_attend_tiles(PlanView pv, Tensors<T> x, int item0) {
             continue;
         }
         if constexpr (W == 1) {
-            for (int j = n_parts[i] - 1; j-- > 0;) {   // the other parts, if any
+            for (int j = n_parts[i] - 1 - folded[i]; j-- > 0;) {   // the other parts, if any
                 const size_t at = part_index(i, part[i] - n_parts[i] + 1 + j);
                 const float2 ml = __ldcg(&pv.part_ml[at]);
                 const float2* src = reinterpret_cast<const float2*>(pv.part_o + at * D);
@@ -357,6 +396,51 @@ k_attend_tiles(PlanView pv, Tensors<T> x, int item0) {
         if (x.lse && lane % 4 == 0 && warp == 0)
             x.lse[(size_t)row_of[i] * (pv.n_kv * group) + head_of[i]] = (m[i] - kWeightExp + log2f(sum[i])) * kLn2;
     }
+    }
+}
+
+// Four warps, each with a (token, query head) of few parts: the lanes are D / 4 columns of four dims x 32 / (D / 4) parts.
+template <typename T, int D>
+__global__ void __launch_bounds__(128)
+k_join_few(PlanView pv, Tensors<T> x) {
+    constexpr int COLS = D / 4, LANES = 32 / COLS;
+    const int lane = threadIdx.x & 31, heads = pv.n_kv * pv.group;
+    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    dependents_wait();
+    if (at >= (long long)pv.n_joins * heads) return;
+    const int head = (int)(at % heads), kvh = head / pv.group, g = head % pv.group;
+    const Token t = pv.joins[at / heads];
+    auto part = [&](int i) { return ((size_t)(t.part_at + i) * pv.group + g) * pv.n_kv + kvh; };
+    const float2 mine = lane < t.n_parts ? __ldcg(&pv.part_ml[part(lane)]) : make_float2(-INFINITY, 0.0f);
+    float M = mine.x;
+    for (int y = 16; y; y >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, y));
+    const float weight = mine.x == -INFINITY ? 0.0f : ex2(mine.x - M);
+    float l = weight * mine.y;
+    for (int y = 16; y; y >>= 1) l += __shfl_xor_sync(~0u, l, y);
+    float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int i0 = 0; i0 < t.n_parts; i0 += LANES) {
+        const int i = i0 + lane / COLS;
+        const float f = __shfl_sync(~0u, weight, i & 31);
+        if (i >= t.n_parts) continue;
+        const float4 o = __ldcg(reinterpret_cast<const float4*>(pv.part_o + part(i) * D) + lane % COLS);
+        acc.x = fmaf(f, o.x, acc.x);
+        acc.y = fmaf(f, o.y, acc.y);
+        acc.z = fmaf(f, o.z, acc.z);
+        acc.w = fmaf(f, o.w, acc.w);
+    }
+#pragma unroll
+    for (int y = COLS; y < 32; y <<= 1) {
+        acc.x += __shfl_xor_sync(~0u, acc.x, y);
+        acc.y += __shfl_xor_sync(~0u, acc.y, y);
+        acc.z += __shfl_xor_sync(~0u, acc.z, y);
+        acc.w += __shfl_xor_sync(~0u, acc.w, y);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (lane < COLS)
+        reinterpret_cast<uint2*>(x.out + t.row * x.out_stride + head * D)[lane] =
+            make_uint2(pack2(T(), acc.x * inv, acc.y * inv), pack2(T(), acc.z * inv, acc.w * inv));
+    if (x.lse && lane == 0) x.lse[(size_t)t.row * heads + head] = (M - kWeightExp + log2f(l)) * kLn2;
 }
 
 // One CTA of four warps per (token of several parts, query head), for tokens of many parts: each warp joins every
@@ -438,6 +522,8 @@ struct t2sx_plan {
     t2sx_pool* pool = nullptr;
     int n_heads = 0, n_sm = 148;
     bool ready = false, shared_rows = false, small = false, tc_writes = false;
+    int32_t most_parts = 0;            // of a token in `joins`
+    int64_t launch_keys[2] = {0, 0};   // of the items of the launches of k_attend_tiles
     CUtensorMap map_k, map_v;
     int32_t *err = nullptr, *err_dev = nullptr;   // pinned: what a kernel that gave up a wait reports
     uint64_t version = 0;          // of the pool at the update
@@ -649,7 +735,8 @@ static int64_t build_items(t2sx_plan* a) {
                 const int32_t pages = std::min(std::min(per, nd.n_pages - pg), pages_of(sees) - start / kPoolPage);
                 if (pages <= 0) continue;
                 a->items.push_back({nd.tokens_at, (int32_t)r, n, nd.pages_at + pg, pages, start, split, nd.end, nd.new_pos, nd.new_row,
-                                    nd.tc ? 0 : nd.new_pos == INT32_MAX ? 1 : 2, 0});
+                                    nd.tc ? 0 : nd.new_pos == INT32_MAX ? 1 : 2,
+                                    std::min(pages * kPoolPage, std::min(sees, nd.end) - start)});
             }
         }
     }
@@ -658,16 +745,22 @@ static int64_t build_items(t2sx_plan* a) {
         return x.launch != y.launch ? x.launch < y.launch : x.n_pages > y.n_pages;
     });
     int32_t n_launch[3] = {0, 0, 0};
+    a->launch_keys[0] = a->launch_keys[1] = 0;
     a->tc_writes = false;
     for (const Item& it : a->items) {
         ++n_launch[it.launch];
+        if (it.launch > 0) a->launch_keys[it.launch - 1] += it.keys;
         a->tc_writes |= it.launch == 0 && it.new_pos != INT32_MAX;
     }
     int64_t parts = 0;
+    a->most_parts = 0;
     for (Token& t : a->info) {
         t.part_at = (int32_t)std::min<int64_t>(parts, INT32_MAX);
         if (t.n_parts > 1) parts += t.n_parts;
-        if (t.n_parts > 1 && !t.ends_here) a->joins.push_back(t);
+        if (t.n_parts > 1 && !t.ends_here) {
+            a->joins.push_back(t);
+            a->most_parts = std::max(a->most_parts, t.n_parts);
+        }
     }
     for (size_t i = 0; i < a->tokens.size(); ++i) {
         const int32_t ordinal = a->tokens[i].part0;
@@ -792,9 +885,14 @@ static cudaError_t launch_attend(t2sx_plan* a, Tensors<T> x, int layer, cudaStre
         cudaFuncSetAttribute(k_attend_tiles<T, D, S::TEAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TEAM * S::RING);
     });
     if (a->small)
-        return launch(k_attend_tiles<T, D, S::TEAM>, dim3((unsigned)w.n_own * w.n_kv), 32 * S::TEAM, S::TEAM * S::RING, st, false, w, x, 0);
+        return launch(k_attend_tiles<T, D, S::TEAM>, dim3((unsigned)w.n_own * w.n_kv), 32 * S::TEAM, S::TEAM * S::RING, st, false, w, x, 0, 1);
     auto tiles = [&](int item0, int n, bool early) {
-        return n ? launch(k_attend_tiles<T, D, 1>, dim3((unsigned)n * w.n_kv), 32, S::RING, st, early, w, x, item0) : cudaSuccess;
+        // Short items (below kLongItem keys, on average) share a warp, as many heads as leave several warps for each place:
+        // a long one hides its own start.
+        const int64_t places = (int64_t)a->n_sm * S::RESIDENT, keys = n ? a->launch_keys[item0 == w.n_tc && w.n_shared ? 0 : 1] / n : 0;
+        const int64_t heads = std::min<int64_t>({(int64_t)w.n_kv, (int64_t)n * w.n_kv / (places * kWarpsPerPlace) + 1, kLongItem / (keys + 1) + 1});
+        return n ? launch(k_attend_tiles<T, D, 1>, dim3((unsigned)n * ((w.n_kv + heads - 1) / heads)), 32, S::RING, st, early, w, x, item0, (int)heads)
+                 : cudaSuccess;
     };
     cudaError_t e = cudaSuccess;
     bool early = false;   // a launch of this call comes before
@@ -814,8 +912,11 @@ static cudaError_t launch_attend(t2sx_plan* a, Tensors<T> x, int layer, cudaStre
     if (e == cudaSuccess) e = tiles(w.n_tc, w.n_shared, early);
     early |= w.n_shared > 0;
     if (e == cudaSuccess) e = tiles(w.n_tc + w.n_shared, w.n_own, early);
-    if (e == cudaSuccess && w.n_joins)
-        e = launch(k_join_parts<T, D>, dim3((unsigned)(w.n_joins * a->n_heads)), 128, 0, st, true, w, x);
+    if (e == cudaSuccess && w.n_joins) {
+        const int64_t rows = (int64_t)w.n_joins * a->n_heads;
+        e = a->most_parts <= 32 ? launch(k_join_few<T, D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, true, w, x)
+                                : launch(k_join_parts<T, D>, dim3((unsigned)rows), 128, 0, st, true, w, x);
+    }
     return e;
 }
 

@@ -26,7 +26,7 @@ struct Item {
     int32_t new_pos;     // from this position on the keys are the step's own (of one sequence) ...
     int32_t new_row;     // ... and that one is this row of the step
     int32_t launch;      // 0: tcgen05, 1: pages of several sequences, 2: the others
-    int32_t pad;
+    int32_t keys;        // of its pages that a row sees
 };
 
 // A token as one of a node's: what it is, and where its parts are.  A token's parts are numbers

@@ -222,14 +222,20 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         const uint32_t flip = x.scale2 < 0.0f ? 0x80008000u : 0u, keep = x.scale2 != 0.0f ? 0xFFFFFFFFu : 0u;
         const int c = lane % W;
         const T* mine = x.q + tok.row * x.q_stride + head * D;
-#pragma unroll 8
-        for (int i = 0; i < 32; i += R) {
-            const int from = i + lane / W, rr = (warp & 3) * 32 + from;
+        uint4 w[32 / R];   // all loads before the stores, which they are not known to differ from
+#pragma unroll
+        for (int i = 0; i < 32 / R; ++i) {
+            const int from = i * R + lane / W, rr = (warp & 3) * 32 + from;
             const uint4* src = reinterpret_cast<const uint4*>(__shfl_sync(~0u, (unsigned long long)mine, from));
-            uint4 w = rr < tile_rows(tile) ? src[c] : make_uint4(0, 0, 0, 0);
-            w.x = (w.x ^ flip) & keep; w.y = (w.y ^ flip) & keep; w.z = (w.z ^ flip) & keep; w.w = (w.w ^ flip) & keep;
+            w[i] = rr < tile_rows(tile) ? src[c] : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 32 / R; ++i) {
+            const int rr = (warp & 3) * 32 + i * R + lane / W;
+            uint4 u = w[i];
+            u.x = (u.x ^ flip) & keep; u.y = (u.y ^ flip) & keep; u.z = (u.z ^ flip) & keep; u.w = (u.w ^ flip) & keep;
             const int at = D == 32 ? rr * 64 + ((c ^ (rr >> 1)) & 3) * 16 : (c >> 3) * (kTileM * 128) + rr * 128 + ((c ^ rr) & 7) * 16;
-            *reinterpret_cast<uint4*>(smem + tile * S::Q + at) = w;
+            *reinterpret_cast<uint4*>(smem + tile * S::Q + at) = u;
         }
         fence_proxy_async_smem();
     }
