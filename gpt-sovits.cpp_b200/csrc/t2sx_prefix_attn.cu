@@ -31,8 +31,9 @@ constexpr int kWarpsPerPlace = 3;    // warps of a launch for each one that the 
 constexpr int kLongItem = 256;       // keys
 constexpr int kMinChunk = 2;         // pages of a split at least
 constexpr int kSplitCost = 4, kJoinCost = 4;   // in pages: what a split costs beside its pages, and joining parts
-constexpr int kTcMinRows = 64;       // rows of a node from which the tcgen05 kernel takes it
+constexpr int kTcMinRowDims = 2049;  // rows x head dim of a node from which the tcgen05 kernel takes it (see build_items)
 constexpr int kTcMinChunk = 4;       // pages of a split of such a node at least
+constexpr int kFoldParts = 4;        // parts of a token up to which the item of its own pages folds them in, one after the other
 constexpr int kSmallPages = 32;      // pages of a sequence in a small step at most
 
 __device__ __forceinline__ void mma16816(__half, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -706,7 +707,11 @@ static int64_t best_chunk(const t2sx_plan* a, bool tc, int64_t slots) {
 static int64_t build_items(t2sx_plan* a) {
     const int group = a->n_heads / a->pool->n_kv, n_kv = a->pool->n_kv;
     a->items.clear(); a->joins.clear();
-    for (Node& nd : a->nodes) nd.tc = !a->small && (int64_t)nd.n_tokens * group >= kTcMinRows;
+    // The tcgen05 kernel reads a page once for up to 256 rows, a warp tile for 16, but a page of few rows costs the former
+    // as much as one of many: 20 and 32 rows of one 32768-position prompt with 8 K/V heads took 46 and 50 us with it and
+    // 55 and 56 without at head dim 128; at 64, 16 prompts of 4032 with 32 and 48 rows took 54 and 45 with, 47 and 60
+    // without; at 32, with 48 and 64 rows, 30 and 31 with, 25 and 31 without.
+    for (Node& nd : a->nodes) nd.tc = !a->small && (int64_t)nd.n_tokens * group * a->pool->dim >= kTcMinRowDims;
     const int64_t warp_chunk = a->small ? kSmallPages : best_chunk(a, false, (int64_t)a->n_sm * resident_warps(a->pool->dim));
     const int64_t tc_chunk = best_chunk(a, true, a->n_sm);
     a->tokens.resize(a->node_rows.size());
@@ -757,6 +762,7 @@ static int64_t build_items(t2sx_plan* a) {
     for (Token& t : a->info) {
         t.part_at = (int32_t)std::min<int64_t>(parts, INT32_MAX);
         if (t.n_parts > 1) parts += t.n_parts;
+        t.ends_here &= t.n_parts <= kFoldParts;
         if (t.n_parts > 1 && !t.ends_here) {
             a->joins.push_back(t);
             a->most_parts = std::max(a->most_parts, t.n_parts);

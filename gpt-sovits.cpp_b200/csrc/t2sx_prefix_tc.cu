@@ -38,13 +38,16 @@ constexpr float kSumLimit = 32768.0f;
 
 template <int D>
 struct TcShape {
-    static constexpr int STAGES = D == 128 ? 5 : 8;
+    // even: where the tiles take every second page, a stage is always the same tile's, whose thread then sees all phases
+    // of its barriers (a wait by parity does not tell a phase from the one before the last)
+    static constexpr int STAGES = D == 128 ? 4 : 8;
+    static_assert(STAGES % 2 == 0, "see above");
     static constexpr int PITCH = D == 32 ? 64 : 128;               // bytes of a row of a swizzled block
     static constexpr int HALVES = D == 128 ? 2 : 1;                // blocks of 64 dims
     static constexpr int TILE = kKeys * D * 2, Q = kTileM * D * 2;
     static constexpr int BARS = 4 * STAGES + 2 * (2 + 2 + 1) + 4;  // K, V full and empty; a tile's scores, weights, output; end, stall, tail, zero
     static constexpr int SMEM = 1024 + 2 * Q + 2 * STAGES * TILE + BARS * 8 + kTileM * 8 + 16;
-    static_assert(2 * STAGES * TILE >= 2 * kTileM * (D + 4) * 4, "the tiles' outputs take the place of the rings");
+    static_assert(2 * Q + 2 * STAGES * TILE >= 2 * kTileM * (D + 4) * 4, "the tiles' outputs take the place of Q and the rings");
 };
 
 // Shared-memory descriptor of an operand whose rows are PITCH bytes, swizzled within them; groups of eight rows
@@ -421,10 +424,10 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         gone |= !bar_wait(end_bar, 0, abort_flag, spin);
         gone = __any_sync(~0u, gone);
         tc_fence_after();
-        // The output goes through shared memory (the rings' place), row by row, so that neighbouring lanes write
+        // The output goes through shared memory (the place of Q and the rings), row by row, so that neighbouring lanes write
         // neighbouring words of a row; rows are four words apart in the banks.
         constexpr int ROW = D + 4;
-        float* stage = reinterpret_cast<float*>(rings) + (size_t)(tile * kTileM + r) * ROW;
+        float* stage = reinterpret_cast<float*>(smem) + (size_t)(tile * kTileM + r) * ROW;
         const bool two = alternate && n > 1;   // this row's other half is in the other tile
         const bool writes = !two || tile == 0;
         float f0 = 1.0f, f1 = 0.0f;
@@ -479,7 +482,7 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
                 const int from = i + lane / W, c = lane % W;
                 const int what = __shfl_sync(~0u, kind, from);
                 char* dst = reinterpret_cast<char*>(__shfl_sync(~0u, (unsigned long long)to, from));
-                const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(rings) + (size_t)(tile * kTileM + (warp & 3) * 32 + from) * ROW + 4 * c);
+                const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(smem) + (size_t)(tile * kTileM + (warp & 3) * 32 + from) * ROW + 4 * c);
                 if (what == 1) reinterpret_cast<uint2*>(dst)[c] = make_uint2(pack2(T(), y.x, y.y), pack2(T(), y.z, y.w));
                 else if (what == 2) reinterpret_cast<float4*>(dst)[c] = y;
             }
