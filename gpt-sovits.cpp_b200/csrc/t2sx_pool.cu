@@ -74,7 +74,7 @@ int launch_moves(t2sx_pool* p, const std::vector<PageMove>& moves, cudaStream_t 
             list, reinterpret_cast<uint4*>(p->k), reinterpret_cast<uint4*>(p->v), p->n_pages, p->n_kv, p->dim * 2 / 16);
         POOL_CK(cudaGetLastError());
     }
-    POOL_CK(p->end(st));
+    p->end(st);
     return T2SX_OK;
 }
 
@@ -133,10 +133,8 @@ int derive(t2sx_pool* p, int32_t n, const int32_t* srcs, const int32_t* dsts, cu
 void t2sx_pool_release_object(t2sx_pool* p) {
     DeviceGuard dg;
     dg.set(p->device);
-    if (p->done) {
-        cudaEventSynchronize(p->done);
-        cudaEventDestroy(p->done);
-    }
+    p->settle();
+    if (p->done) cudaEventDestroy(p->done);
     delete p;
 }
 

@@ -549,7 +549,7 @@ static void plan_release(t2sx_plan* a) {
     t2sx_pool* p = a->pool;
     DeviceGuard dg;
     dg.set(p->device);
-    cudaEventSynchronize(p->done);
+    p->settle();
     for (int i = 0; i < 2; ++i) {
         if (a->sent[i]) cudaEventDestroy(a->sent[i]);
         if (a->host[i]) cudaFreeHost(a->host[i]);
@@ -849,7 +849,7 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
         POOL_CK(p->begin(st));
         auto grow = [&](uint8_t*& mem, size_t& have, size_t want) -> cudaError_t {
             if (have >= want) return cudaSuccess;
-            cudaError_t e = cudaEventSynchronize(p->done);   // nothing of the plan runs any more
+            cudaError_t e = p->settle();   // nothing of the plan runs any more
             if (e == cudaSuccess && mem) e = cudaFree(mem);
             mem = nullptr;
             have = 0;
@@ -866,7 +866,7 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
         put(o_info, a->info); put(o_items, a->items); put(o_tokens, a->tokens); put(o_pages, a->pages); put(o_joins, a->joins);
         if (bytes) POOL_CK(cudaMemcpyAsync(a->dev, a->host[b], bytes, cudaMemcpyHostToDevice, st));
         POOL_CK(cudaEventRecord(a->sent[b], st));
-        POOL_CK(p->end(st));
+        p->end(st);
         PlanView& w = a->view;
         w.rows_of = (const Token*)(a->dev + o_info);
         w.items = (const Item*)(a->dev + o_items);
@@ -949,7 +949,7 @@ extern "C" int t2sx_plan_sync(t2sx_plan* a) {
     if (!a) return bad("t2sx_plan_sync: null plan");
     DeviceGuard dg;
     POOL_CK(dg.set(a->pool->device));
-    if (a->pool->worked) POOL_CK(cudaEventSynchronize(a->pool->done));
+    POOL_CK(a->pool->settle());
     return plan_error(a);
 }
 
@@ -979,6 +979,6 @@ extern "C" int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, 
     POOL_CK(p->begin(st));
     auto go = p->type == T2SX_TYPE_F16 ? attend<__half> : attend<__nv_bfloat16>;
     POOL_CK(go(a, layer, q_dev, q_stride, k_new_dev, v_new_dev, kv_stride, scale, out_dev, out_stride, lse_dev, st));
-    POOL_CK(p->end(st));
+    p->end(st);
     return T2SX_OK;
 }

@@ -465,6 +465,8 @@ class PagePool:
         self.h = h
         self.dtype, self.n_layers, self.n_pages = dtype, n_layers, n_pages
         self.n_kv_heads, self.head_dim, self.max_seqs = n_kv_heads, head_dim, max_seqs
+        self._width = C.c_int32(0)
+        self._width_ref = C.byref(self._width)
 
     def available(self) -> int:
         """Pages that no sequence uses."""
@@ -481,10 +483,10 @@ class PagePool:
     def table(self, seqs) -> np.ndarray:
         """Page ids of the sequences, int32 [n][most pages of one], filled up with -1."""
         ids, n, _keep = _ids(seqs)
-        width = C.c_int32(0)
-        _ck(lib().t2sx_pool_table(self.h, n, ids, 0, None, C.byref(width)))
+        fn, width = lib().t2sx_pool_table, self._width
+        _ck(fn(self.h, n, ids, 0, None, self._width_ref))
         out = np.empty((n, width.value), dtype=np.int32)
-        _ck(lib().t2sx_pool_table(self.h, n, ids, width.value, out.__array_interface__["data"][0], None))
+        _ck(fn(self.h, n, ids, width.value, out.__array_interface__["data"][0], None))
         return out
 
     def _pairs(self, fn, srcs, dsts, stream):
@@ -542,6 +544,8 @@ class AttnPlan:
         _ck(lib().t2sx_plan_create(pool.h, n_heads, C.byref(h)))
         self.h = h
         self.pool, self.n_heads, self.rows = pool, n_heads, 0
+        self._row, self._kv_row = n_heads * pool.head_dim, pool.n_kv_heads * pool.head_dim
+        self._attend = lib().t2sx_plan_attend
 
     def update(self, seqs, n_new, stream: int = 0):
         """The step's sequences and how many of their last positions are rows of the step."""
@@ -556,11 +560,12 @@ class AttnPlan:
                kv_stride: int | None = None, out_stride: int | None = None, stream: int = 0):
         """out[r] = softmax(scale * q[r] . K) . V over the positions that row r sees, after the rows' own
         k_new, v_new (if given) have been written to the cache.  Strides in elements; default: dense rows."""
-        dim = self.pool.head_dim
-        row = self.n_heads * dim
-        _ck(lib().t2sx_plan_attend(self.h, layer, q_ptr, row if q_stride is None else q_stride, k_new_ptr, v_new_ptr,
-                                   self.pool.n_kv_heads * dim if kv_stride is None else kv_stride, scale, out_ptr,
-                                   row if out_stride is None else out_stride, lse_ptr, stream))
+        row = self._row
+        rc = self._attend(self.h, layer, q_ptr, row if q_stride is None else q_stride, k_new_ptr, v_new_ptr,
+                          self._kv_row if kv_stride is None else kv_stride, scale, out_ptr,
+                          row if out_stride is None else out_stride, lse_ptr, stream)
+        if rc:
+            _ck(rc)
 
     def sync(self):
         """Waits for the pool's device work; raises T2SXError(ERR_TIMEOUT) if an attend() gave up a bounded
@@ -585,6 +590,7 @@ def token_logprobs(dtype: int, rows: int, vocab: int, logits_ptr: int, tokens_pt
                    device: int = 0, stream: int = 0):
     """Log probability, entropy and rank of tokens[r] under row r of the logits, and the top_k (<= 32) best
     tokens with theirs.  stride: elements between rows (default: dense)."""
-    _ck(lib().t2sx_token_logprobs(device, dtype, rows, vocab, logits_ptr, vocab if stride is None else stride,
-                                  tokens_ptr, top_k, logprob_ptr, entropy_ptr, rank_ptr, top_ids_ptr,
-                                  top_logprobs_ptr, stream))
+    rc = lib().t2sx_token_logprobs(device, dtype, rows, vocab, logits_ptr, vocab if stride is None else stride, tokens_ptr,
+                                   top_k, logprob_ptr, entropy_ptr, rank_ptr, top_ids_ptr, top_logprobs_ptr, stream)
+    if rc:
+        _ck(rc)

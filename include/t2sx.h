@@ -264,8 +264,9 @@ T2SX_API int t2sx_kvcache_attn_prefill(t2sx_kvcache* c, int32_t n, const int32_t
  * Pages are taken lowest free id first; every call either takes full effect or none.
  * head_dim: 32, 64 or 128.  n_pages at most 2^26.
  * Threading: single-owner, as a session.  Streams: calls take effect in call order, whatever
- * streams they are given; a call on another stream than the last one waits for the latter.  The
- * caller orders its own accesses to the storage and to tensors.  Not for stream capture. */
+ * streams they are given; a call on another stream than the last one waits for the latter, so a
+ * stream given to a call is not destroyed before the pool's next call or its end.  The caller
+ * orders its own accesses to the storage and to tensors.  Not for stream capture. */
 typedef struct t2sx_pool t2sx_pool;
 T2SX_API int t2sx_pool_create(int32_t device, int32_t type, int32_t n_layers, int32_t n_pages, int32_t n_kv_heads,
                               int32_t head_dim, int32_t max_seqs, void* k_dev, void* v_dev, t2sx_pool** out);
