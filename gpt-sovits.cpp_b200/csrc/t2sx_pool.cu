@@ -15,23 +15,26 @@ using namespace t2sx;
 namespace {
 
 // Moves per launch: the list travels as a kernel parameter (no staging buffer, nothing to order).
-constexpr int kMovesPerLaunch = 512;
+// Two sizes of it: the host's time of a launch grows with its parameters.
+constexpr int kFewMoves = 32, kMovesPerLaunch = 512;
 constexpr int kFan = 8;            // destinations that one read of a page serves
 constexpr int kHeadsPerCta = 8;    // one per warp
 struct Fan {                       // moves of one source and fill
     int32_t src;
     uint16_t first, n, fill, pad;
 };
+template <int N>
 struct MoveList {
-    int32_t dst[kMovesPerLaunch];
-    Fan fan[kMovesPerLaunch];
+    int32_t dst[N];
+    Fan fan[N];
 };
 
 // One CTA per (fan, layer, K or V, 8 heads); a head's filled positions are contiguous in its page.  Bound by
 // the bytes written: a fork's partial page is read once for up to eight copies (through L2 it cost 306 us
 // instead of 139 us for 512 copies of 32 pages of 24 layers).
+template <int N>
 __global__ void __launch_bounds__(32 * kHeadsPerCta)
-k_move_pages(const __grid_constant__ MoveList list, uint4* __restrict__ k, uint4* __restrict__ v, int n_pages, int n_kv,
+k_move_pages(const __grid_constant__ MoveList<N> list, uint4* __restrict__ k, uint4* __restrict__ v, int n_pages, int n_kv,
              int row_vec) {
     const Fan f = list.fan[blockIdx.x];
     const int lane = threadIdx.x & 31, h = (blockIdx.z >> 1) * kHeadsPerCta + (threadIdx.x >> 5);
@@ -55,6 +58,20 @@ k_move_pages(const __grid_constant__ MoveList list, uint4* __restrict__ k, uint4
     }
 }
 
+template <int N>
+void launch_list(t2sx_pool* p, const PageMove* moves, int n, cudaStream_t st) {
+    MoveList<N> list;
+    int fans = 0;
+    for (int i = 0; i < n; ++i) {
+        const PageMove& m = moves[i];
+        list.dst[i] = m.dst;
+        if (fans && list.fan[fans - 1].src == m.src && list.fan[fans - 1].n < kFan) ++list.fan[fans - 1].n;
+        else list.fan[fans++] = Fan{m.src, (uint16_t)i, 1, (uint16_t)m.fill, 0};
+    }
+    k_move_pages<N><<<dim3(fans, p->n_layers, 2 * ((p->n_kv + kHeadsPerCta - 1) / kHeadsPerCta)), 32 * kHeadsPerCta, 0, st>>>(
+        list, reinterpret_cast<uint4*>(p->k), reinterpret_cast<uint4*>(p->v), p->n_pages, p->n_kv, p->dim * 2 / 16);
+}
+
 int launch_moves(t2sx_pool* p, const std::vector<PageMove>& moves, cudaStream_t st) {
     if (moves.empty()) return T2SX_OK;
     DeviceGuard dg;
@@ -62,16 +79,8 @@ int launch_moves(t2sx_pool* p, const std::vector<PageMove>& moves, cudaStream_t 
     POOL_CK(p->begin(st));
     for (size_t at = 0; at < moves.size(); at += kMovesPerLaunch) {
         const int n = (int)std::min<size_t>(kMovesPerLaunch, moves.size() - at);
-        MoveList list;
-        int fans = 0;
-        for (int i = 0; i < n; ++i) {
-            const PageMove& m = moves[at + i];
-            list.dst[i] = m.dst;
-            if (fans && list.fan[fans - 1].src == m.src && list.fan[fans - 1].n < kFan) ++list.fan[fans - 1].n;
-            else list.fan[fans++] = Fan{m.src, (uint16_t)i, 1, (uint16_t)m.fill, 0};
-        }
-        k_move_pages<<<dim3(fans, p->n_layers, 2 * ((p->n_kv + kHeadsPerCta - 1) / kHeadsPerCta)), 32 * kHeadsPerCta, 0, st>>>(
-            list, reinterpret_cast<uint4*>(p->k), reinterpret_cast<uint4*>(p->v), p->n_pages, p->n_kv, p->dim * 2 / 16);
+        if (n <= kFewMoves) launch_list<kFewMoves>(p, moves.data() + at, n, st);
+        else launch_list<kMovesPerLaunch>(p, moves.data() + at, n, st);
         POOL_CK(cudaGetLastError());
     }
     p->end(st);
