@@ -105,7 +105,7 @@ __device__ __forceinline__ uint32_t tile_at(int row, int c) {
 // results in shared memory.
 template <typename T, int D, int W>
 __global__ void __launch_bounds__(32 * W, W == 1 ? TileShape<D>::RESIDENT : 1)
-k_attend_tiles(PlanView pv, Tensors<T> x, int item0, int heads_per) {
+k_attend_tiles(PlanView pv, Tensors<T> x, int item0, int heads_per, int folds) {
     using S = TileShape<D>;
     constexpr int NT = S::KEYS / 8, DT = D / 8, KS = D / 16;   // key tiles, dim tiles, steps along the dims
     extern __shared__ __align__(1024) unsigned char ring[];
@@ -358,7 +358,9 @@ k_attend_tiles(PlanView pv, Tensors<T> x, int item0, int heads_per) {
         }
     }
     auto mine = [&](int d) { return W == 1 || d % W == warp; };
-    dependents_wait();   // the parts of the launch before
+    // The parts of the launch before.  Where none are folded in, one CTA waits, so that this launch does not end before that
+    // one, and the others go on beside it.
+    if (folds || blockIdx.x == gridDim.x - 1) dependents_wait();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         if (!live[i] || limit[i] <= it.pos0) continue;   // such a row has no part here
@@ -522,7 +524,7 @@ int sm_count(int device) {
 struct t2sx_plan {
     t2sx_pool* pool = nullptr;
     int n_heads = 0, n_sm = 148;
-    bool ready = false, shared_rows = false, small = false, tc_writes = false;
+    bool ready = false, shared_rows = false, small = false, tc_writes = false, folds = false;
     int32_t most_parts = 0;            // of a token in `joins`
     int64_t launch_keys[2] = {0, 0};   // of the items of the launches of k_attend_tiles
     CUtensorMap map_k, map_v;
@@ -759,10 +761,12 @@ static int64_t build_items(t2sx_plan* a) {
     }
     int64_t parts = 0;
     a->most_parts = 0;
+    a->folds = false;
     for (Token& t : a->info) {
         t.part_at = (int32_t)std::min<int64_t>(parts, INT32_MAX);
         if (t.n_parts > 1) parts += t.n_parts;
         t.ends_here &= t.n_parts <= kFoldParts;
+        a->folds |= t.ends_here && t.n_parts > 1;
         if (t.n_parts > 1 && !t.ends_here) {
             a->joins.push_back(t);
             a->most_parts = std::max(a->most_parts, t.n_parts);
@@ -891,13 +895,13 @@ static cudaError_t launch_attend(t2sx_plan* a, Tensors<T> x, int layer, cudaStre
         cudaFuncSetAttribute(k_attend_tiles<T, D, S::TEAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TEAM * S::RING);
     });
     if (a->small)
-        return launch(k_attend_tiles<T, D, S::TEAM>, dim3((unsigned)w.n_own * w.n_kv), 32 * S::TEAM, S::TEAM * S::RING, st, false, w, x, 0, 1);
+        return launch(k_attend_tiles<T, D, S::TEAM>, dim3((unsigned)w.n_own * w.n_kv), 32 * S::TEAM, S::TEAM * S::RING, st, false, w, x, 0, 1, 1);
     auto tiles = [&](int item0, int n, bool early) {
         // Short items (below kLongItem keys, on average) share a warp, as many heads as leave several warps for each place:
         // a long one hides its own start.
         const int64_t places = (int64_t)a->n_sm * S::RESIDENT, keys = n ? a->launch_keys[item0 == w.n_tc && w.n_shared ? 0 : 1] / n : 0;
         const int64_t heads = std::min<int64_t>({(int64_t)w.n_kv, (int64_t)n * w.n_kv / (places * kWarpsPerPlace) + 1, kLongItem / (keys + 1) + 1});
-        return n ? launch(k_attend_tiles<T, D, 1>, dim3((unsigned)n * ((w.n_kv + heads - 1) / heads)), 32, S::RING, st, early, w, x, item0, (int)heads)
+        return n ? launch(k_attend_tiles<T, D, 1>, dim3((unsigned)n * ((w.n_kv + heads - 1) / heads)), 32, S::RING, st, early, w, x, item0, (int)heads, item0 == w.n_tc + w.n_shared ? (int)a->folds : 0)
                  : cudaSuccess;
     };
     cudaError_t e = cudaSuccess;
