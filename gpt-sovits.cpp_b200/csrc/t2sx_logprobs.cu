@@ -31,8 +31,8 @@ __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 constexpr int kGroup = 4;            // 16-byte vectors that a thread has in flight
-constexpr int kCandidates = 1024;    // of one CTA (a warp's share of it for rows of one warp)
-constexpr int kHits = 512;           // slots of one CTA that candidates come from (a warp's share likewise)
+constexpr int kCandidates = 1024;    // of one CTA of eight warps, a quarter of it for rows of fewer
+constexpr int kHits = 512;           // slots of one CTA that candidates come from (a quarter likewise)
 constexpr int kMaxTop = 32;
 constexpr int kMaxSplit = 8;         // CTAs per row (a portable cluster)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -80,6 +80,16 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         "l"(*reinterpret_cast<unsigned long long*>(&c)));
     return *reinterpret_cast<float2*>(&r);
 }
+
+// Masks of two comparisons, 0xFFFF for each half, added up modulo 2^32: with l ones in the low halves and h in the high
+// ones that is 65536 (l - h) - l (less than 65536 of either).
+struct CountMasks {
+    unsigned acc = 0;
+    __device__ __forceinline__ int sum() const {
+        const unsigned l = -acc & 0xFFFFu;
+        return (int)(l + (l - ((acc + l) >> 16) & 0xFFFFu));
+    }
+};
 
 // A 16-byte vector of logits: its elements in f32, its maximum (NaN left out), -inf in every place.
 template <typename T>
@@ -137,13 +147,12 @@ struct Vec<__half> {
         }
         return fmaxf(__low2float(m), __high2float(m));
     }
-    struct Count {   // ones added up in 16 bits: exact up to 256, and a group has 16 for each half
-        __half2 acc = __float2half2_rn(0.0f);
+    struct Count : CountMasks {
         __device__ __forceinline__ void add(const uint4& u, float above) {
             const __half2 *h = reinterpret_cast<const __half2*>(&u), a = __float2half2_rn(above);
-            acc = __hadd2(acc, __hadd2(__hadd2(__hgt2(h[0], a), __hgt2(h[1], a)), __hadd2(__hgt2(h[2], a), __hgt2(h[3], a))));
+            acc += __hgt2_mask(h[0], a) + __hgt2_mask(h[1], a);
+            acc += __hgt2_mask(h[2], a) + __hgt2_mask(h[3], a);
         }
-        __device__ __forceinline__ int sum() const { return (int)(__low2float(acc) + __high2float(acc)); }
     };
     static __device__ __forceinline__ float below(float x) {
         const unsigned b = __half_as_ushort(__float2half_rn(x));
@@ -175,13 +184,12 @@ struct Vec<__nv_bfloat16> {
         }
         return fmaxf(__low2float(m), __high2float(m));
     }
-    struct Count {   // ones added up in 16 bits: exact up to 256, and a group has 16 for each half
-        __nv_bfloat162 acc = __float2bfloat162_rn(0.0f);
+    struct Count : CountMasks {
         __device__ __forceinline__ void add(const uint4& u, float above) {
             const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162*>(&u), a = __float2bfloat162_rn(above);
-            acc = __hadd2(acc, __hadd2(__hadd2(__hgt2(h[0], a), __hgt2(h[1], a)), __hadd2(__hgt2(h[2], a), __hgt2(h[3], a))));
+            acc += __hgt2_mask(h[0], a) + __hgt2_mask(h[1], a);
+            acc += __hgt2_mask(h[2], a) + __hgt2_mask(h[3], a);
         }
-        __device__ __forceinline__ int sum() const { return (int)(__low2float(acc) + __high2float(acc)); }
     };
     static __device__ __forceinline__ float below(float x) {
         const unsigned b = __bfloat16_as_ushort(__float2bfloat16_rn(x));
@@ -253,26 +261,30 @@ struct Shared {   // of one row's threads in a CTA
     Stat stat[WARPS];
     float best_max[WARPS][32];
     int count, n_hits;
-    unsigned short hits[WARPS == 1 ? kHits / 4 : kHits];   // slots that reach T0: number x threads + thread
+    unsigned short hits[WARPS < 8 ? kHits / 4 : kHits];   // slots that reach T0: number x threads + thread
     unsigned long long best[WARPS];
-    static constexpr int PARTS = WARPS == 1 ? 1 : kMaxSplit;
+    static constexpr int PARTS = WARPS < 8 ? 1 : kMaxSplit;
     Stat joined[PARTS];                                  // in the first CTA of a row: all of its CTAs'
     unsigned long long lists[PARTS][kMaxTop];
-    unsigned long long cand[WARPS == 1 ? kCandidates / 4 : kCandidates];
+    unsigned long long cand[WARPS < 8 ? kCandidates / 4 : kCandidates];
 };
 
-// WARPS == 1: a warp per row, four rows in a CTA.  Else a row per CTA, or per cluster of `split` CTAs:
+// WARPS == 1: a warp per row, four rows in a CTA.  Else a row per CTA, or (WARPS == 8) per cluster of `split` CTAs:
 // each takes a range of the row's vectors, and the first one joins what they found.
+//
+// Bound by arithmetic, not by the bytes, for 16-bit logits: an element is an exponential (16 a cycle and SM), three packed
+// operations and a conversion.  2048 rows of 100003 in bf16 with the 20 best take 101 us, 4.1 TB/s; 4 rows of 131072 in f16
+// 10.3 us, of which most is the way from launch to the joined lists; 2048 rows of 1025 in f32 8.2 us.
 template <typename T, int WARPS>
-__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS, WARPS == 1 ? 6 : 4)
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS, WARPS == 1 ? 6 : 32 / WARPS)
 k_logprobs(const T* __restrict__ logits, Args a) {
     constexpr int E = Vec<T>::E, N = 32 * WARPS, ROWS = WARPS == 1 ? 4 : 1;
-    constexpr int CAND = WARPS == 1 ? kCandidates / 4 : kCandidates, HITS = WARPS == 1 ? kHits / 4 : kHits;
+    constexpr int CAND = WARPS < 8 ? kCandidates / 4 : kCandidates, HITS = WARPS < 8 ? kHits / 4 : kHits;
     extern __shared__ __align__(16) unsigned char raw[];
     const int sub = WARPS == 1 ? threadIdx.x >> 5 : 0, tid = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
     const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
     Shared<WARPS>& sh = reinterpret_cast<Shared<WARPS>*>(raw)[sub];
-    const int split = WARPS == 1 ? 1 : (int)gridDim.y, part = WARPS == 1 ? 0 : (int)blockIdx.y;
+    const int split = WARPS < 8 ? 1 : (int)gridDim.y, part = WARPS < 8 ? 0 : (int)blockIdx.y;
     const long long row = (long long)blockIdx.x * ROWS + sub;
     if (WARPS == 1 && row >= a.rows) return;   // warps of such a CTA wait for none of the others
     auto sync = [] {
@@ -584,10 +596,20 @@ cudaError_t launch(const T* x, Args a, int split, cudaStream_t st) {
 }
 
 template <typename T>
-cudaError_t dispatch(const T* x, const Args& a, cudaStream_t st) {
-    if (a.vocab <= 2048) return launch<T, 1>(x, a, 1, st);
+cudaError_t dispatch(const T* x, const Args& a, int sms, cudaStream_t st) {
+    // Warps of a row: those that let all rows run at one time, since what follows a row's pass (the merges of the
+    // warps' maxima, the candidates) costs each of its warps as much.  With 1, 2, 4, 8 warps, 20 best, in us:
+    //   2048 x 1025 f32   10.4  10.4  14.5  26.8        2048 x 200 f32      8.3  10.3  14.4  26.8
+    //   2048 x 4096 f32   16.6  14.5  18.6  27.7        2048 x 100003 bf16  115   94    95    99
+    //   1184 x 50000 bf16 49.5  37.1  35.2  41.2        512 x 32000 f16    28.9  20.4  16.6  17.4
+    //   256 x 1025 f32     8.4   6.8   6.3   8.3        8 x 1025 f32        8.3   6.4   6.2   7.2
+    //   256 x 32000 bf16  30.9  17.1  12.5  12.5        4 x 131072 f16     82.6   -     -    18.8
+    if (a.rows > 8 * sms) return a.vocab <= 2048 ? launch<T, 1>(x, a, 1, st) : launch<T, 2>(x, a, 1, st);
+    if (a.rows > 2 * sms || a.vocab <= 4096) return launch<T, 4>(x, a, 1, st);
+    // CTAs of a row: 4 x 131072 takes 18.8, 14.6, 12.4, 11.6 us with 1, 2, 4, 8 of them; 64 x 8192 8.3 with one, 10.4
+    // with four
     int split = 1;
-    while (split < kMaxSplit && (long long)a.rows * split * 2 <= 296 && a.vocab / (2 * split) >= 4096) split *= 2;
+    while (split < kMaxSplit && a.rows * split <= sms && a.vocab / (2 * split) >= 4096) split *= 2;
     return launch<T, 8>(x, a, split, st);
 }
 
@@ -614,12 +636,15 @@ extern "C" int t2sx_token_logprobs(int32_t device, int32_t type, int64_t rows, i
     DeviceGuard dg;
     cudaError_t e = dg.set(device);
     if (e != cudaSuccess) return t2sx_set_error(T2SX_ERR_CUDA, cudaGetErrorString(e));
+    int sms = 0;
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess) return t2sx_set_error(T2SX_ERR_CUDA, cudaGetErrorString(e));
     cudaStream_t st = (cudaStream_t)stream;
     const Args a = {(long long)stride, (int)rows, (int)vocab, top_k, 1, tokens_dev, logprob_dev, entropy_dev, rank_dev, top_ids_dev,
                     top_logprobs_dev};
-    if (type == T2SX_TYPE_F32) e = dispatch((const float*)logits_dev, a, st);
-    else if (type == T2SX_TYPE_F16) e = dispatch((const __half*)logits_dev, a, st);
-    else e = dispatch((const __nv_bfloat16*)logits_dev, a, st);
+    if (type == T2SX_TYPE_F32) e = dispatch((const float*)logits_dev, a, sms, st);
+    else if (type == T2SX_TYPE_F16) e = dispatch((const __half*)logits_dev, a, sms, st);
+    else e = dispatch((const __nv_bfloat16*)logits_dev, a, sms, st);
     if (e != cudaSuccess) return t2sx_set_error(T2SX_ERR_CUDA, cudaGetErrorString(e));
     return T2SX_OK;
 }
