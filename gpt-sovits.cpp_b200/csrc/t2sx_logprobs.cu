@@ -322,7 +322,14 @@ k_logprobs(const T* __restrict__ logits, Args a) {
 #pragma unroll
         for (int g = 0; g < kGroup; ++g) {
             c[g] = u[g];
-            u[g] = load(base + (kGroup + g) * N + tid);
+            u[g] = Vec<T>::none();
+        }
+        if (base + 2 * kGroup * N <= v1) {
+#pragma unroll
+            for (int g = 0; g < kGroup; ++g) u[g] = __ldg(xv + (base + tid) + (kGroup + g) * N);
+        } else if (base + kGroup * N < v1) {
+#pragma unroll
+            for (int g = 0; g < kGroup; ++g) u[g] = load(base + (kGroup + g) * N + tid);
         }
         const float g_max = Vec<T>::max(c);
         slot = fmaxf(slot, g_max);
@@ -343,11 +350,16 @@ k_logprobs(const T* __restrict__ logits, Args a) {
         }
         if (g_max >= xt) {
             typename Vec<T>::Count more;
+            // up to the token equal values come before it, too
+            const bool after = base * E - off > t;
+            if ((after || (base + kGroup * N) * E - off <= t) && xt > -INFINITY) {
+#pragma unroll
+                for (int g = 0; g < kGroup; ++g) more.add(c[g], after ? xt : xt_below);
+            } else
 #pragma unroll
             for (int g = 0; g < kGroup; ++g) {
                 const int vec = base + g * N + tid, j = vec * E - off;
                 if ((j + E <= t || j > t) && xt > -INFINITY) {
-                    // up to the token equal values come before it, too
                     more.add(c[g], j > t ? xt : xt_below);
                 } else if (vec < v1) {
                     const unsigned b[4] = {c[g].x, c[g].y, c[g].z, c[g].w};
