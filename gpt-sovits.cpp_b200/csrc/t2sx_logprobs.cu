@@ -272,9 +272,10 @@ struct Shared {   // of one row's threads in a CTA
 // WARPS == 1: a warp per row, four rows in a CTA.  Else a row per CTA, or (WARPS == 8) per cluster of `split` CTAs:
 // each takes a range of the row's vectors, and the first one joins what they found.
 //
-// Bound by arithmetic, not by the bytes, for 16-bit logits: an element is an exponential (16 a cycle and SM), three packed
-// operations and a conversion.  2048 rows of 100003 in bf16 with the 20 best take 101 us, 4.1 TB/s; 4 rows of 131072 in f16
-// 10.3 us, of which most is the way from launch to the joined lists; 2048 rows of 1025 in f32 8.2 us.
+// Bound by issue and the exponential unit for 16-bit logits: an element is an exponential (16 a cycle and SM) and some eight
+// other instructions, packed ones counted once.  2048 rows of 100003 in bf16 with the 20 best take 85 us, 4.8 TB/s (77 without
+// list and rank); 4 rows of 131072 in f16 10.3 us, of which most is the way from launch to the joined lists; 2048 rows of 1025 in
+// f32 8.2 us.
 template <typename T, int WARPS>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS, WARPS == 1 ? 6 : 32 / WARPS)
 k_logprobs(const T* __restrict__ logits, Args a) {
@@ -611,11 +612,11 @@ template <typename T>
 cudaError_t dispatch(const T* x, const Args& a, int sms, cudaStream_t st) {
     // Warps of a row: those that let all rows run at one time, since what follows a row's pass (the merges of the
     // warps' maxima, the candidates) costs each of its warps as much.  With 1, 2, 4, 8 warps, 20 best, in us:
-    //   2048 x 1025 f32   10.4  10.4  14.5  26.8        2048 x 200 f32      8.3  10.3  14.4  26.8
-    //   2048 x 4096 f32   16.6  14.5  18.6  27.7        2048 x 100003 bf16  115   94    95    99
-    //   1184 x 50000 bf16 49.5  37.1  35.2  41.2        512 x 32000 f16    28.9  20.4  16.6  17.4
-    //   256 x 1025 f32     8.4   6.8   6.3   8.3        8 x 1025 f32        8.3   6.4   6.2   7.2
-    //   256 x 32000 bf16  30.9  17.1  12.5  12.5        4 x 131072 f16     82.6   -     -    18.8
+    //   2048 x 1025 f32   10.4  10.4  14.6  27.2        2048 x 200 f32      8.3  10.3  14.4  26.8
+    //   2048 x 4096 f32   16.6  14.5  18.6  28.8        2048 x 100003 bf16  105   84.6  86.1  92.6
+    //   1184 x 50000 bf16 46.8  33.4  32.9  39.2        512 x 32000 f16    25.0  18.2  15.5  16.6
+    //   256 x 1025 f32     8.4   7.0   6.3   8.3        8 x 1025 f32        8.3   6.5   6.2   7.4
+    //   256 x 32000 bf16  26.9  15.8  12.5  12.4        4 x 131072 f16     82.6   -     -    18.8
     if (a.rows > 8 * sms) return a.vocab <= 2048 ? launch<T, 1>(x, a, 1, st) : launch<T, 2>(x, a, 1, st);
     if (a.rows > 2 * sms || a.vocab <= 4096) return launch<T, 4>(x, a, 1, st);
     // CTAs of a row: 4 x 131072 takes 18.8, 14.6, 12.4, 11.6 us with 1, 2, 4, 8 of them; 64 x 8192 8.3 with one, 10.4

@@ -21,20 +21,18 @@ using namespace t2sx::attn;
 
 namespace {
 
-#ifndef C32
-#define C32 32,3,16
-#define C64 32,3,9
-#define C128 32,3,4
-#endif
 constexpr int kTileRows = 16;        // rows of a warp's tile (the m of mma.m16n8k16)
 constexpr int kWarpsPerPlace = 3;    // warps of a launch for each one that the device holds at a time, where items are many
-constexpr int kLongItem = 256;       // keys
+constexpr int kLongItem = 256;       // keys: shorter items of several K/V heads share a warp; 2048 sequences with 20 positions each of
+                                     // their own take 87 us so and 93 without, with 100 each 116 and 123
 constexpr int kMinChunk = 2;         // pages of a split at least
 constexpr int kSplitCost = 4, kJoinCost = 4;   // in pages: what a split costs beside its pages, and joining parts
 constexpr int kTcMinRowDims = 2049;  // rows x head dim of a node from which the tcgen05 kernel takes it (see build_items)
 constexpr int kTcMinChunk = 4;       // pages of a split of such a node at least
-constexpr int kFoldParts = 4;        // parts of a token up to which the item of its own pages folds them in, one after the other
-constexpr int kSmallPages = 32;      // pages of a sequence in a small step at most
+constexpr int kFoldParts = 4;        // parts of a token up to which the item of its own pages folds them in, one after the other:
+                                     // 2048 sequences, 32 to a prompt, take 340 us so and 351 with a launch that joins them; with up
+                                     // to eight parts 256 sequences of one long prompt take 117 instead of 107
+constexpr int kSmallWork = 2048;     // pages x head dim of a CTA of a small step at most, an eighth of it with two CTAs to an SM
 
 __device__ __forceinline__ void mma16816(__half, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -79,13 +77,14 @@ k_write_rows(const Token* __restrict__ rows_of, int rows, const uint4* __restric
 }
 
 // Tiles of a head dimension: keys per stage of a warp's ring, its stages, the warps of an SM that this leaves
-// room for, and the warps of a CTA that shares out one item.
-template <int KEYS_, int STAGES_, int RESIDENT_>
-struct Cfg { static constexpr int KEYS = KEYS_, STAGES = STAGES_, RESIDENT = RESIDENT_; };
+// room for, and the warps of a CTA that shares out one item.  Measured as (keys, stages, warps), in us:
+//   dim 32   2048 sequences, 32 to a prompt, 500 positions each of their own: (32, 3, 16) 349, (32, 4, 13) 352, (64, 3, 9) 363, (64, 2, 13) 386
+//   dim 64   64 sequences of 8000, 8 heads:  (32, 3, 9) 149, (16, 4, 13) 157, (16, 6, 9) 159, (32, 2, 13) 171, (64, 2, 6) 172
+//   dim 128  64 sequences of 4000, 8 heads:  (32, 3, 4) 141, (16, 4, 7) 143, (16, 3, 8) 148, (16, 6, 4) 154, (32, 2, 6) 173
+// Two stages in flight keep the copies going; beyond that fewer warps are left than the softmax needs.
 template <int D>
 struct TileShape {
-    using C = std::conditional_t<D == 32, Cfg<C32>, std::conditional_t<D == 64, Cfg<C64>, Cfg<C128>>>;
-    static constexpr int KEYS = C::KEYS, STAGES = C::STAGES, RESIDENT = C::RESIDENT, TEAM = D == 128 ? 4 : 8;
+    static constexpr int KEYS = 32, STAGES = 3, RESIDENT = D == 32 ? 16 : D == 64 ? 9 : 4, TEAM = D == 128 ? 4 : 8;
     static constexpr int HALF = KEYS * D * 2;   // bytes of a stage's K (or V)
     static constexpr int RING = STAGES * 2 * HALF;
     static_assert(RING >= kTileRows * D * 4, "a warp's results take the place of its ring");
@@ -103,6 +102,12 @@ __device__ __forceinline__ uint32_t tile_at(int row, int c) {
 // running on from one to the next, so that a short item's start is paid once.  W > 1: a
 // CTA per (item, K/V head), whose warps share out the item's tiles, each with a ring of its own, and join their
 // results in shared memory.
+//
+// Bound by the cache's bytes where a page has few rows: 2048 sequences, 32 to a prompt, 16 heads of 32 dims, some
+// 500 positions each of their own, take 340 us for 2.2 GB (6.4 TB/s); one sequence of 65536 positions, 8 heads of 128, 53 us.
+// Warps alone (no CTA-wide barrier in the loop) because items differ in length; mma.sync because a page of a few
+// rows is a memory-bound product, whatever the tensor cores' rate.  A small step runs the W > 1 form as its only
+// launch: 6.9 us for four candidates of one prompt.
 template <typename T, int D, int W>
 __global__ void __launch_bounds__(32 * W, W == 1 ? TileShape<D>::RESIDENT : 1)
 k_attend_tiles(PlanView pv, Tensors<T> x, int item0, int heads_per, int folds) {
@@ -198,211 +203,215 @@ k_attend_tiles(PlanView pv, Tensors<T> x, int item0, int heads_per, int folds) {
     const bool upper = it.rows > 8;
     int stage = 0;
     for (int kvh = kv0; kvh < kv1; ++kvh) {
-    int head_of[2];
+        int head_of[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) head_of[i] = kvh * group + g_of[i];
-    auto part_index = [&](int i, int part) { return ((size_t)part * group + g_of[i]) * pv.n_kv + kvh; };
-    uint4 own_word = make_uint4(0, 0, 0, 0);
-    if (own0) own_word = *own_src(own0, kvh);
-    uint32_t qf[KS][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(x.q + q_at[i] + (long long)kvh * group * D);
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            qf[k][i] = live[i] ? src[k * 8 + lane % 4] : 0;
-            qf[k][i + 2] = live[i] ? src[k * 8 + 4 + lane % 4] : 0;
-        }
-    }
-    float o[DT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    // The parts of the launch before: the first head's are folded in at its end (they may not be there yet), those
-    // of the others are what the head starts from.
-    const bool start_from = W == 1 && kvh > kv0;
-    int folded[2] = {0, 0};
-    if (start_from) {
+        for (int i = 0; i < 2; ++i) head_of[i] = kvh * group + g_of[i];
+        auto part_index = [&](int i, int part) { return ((size_t)part * group + g_of[i]) * pv.n_kv + kvh; };
+        uint4 own_word = make_uint4(0, 0, 0, 0);
+        if (own0) own_word = *own_src(own0, kvh);
+        uint32_t qf[KS][4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            if (!live[i] || !ends[i] || n_parts[i] < 2 || limit[i] <= it.pos0) continue;
-            const size_t at = part_index(i, part[i] - 1);
-            const float2 ml = __ldcg(&pv.part_ml[at]);
-            m[i] = ml.x;
-            l[i] = lane % 4 == 0 ? ml.y : 0.0f;
-            const float2* src = reinterpret_cast<const float2*>(pv.part_o + at * D);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const float2 y = __ldcg(&src[d * 4 + lane % 4]);
-                o[d][2 * i] = y.x;
-                o[d][2 * i + 1] = y.y;
-            }
-            folded[i] = 1;
-        }
-    }
-    for (int t = first; t < tiles; ++t) {
-        cp_wait<S::STAGES - 2>();
-        __syncwarp();
-        const uint32_t kt = ring0 + stage * 2 * S::HALF, vt = kt + S::HALF;
-        stage = stage + 1 == S::STAGES ? 0 : stage + 1;
-        const int pos = it.pos0 + t * S::KEYS;
-        float s[NT][4] = {};
-#pragma unroll
-        for (int n = 0; n < NT; n += 2)
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(x.q + q_at[i] + (long long)kvh * group * D);
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                uint32_t b[4];
-                ldsm4(b, kt + tile_at<D>(n * 8 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
-                mma16816(T(), s[n], qf[k], b[0], b[1]);
-                mma16816(T(), s[n + 1], qf[k], b[2], b[3]);
-            }
-        const bool masked = pos + S::KEYS > free_to;
-        uint32_t p[NT][2];
-        bool grew = false;
-        float alpha[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (i == 1 && !upper) {
-                alpha[1] = 1.0f;
-#pragma unroll
-                for (int n = 0; n < NT; ++n) p[n][1] = 0;
-                break;
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float y = s[n][2 * i + e] * x.scale2;
-                    if (masked && pos + n * 8 + 2 * (lane % 4) + e >= limit[i]) y = -INFINITY;
-                    s[n][2 * i + e] = y;
-                    mx = fmaxf(mx, y);
-                }
-            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-            mx = fmaxf(mx, m[i]);
-            const float base = mx == -INFINITY ? 0.0f : mx - kWeightExp;
-            alpha[i] = m[i] == -INFINITY ? 0.0f : ex2(m[i] - mx);
-            grew |= mx > m[i];
-            m[i] = mx;
-            float sum = 0.0f;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float a = ex2(s[n][2 * i] - base), b = ex2(s[n][2 * i + 1] - base);
-                sum += a + b;
-                p[n][i] = pack2(T(), a, b);
-            }
-            l[i] = fmaf(l[i], alpha[i], sum);
-        }
-        if (__any_sync(~0u, grew)) {
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                o[d][0] *= alpha[0]; o[d][1] *= alpha[0];
-                o[d][2] *= alpha[1]; o[d][3] *= alpha[1];
+                qf[k][i] = live[i] ? src[k * 8 + lane % 4] : 0;
+                qf[k][i + 2] = live[i] ? src[k * 8 + 4 + lane % 4] : 0;
             }
         }
+        float o[DT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        // The parts of the launch before: the first head's are folded in at its end (they may not be there yet), those
+        // of the others are what the head starts from.
+        const bool start_from = W == 1 && kvh > kv0;
+        int folded[2] = {0, 0};
+        if (start_from) {
 #pragma unroll
-        for (int n = 0; n < NT; n += 2) {
-            const uint32_t a[4] = {p[n][0], p[n][1], p[n + 1][0], p[n + 1][1]};
-#pragma unroll
-            for (int d = 0; d < DT; d += 2) {
-                uint32_t b[4];
-                ldsm4_t(b, vt + tile_at<D>(n * 8 + (lane & 15), d + (lane >> 4)));
-                mma16816(T(), o[d], a, b[0], b[1]);
-                mma16816(T(), o[d + 1], a, b[2], b[3]);
-            }
-        }
-        __syncwarp();
-        request();
-    }
-    if (own0) *own_dst(own0, kvh) = own_word;
-    for (int r = 1; r < it.rows; ++r)
-        if (const Token* t = own(r)) *own_dst(t, kvh) = *own_src(t, kvh);
-    float sum[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        sum[i] = l[i];
-        sum[i] += __shfl_xor_sync(~0u, sum[i], 1);
-        sum[i] += __shfl_xor_sync(~0u, sum[i], 2);
-    }
-    if constexpr (W > 1) {
-        // the warps' results in the place of their rings; then each warp joins the dim tiles warp, warp + W, ...
-        __shared__ float2 ml[W][16];
-        cp_wait<0>();
-        __syncthreads();
-        float2* all_o = reinterpret_cast<float2*>(ring);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (lane % 4 == 0) ml[warp][lane / 4 + 8 * i] = make_float2(m[i], sum[i]);
-#pragma unroll
-            for (int d = 0; d < DT; ++d) all_o[((warp * 2 + i) * DT + d) * 32 + lane] = make_float2(o[d][2 * i], o[d][2 * i + 1]);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float M = -INFINITY;
-            for (int j = 0; j < W; ++j) M = fmaxf(M, ml[j][lane / 4 + 8 * i].x);
-            m[i] = M;
-            sum[i] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) o[d][2 * i] = o[d][2 * i + 1] = 0.0f;
-            for (int j = 0; j < W; ++j) {
-                const float2 part = ml[j][lane / 4 + 8 * i];
-                const float f = part.x == -INFINITY ? 0.0f : ex2(part.x - M);
-                sum[i] = fmaf(part.y, f, sum[i]);
+            for (int i = 0; i < 2; ++i) {
+                if (!live[i] || !ends[i] || n_parts[i] < 2 || limit[i] <= it.pos0) continue;
+                const size_t at = part_index(i, part[i] - 1);
+                const float2 ml = __ldcg(&pv.part_ml[at]);
+                m[i] = ml.x;
+                l[i] = lane % 4 == 0 ? ml.y : 0.0f;
+                const float2* src = reinterpret_cast<const float2*>(pv.part_o + at * D);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    if (d % W != warp) continue;
-                    const float2 y = all_o[((j * 2 + i) * DT + d) * 32 + lane];
-                    o[d][2 * i] = fmaf(y.x, f, o[d][2 * i]);
-                    o[d][2 * i + 1] = fmaf(y.y, f, o[d][2 * i + 1]);
+                    const float2 y = __ldcg(&src[d * 4 + lane % 4]);
+                    o[d][2 * i] = y.x;
+                    o[d][2 * i + 1] = y.y;
+                }
+                folded[i] = 1;
+            }
+        }
+        for (int t = first; t < tiles; ++t) {
+            cp_wait<S::STAGES - 2>();
+            __syncwarp();
+            const uint32_t kt = ring0 + stage * 2 * S::HALF, vt = kt + S::HALF;
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+            const int pos = it.pos0 + t * S::KEYS;
+            float s[NT][4] = {};
+#pragma unroll
+            for (int n = 0; n < NT; n += 2)
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    uint32_t b[4];
+                    ldsm4(b, kt + tile_at<D>(n * 8 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+                    mma16816(T(), s[n], qf[k], b[0], b[1]);
+                    mma16816(T(), s[n + 1], qf[k], b[2], b[3]);
+                }
+            const bool masked = pos + S::KEYS > free_to;
+            uint32_t p[NT][2];
+            bool grew = false;
+            float alpha[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (i == 1 && !upper) {
+                    alpha[1] = 1.0f;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) p[n][1] = 0;
+                    break;
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float y = s[n][2 * i + e] * x.scale2;
+                        if (masked && pos + n * 8 + 2 * (lane % 4) + e >= limit[i]) y = -INFINITY;
+                        s[n][2 * i + e] = y;
+                        mx = fmaxf(mx, y);
+                    }
+                mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+                mx = fmaxf(mx, m[i]);
+                const float base = mx == -INFINITY ? 0.0f : mx - kWeightExp;
+                alpha[i] = m[i] == -INFINITY ? 0.0f : ex2(m[i] - mx);
+                grew |= mx > m[i];
+                m[i] = mx;
+                float sum = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float a = ex2(s[n][2 * i] - base), b = ex2(s[n][2 * i + 1] - base);
+                    sum += a + b;
+                    p[n][i] = pack2(T(), a, b);
+                }
+                l[i] = fmaf(l[i], alpha[i], sum);
+            }
+            if (__any_sync(~0u, grew)) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    o[d][0] *= alpha[0]; o[d][1] *= alpha[0];
+                    o[d][2] *= alpha[1]; o[d][3] *= alpha[1];
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n += 2) {
+                const uint32_t a[4] = {p[n][0], p[n][1], p[n + 1][0], p[n + 1][1]};
+#pragma unroll
+                for (int d = 0; d < DT; d += 2) {
+                    uint32_t b[4];
+                    ldsm4_t(b, vt + tile_at<D>(n * 8 + (lane & 15), d + (lane >> 4)));
+                    mma16816(T(), o[d], a, b[0], b[1]);
+                    mma16816(T(), o[d + 1], a, b[2], b[3]);
+                }
+            }
+            __syncwarp();
+            request();
+        }
+        if (own0) *own_dst(own0, kvh) = own_word;
+        for (int r = 1; r < it.rows; ++r)
+            if (const Token* t = own(r)) *own_dst(t, kvh) = *own_src(t, kvh);
+        float sum[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            sum[i] = l[i];
+            sum[i] += __shfl_xor_sync(~0u, sum[i], 1);
+            sum[i] += __shfl_xor_sync(~0u, sum[i], 2);
+        }
+        if constexpr (W > 1) {
+            // the warps' results in the place of their rings; then each warp joins the dim tiles warp, warp + W, ...
+            __shared__ float2 ml[W][16];
+            cp_wait<0>();
+            __syncthreads();
+            float2* all_o = reinterpret_cast<float2*>(ring);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (lane % 4 == 0) ml[warp][lane / 4 + 8 * i] = make_float2(m[i], sum[i]);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) all_o[((warp * 2 + i) * DT + d) * 32 + lane] = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float M = -INFINITY;
+                for (int j = 0; j < W; ++j) M = fmaxf(M, ml[j][lane / 4 + 8 * i].x);
+                m[i] = M;
+                sum[i] = 0.0f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d][2 * i] = o[d][2 * i + 1] = 0.0f;
+                for (int j = 0; j < W; ++j) {
+                    const float2 part = ml[j][lane / 4 + 8 * i];
+                    const float f = part.x == -INFINITY ? 0.0f : ex2(part.x - M);
+                    sum[i] = fmaf(part.y, f, sum[i]);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        if (d % W != warp) continue;
+                        const float2 y = all_o[((j * 2 + i) * DT + d) * 32 + lane];
+                        o[d][2 * i] = fmaf(y.x, f, o[d][2 * i]);
+                        o[d][2 * i + 1] = fmaf(y.y, f, o[d][2 * i + 1]);
+                    }
                 }
             }
         }
-    }
-    auto mine = [&](int d) { return W == 1 || d % W == warp; };
-    // The parts of the launch before.  Where none are folded in, one CTA waits, so that this launch does not end before that
-    // one, and the others go on beside it.
-    if (folds || blockIdx.x == gridDim.x - 1) dependents_wait();
+        auto mine = [&](int d) { return W == 1 || d % W == warp; };
+        // The parts of the launch before.  Where none are folded in, one CTA waits, so that this launch does not end before that
+        // one, and the others go on beside it.
+        if (folds || blockIdx.x == gridDim.x - 1) dependents_wait();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if (!live[i] || limit[i] <= it.pos0) continue;   // such a row has no part here
-        if (n_parts[i] > 1 && !ends[i]) {
-            const size_t at = part_index(i, part[i]);
-            float2* dst = reinterpret_cast<float2*>(pv.part_o + at * D);
+        for (int i = 0; i < 2; ++i) {
+            if (!live[i] || limit[i] <= it.pos0) continue;   // such a row has no part here
+            if (n_parts[i] > 1 && !ends[i]) {
+                const size_t at = part_index(i, part[i]);
+                float2* dst = reinterpret_cast<float2*>(pv.part_o + at * D);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    if (mine(d)) dst[d * 4 + lane % 4] = make_float2(o[d][2 * i], o[d][2 * i + 1]);
+                if (lane % 4 == 0 && warp == 0) pv.part_ml[at] = make_float2(m[i], sum[i]);
+                continue;
+            }
+            if constexpr (W == 1) {
+                for (int j = n_parts[i] - 1 - folded[i]; j-- > 0;) {   // the other parts, if any
+                    const size_t at = part_index(i, part[i] - n_parts[i] + 1 + j);
+                    const float2 ml = __ldcg(&pv.part_ml[at]);
+                    const float2* src = reinterpret_cast<const float2*>(pv.part_o + at * D);
+                    float2 y[DT];
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) y[d] = __ldcg(&src[d * 4 + lane % 4]);
+                    const float M = fmaxf(m[i], ml.x), f = m[i] == -INFINITY ? 0.0f : ex2(m[i] - M), g = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
+                    m[i] = M;
+                    sum[i] = fmaf(sum[i], f, ml.y * g);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        o[d][2 * i] = fmaf(o[d][2 * i], f, y[d].x * g);
+                        o[d][2 * i + 1] = fmaf(o[d][2 * i + 1], f, y[d].y * g);
+                    }
+                }
+            }
+            const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
+            uint32_t* dst = reinterpret_cast<uint32_t*>(x.out + row_of[i] * x.out_stride + head_of[i] * D);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
-                if (mine(d)) dst[d * 4 + lane % 4] = make_float2(o[d][2 * i], o[d][2 * i + 1]);
-            if (lane % 4 == 0 && warp == 0) pv.part_ml[at] = make_float2(m[i], sum[i]);
-            continue;
+                if (mine(d)) dst[d * 4 + lane % 4] = pack2(T(), o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
+            if (x.lse && lane % 4 == 0 && warp == 0)
+                x.lse[(size_t)row_of[i] * (pv.n_kv * group) + head_of[i]] = (m[i] - kWeightExp + log2f(sum[i])) * kLn2;
         }
-        if constexpr (W == 1) {
-            for (int j = n_parts[i] - 1 - folded[i]; j-- > 0;) {   // the other parts, if any
-                const size_t at = part_index(i, part[i] - n_parts[i] + 1 + j);
-                const float2 ml = __ldcg(&pv.part_ml[at]);
-                const float2* src = reinterpret_cast<const float2*>(pv.part_o + at * D);
-                float2 y[DT];
-#pragma unroll
-                for (int d = 0; d < DT; ++d) y[d] = __ldcg(&src[d * 4 + lane % 4]);
-                const float M = fmaxf(m[i], ml.x), f = m[i] == -INFINITY ? 0.0f : ex2(m[i] - M), g = ml.x == -INFINITY ? 0.0f : ex2(ml.x - M);
-                m[i] = M;
-                sum[i] = fmaf(sum[i], f, ml.y * g);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    o[d][2 * i] = fmaf(o[d][2 * i], f, y[d].x * g);
-                    o[d][2 * i + 1] = fmaf(o[d][2 * i + 1], f, y[d].y * g);
-                }
-            }
-        }
-        const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
-        uint32_t* dst = reinterpret_cast<uint32_t*>(x.out + row_of[i] * x.out_stride + head_of[i] * D);
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-            if (mine(d)) dst[d * 4 + lane % 4] = pack2(T(), o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
-        if (x.lse && lane % 4 == 0 && warp == 0)
-            x.lse[(size_t)row_of[i] * (pv.n_kv * group) + head_of[i]] = (m[i] - kWeightExp + log2f(sum[i])) * kLn2;
-    }
     }
 }
 
-// Four warps, each with a (token, query head) of few parts: the lanes are D / 4 columns of four dims x 32 / (D / 4) parts.
+// Joining the parts: out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  Bound by the parts' bytes, which the launch before
+// has just left in the L2 cache, and by latency.
+//
+// Four warps, each with a (token, query head) of few parts (at most 32; 256 sequences of one long prompt take 107 us so and
+// 113 with a CTA for each of their rows): the lanes are D / 4 columns of four dims x 32 / (D / 4) parts.
 template <typename T, int D>
 __global__ void __launch_bounds__(128)
 k_join_few(PlanView pv, Tensors<T> x) {
@@ -714,7 +723,7 @@ static int64_t build_items(t2sx_plan* a) {
     // 55 and 56 without at head dim 128; at 64, 16 prompts of 4032 with 32 and 48 rows took 54 and 45 with, 47 and 60
     // without; at 32, with 48 and 64 rows, 30 and 31 with, 25 and 31 without.
     for (Node& nd : a->nodes) nd.tc = !a->small && (int64_t)nd.n_tokens * group * a->pool->dim >= kTcMinRowDims;
-    const int64_t warp_chunk = a->small ? kSmallPages : best_chunk(a, false, (int64_t)a->n_sm * resident_warps(a->pool->dim));
+    const int64_t warp_chunk = a->small ? INT32_MAX : best_chunk(a, false, (int64_t)a->n_sm * resident_warps(a->pool->dim));
     const int64_t tc_chunk = best_chunk(a, true, a->n_sm);
     a->tokens.resize(a->node_rows.size());
     for (const Node& nd : a->nodes) {
@@ -821,14 +830,16 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
             }
         }
         // A small step: a CTA for each (tile of rows, K/V head), all at one time, with no parts to join; its shared pages
-        // come from L2 however often they are read.
-        int64_t row_tiles = 0;
-        a->small = true;
+        // come from L2 however often they are read.  By CTAs, pages and head dim, us with it and without:
+        //   64, 6, 32: 6.9, 12.6     128, 24, 32: 10.5, 12.5    128, 6, 64: 8.4, 14.6    128, 24, 64: 12.7, 16.6
+        //   288, 6, 32: 12.0, 12.7   192, 24, 32: 15.0, 12.6    256, 6, 64: 14.6, 12.6   32, 24, 128: 24.7, 16.7
+        int64_t row_tiles = 0, longest = 0;
         for (int32_t i = 0; i < n; ++i) {
             row_tiles += ((int64_t)n_new[i] * (a->n_heads / p->n_kv) + kTileRows - 1) / kTileRows;
-            a->small &= n_new[i] == 0 || p->table[seqs[i]].size() <= (size_t)kSmallPages;
+            if (n_new[i]) longest = std::max(longest, (int64_t)p->table[seqs[i]].size());
         }
-        a->small &= row_tiles * p->n_kv <= 2 * a->n_sm;
+        const int64_t ctas = row_tiles * p->n_kv;
+        a->small = ctas <= 2 * a->n_sm && longest * p->dim <= (ctas <= a->n_sm ? kSmallWork : kSmallWork / 8);
         build_nodes(a, n, seqs, n_new);
         const int64_t n_parts = build_items(a);
         if (n_parts >= INT32_MAX || a->items.size() * p->n_kv > (size_t)INT32_MAX ||
@@ -896,13 +907,15 @@ static cudaError_t launch_attend(t2sx_plan* a, Tensors<T> x, int layer, cudaStre
     });
     if (a->small)
         return launch(k_attend_tiles<T, D, S::TEAM>, dim3((unsigned)w.n_own * w.n_kv), 32 * S::TEAM, S::TEAM * S::RING, st, false, w, x, 0, 1, 1);
-    auto tiles = [&](int item0, int n, bool early) {
+    auto tiles = [&](int which, bool early) {   // 0: pages of several sequences, 1: the others
+        const int n = which ? w.n_own : w.n_shared;
+        if (!n) return cudaSuccess;
         // Short items (below kLongItem keys, on average) share a warp, as many heads as leave several warps for each place:
         // a long one hides its own start.
-        const int64_t places = (int64_t)a->n_sm * S::RESIDENT, keys = n ? a->launch_keys[item0 == w.n_tc && w.n_shared ? 0 : 1] / n : 0;
+        const int64_t places = (int64_t)a->n_sm * S::RESIDENT, keys = a->launch_keys[which] / n;
         const int64_t heads = std::min<int64_t>({(int64_t)w.n_kv, (int64_t)n * w.n_kv / (places * kWarpsPerPlace) + 1, kLongItem / (keys + 1) + 1});
-        return n ? launch(k_attend_tiles<T, D, 1>, dim3((unsigned)n * ((w.n_kv + heads - 1) / heads)), 32, S::RING, st, early, w, x, item0, (int)heads, item0 == w.n_tc + w.n_shared ? (int)a->folds : 0)
-                 : cudaSuccess;
+        return launch(k_attend_tiles<T, D, 1>, dim3((unsigned)(n * ((w.n_kv + heads - 1) / heads))), 32, S::RING, st, early, w, x,
+                      w.n_tc + (which ? w.n_shared : 0), (int)heads, which ? (int)a->folds : 0);
     };
     cudaError_t e = cudaSuccess;
     bool early = false;   // a launch of this call comes before
@@ -919,9 +932,9 @@ static cudaError_t launch_attend(t2sx_plan* a, Tensors<T> x, int layer, cudaStre
         if (e == cudaSuccess) e = launch_tc(w, x, a->pool, a->map_k, a->map_v, layer * a->pool->n_pages, a->err_dev, early, st);
         early = true;
     }
-    if (e == cudaSuccess) e = tiles(w.n_tc, w.n_shared, early);
+    if (e == cudaSuccess) e = tiles(0, early);
     early |= w.n_shared > 0;
-    if (e == cudaSuccess) e = tiles(w.n_tc + w.n_shared, w.n_own, early);
+    if (e == cudaSuccess) e = tiles(1, early);
     if (e == cudaSuccess && w.n_joins) {
         const int64_t rows = (int64_t)w.n_joins * a->n_heads;
         e = a->most_parts <= 32 ? launch(k_join_few<T, D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, true, w, x)

@@ -8,12 +8,20 @@
 //              The maximum that the weights refer to is looked for, and the output rescaled, only when a
 //              tile's weights add up to 2^15 (f16 ends at 2^16);
 //   warp 8     TMA: the K and V tiles of the pages, in two rings;
-//   warps 9-10 the MMAs, one thread for each tile: S = Q K^T (M 128, N 64) into one of two score buffers of a tile, then O += P V with P from
-//              TMEM (M 128, N head dim).  S is issued two pages ahead, so that the tensor cores work while
-//              the softmax does.
+//   warps 9-10 the MMAs, one thread for each tile: S = Q K^T (M 128, N 64) into one of two score buffers of a
+//              tile, then O += P V with P from TMEM (M 128, N head dim).  S is issued two pages ahead, so that the
+//              tensor cores work while the softmax does.
 // TMEM columns of a tile: scores and weights 2 x 64, output from column 128 on.
-// Two tiles to a CTA because the L2 cache bounds the traffic: with one tile each and two CTAs per SM a tile
-// waited 600 cycles of 1700 for its keys.
+//
+// What bounds it: the tensor cores.  An MMA of M 128 and N 64 takes as long as one of N 128 (64 cycles for 16 of
+// the K index), so a page costs the two tiles 2 x (8 x 64 + 4 x 64) = 1536 cycles at head dim 128, and the loop takes
+// 1526.  At head dim 64 the MMAs take 1024, the exponentials (8 cycles to a warp's instruction) 1066, and the loop
+// 1555.  A step of 256 sequences over one prompt of 16384 positions (32 heads, 8 K/V heads of 128 dims, bf16; up to 256
+// positions each of their own) takes 107 us with all its launches, some 65 of them here.  When it took 116, it took with
+//   scores of 128 keys in one buffer (N 128): 135, and 128 with 16 softmax warps, since the MMAs then wait for the
+//              softmax; there is no TMEM for a second buffer of that size beside two outputs;
+//   one tile per CTA, two CTAs per SM: 153;    16 softmax warps on these buffers: 117;
+//   the tiles' softmax taking turns: 146;      a polynomial for 4 of 32 pairs of exponentials: 113, for 8: 117.
 //
 // Every wait is bounded; a CTA whose wait runs out raises its abort flag, lets its copies and MMAs land, writes
 // NaN and sets the plan's error word.
@@ -140,7 +148,7 @@ __device__ __forceinline__ void v_pack2(__nv_bfloat16, uint32_t& d, float2 a) {
 // The softmax weights of a row's scores in 16 bits, two to a word, and their sum: 2^(scale s - m + kWeightExp).
 // The exponential unit takes a warp's instruction every 8 cycles, and a warp issues in order: the multiplications of
 // later scores and the additions and conversions of earlier ones stand between the exponentials, which then follow
-// one another without a pause (left to the compiler the 64 of them took 1000 cycles instead of 560).
+// one another without a pause (left to the compiler the 64 of them took 1000 cycles instead of 610).
 template <typename T>
 __device__ __forceinline__ float weights(const uint32_t (&sc)[kKeys], uint32_t (&p)[kKeys / 2], float scale, float m) {
     constexpr int N = kKeys / 2, AHEAD = 4, LAG = 3;
