@@ -628,3 +628,45 @@ def test_logprobs_optional_outputs(t2sx_mod):
     lp = torch.empty(4, device="cuda")
     t2sx_mod.token_logprobs(0, 4, 50, x.data_ptr(), t.data_ptr(), lp.data_ptr(), stream=_stream())
     assert ((lp.double() - x.double().log_softmax(-1)[:, 0]).abs() < 2.0 ** -14).all()
+
+
+@gpu
+def test_candidates_together(t2sx_mod):
+    """candidates.draw(): scores of what it draws against a plain forward pass in 64 bits over each whole sequence.
+    Six roundings to f16 in each of two layers, of activations and as many of weights, independent of one another, move a
+    row by sqrt(24) 2^-12 of its length, and a logit by that share of its spread (0.02 x 512 / sqrt(512) = 0.45): 0.0006.
+    2^-8 is six times that."""
+    _need_gpu()
+    import candidates
+    import synth
+    tensors = [(n, a) for n, a in synth.tensor_values(3, n_layer=2)]
+    dec = candidates.Decoder(tensors)
+    rng = np.random.default_rng(5)
+    prompts = [rng.integers(0, candidates.EOS, m).tolist() for m in (130, 64, 1)]
+    found = candidates.draw(dec, prompts, each=5, steps=9, seed=1)
+    again = candidates.draw(dec, prompts, each=5, steps=9, seed=1)
+    assert found == again
+    w = {n: torch.tensor(a).double() for n, a in tensors}
+
+    def scores(tokens):
+        n, d = len(tokens), 512
+        freq = torch.exp(torch.arange(0, d, 2).double() * (-math.log(10000.0) / d))
+        angle = torch.arange(n).double()[:, None] * freq
+        x = w["encoder.audio_embedding"][tokens] + torch.stack([angle.sin(), angle.cos()], 2).flatten(1)
+        for i in range(2):
+            g = lambda name: w[f"attention.{i}.{name}"]
+            q, k, v = ((x @ g("qkv_w").T + g("qkv_b")).view(n, 3, 16, 32).permute(1, 2, 0, 3))
+            s = (q @ k.transpose(1, 2)) * 32 ** -0.5
+            s = s.masked_fill(torch.ones(n, n, dtype=torch.bool).triu(1), -math.inf).softmax(-1)
+            a = (s @ v).transpose(0, 1).reshape(n, d)
+            x = torch.nn.functional.layer_norm(x + a @ g("out_proj_w").T + g("out_proj_b"), (d,), g("ln1_w"), g("ln1_b"))
+            up = (x @ g("ffn_up_w").T + g("ffn_up_b")).relu()
+            x = torch.nn.functional.layer_norm(x + up @ g("ffn_down_w").T + g("ffn_down_b"), (d,), g("ln2_w"), g("ln2_b"))
+        return (x @ w["sampler.lm_head_w"].T).log_softmax(-1)
+
+    for prompt, kept in zip(prompts, found):
+        assert len(kept) == 3 and [c[0] for c in kept] == sorted((c[0] for c in kept), reverse=True)
+        for mean, drawn in kept:
+            assert 1 <= len(drawn) <= 9 and (len(drawn) == 9 or drawn[-1] == candidates.EOS)
+            lp = scores(prompt + drawn)[len(prompt) - 1:-1].gather(1, torch.tensor(drawn)[:, None])
+            assert abs(mean - lp.mean().item()) <= 2.0 ** -8, (mean, lp)
