@@ -25,6 +25,9 @@ constexpr int kTileRows = 16;        // rows of a warp's tile (the m of mma.m16n
 constexpr int kWarpsPerPlace = 3;    // warps of a launch for each one that the device holds at a time, where items are many
 constexpr int kLongItem = 256;       // keys: shorter items of several K/V heads share a warp; 2048 sequences with 20 positions each of
                                      // their own take 87 us so and 93 without, with 100 each 116 and 123
+constexpr int kShortItem = 1024;     // keys: up to which, on average, items that are more than the warps that the device holds take the tiles for short
+                                     // ones (see TileShape).  256 sequences over one prompt, 8 heads of 128, 500 positions each of
+                                     // their own: 126 us with them, 134 without; 64 sequences of 9000, 8 heads of 64: 162, 134
 constexpr int kMinChunk = 2;         // pages of a split at least
 constexpr int kSplitCost = 4, kJoinCost = 4;   // in pages: what a split costs beside its pages, and joining parts
 constexpr int kTcMinRowDims = 2049;  // rows x head dim of a node from which the tcgen05 kernel takes it (see build_items)
@@ -78,13 +81,20 @@ k_write_rows(const Token* __restrict__ rows_of, int rows, const uint4* __restric
 
 // Tiles of a head dimension: keys per stage of a warp's ring, its stages, the warps of an SM that this leaves
 // room for, and the warps of a CTA that shares out one item.  Measured as (keys, stages, warps), in us:
-//   dim 32   2048 sequences, 32 to a prompt, 500 positions each of their own: (32, 3, 16) 349, (32, 4, 13) 352, (64, 3, 9) 363, (64, 2, 13) 386
-//   dim 64   64 sequences of 8000, 8 heads:  (32, 3, 9) 149, (16, 4, 13) 157, (16, 6, 9) 159, (32, 2, 13) 171, (64, 2, 6) 172
-//   dim 128  64 sequences of 4000, 8 heads:  (32, 3, 4) 141, (16, 4, 7) 143, (16, 3, 8) 148, (16, 6, 4) 154, (32, 2, 6) 173
-// Two stages in flight keep the copies going; beyond that fewer warps are left than the softmax needs.
+//   dim 32   2048 sequences, 32 to a prompt, 500 positions each of their own: (32, 3, 16) 342, (32, 4, 13) 352, (64, 3, 9) 363,
+//            (64, 2, 13) 386, (16, 4, 20) 340;  100 positions: (32, 3, 16) 115, (16, 4, 20) 116, (16, 6, 16) 123;
+//            20 positions: 87, 80, 92
+//   dim 64   64 sequences of 8000, 8 heads:  (32, 3, 9) 134, (16, 3, 13) 140, (16, 4, 13) 140, (16, 5, 10) 136
+//            512 sequences, 32 to a prompt, 20 positions each of their own: 40, 36, 38, 40;  100: 51, 48, 48, 50
+//   dim 128  64 sequences of 4000, 8 heads:  (32, 3, 4) 138, (16, 3, 8) 148, (16, 4, 7) 151, (16, 5, 5) 137
+//            1024 sequences, 128 to a prompt, 50 positions each of their own: 138, 109, 116, 123
+// Long items want their copies far ahead, short ones many warps: an item's start is a chain of waits (item, token, page, keys).
 template <int D>
+constexpr int kTeam = D == 128 ? 4 : 8;
+template <int D, bool SHORT>
 struct TileShape {
-    static constexpr int KEYS = 32, STAGES = 3, RESIDENT = D == 32 ? 16 : D == 64 ? 9 : 4, TEAM = D == 128 ? 4 : 8;
+    static constexpr int KEYS = SHORT ? 16 : 32, STAGES = SHORT && D == 32 ? 4 : 3;
+    static constexpr int RESIDENT = SHORT ? (D == 32 ? 20 : D == 64 ? 13 : 8) : D == 32 ? 16 : D == 64 ? 9 : 4;
     static constexpr int HALF = KEYS * D * 2;   // bytes of a stage's K (or V)
     static constexpr int RING = STAGES * 2 * HALF;
     static_assert(RING >= kTileRows * D * 4, "a warp's results take the place of its ring");
@@ -108,10 +118,10 @@ __device__ __forceinline__ uint32_t tile_at(int row, int c) {
 // Warps alone (no CTA-wide barrier in the loop) because items differ in length; mma.sync because a page of a few
 // rows is a memory-bound product, whatever the tensor cores' rate.  A small step runs the W > 1 form as its only
 // launch: 6.9 us for four candidates of one prompt.
-template <typename T, int D, int W>
-__global__ void __launch_bounds__(32 * W, W == 1 ? TileShape<D>::RESIDENT : 1)
+template <typename T, int D, int W, bool SHORT>
+__global__ void __launch_bounds__(32 * W, W == 1 ? TileShape<D, SHORT>::RESIDENT : 1)
 k_attend_tiles(PlanView pv, Tensors<T> x, int item0, int heads_per, int folds) {
-    using S = TileShape<D>;
+    using S = TileShape<D, SHORT>;
     constexpr int NT = S::KEYS / 8, DT = D / 8, KS = D / 16;   // key tiles, dim tiles, steps along the dims
     extern __shared__ __align__(1024) unsigned char ring[];
     const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5;
@@ -519,7 +529,7 @@ struct Node {
 };
 
 int resident_warps(int dim) {
-    return dim == 32 ? TileShape<32>::RESIDENT : dim == 64 ? TileShape<64>::RESIDENT : TileShape<128>::RESIDENT;
+    return dim == 32 ? TileShape<32, false>::RESIDENT : dim == 64 ? TileShape<64, false>::RESIDENT : TileShape<128, false>::RESIDENT;
 }
 
 int sm_count(int device) {
@@ -899,23 +909,30 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
 template <typename T, int D>
 static cudaError_t launch_attend(t2sx_plan* a, Tensors<T> x, int layer, cudaStream_t st) {
     const PlanView& w = a->view;
-    using S = TileShape<D>;
+    using S = TileShape<D, false>;
+    using Short = TileShape<D, true>;
     static std::once_flag once[64];
     std::call_once(once[a->pool->device & 63], [] {
-        cudaFuncSetAttribute(k_attend_tiles<T, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::RING);
-        cudaFuncSetAttribute(k_attend_tiles<T, D, S::TEAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TEAM * S::RING);
+        cudaFuncSetAttribute(k_attend_tiles<T, D, 1, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::RING);
+        cudaFuncSetAttribute(k_attend_tiles<T, D, 1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Short::RING);
+        cudaFuncSetAttribute(k_attend_tiles<T, D, kTeam<D>, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTeam<D> * S::RING);
     });
     if (a->small)
-        return launch(k_attend_tiles<T, D, S::TEAM>, dim3((unsigned)w.n_own * w.n_kv), 32 * S::TEAM, S::TEAM * S::RING, st, false, w, x, 0, 1, 1);
+        return launch(k_attend_tiles<T, D, kTeam<D>, false>, dim3((unsigned)w.n_own * w.n_kv), 32 * kTeam<D>, kTeam<D> * S::RING, st, false, w, x, 0, 1, 1);
+    // One choice for both launches: between kernels of different shares of shared memory an SM has to run empty (2048
+    // sequences of 500 positions take 350 us with one launch of each kind, 340 with two of either).
+    const int64_t n_items = w.n_shared + w.n_own;
+    const bool is_short = n_items * w.n_kv > (int64_t)a->n_sm * S::RESIDENT && a->launch_keys[0] + a->launch_keys[1] <= n_items * kShortItem;
     auto tiles = [&](int which, bool early) {   // 0: pages of several sequences, 1: the others
         const int n = which ? w.n_own : w.n_shared;
         if (!n) return cudaSuccess;
         // Short items (below kLongItem keys, on average) share a warp, as many heads as leave several warps for each place:
         // a long one hides its own start.
-        const int64_t places = (int64_t)a->n_sm * S::RESIDENT, keys = a->launch_keys[which] / n;
+        const int64_t keys = a->launch_keys[which] / n;
+        const int64_t places = (int64_t)a->n_sm * (is_short ? Short::RESIDENT : S::RESIDENT);
         const int64_t heads = std::min<int64_t>({(int64_t)w.n_kv, (int64_t)n * w.n_kv / (places * kWarpsPerPlace) + 1, kLongItem / (keys + 1) + 1});
-        return launch(k_attend_tiles<T, D, 1>, dim3((unsigned)(n * ((w.n_kv + heads - 1) / heads))), 32, S::RING, st, early, w, x,
-                      w.n_tc + (which ? w.n_shared : 0), (int)heads, which ? (int)a->folds : 0);
+        return launch(is_short ? k_attend_tiles<T, D, 1, true> : k_attend_tiles<T, D, 1, false>, dim3((unsigned)(n * ((w.n_kv + heads - 1) / heads))), 32,
+                      is_short ? Short::RING : S::RING, st, early, w, x, w.n_tc + (which ? w.n_shared : 0), (int)heads, which ? (int)a->folds : 0);
     };
     cudaError_t e = cudaSuccess;
     bool early = false;   // a launch of this call comes before
