@@ -29,7 +29,7 @@ constexpr int kShortItem = 1024;     // keys: up to which, on average, items tha
                                      // ones (see TileShape).  256 sequences over one prompt, 8 heads of 128, 500 positions each of
                                      // their own: 126 us with them, 134 without; 64 sequences of 9000, 8 heads of 64: 162, 134
 constexpr int kMinChunk = 2;         // pages of a split at least
-constexpr int kSplitCost = 4, kJoinCost = 4;   // in pages: what a split costs beside its pages, and joining parts
+constexpr int kSplitCost = 4, kTcSplitCost = 8, kJoinCost = 4;   // in pages: what a split costs beside its pages, and joining parts
 constexpr int kTcMinRowDims = 2049;  // rows x head dim of a node from which the tcgen05 kernel takes it (see build_items)
 constexpr int kTcMinChunk = 4;       // pages of a split of such a node at least
 constexpr int kFoldParts = 4;        // parts of a token up to which the item of its own pages folds them in, one after the other:
@@ -699,24 +699,29 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
 static int64_t best_chunk(const t2sx_plan* a, bool tc, int64_t slots) {
     const int group = a->n_heads / a->pool->n_kv, tile = tc ? kTcRows : kTileRows;
     const int64_t least = tc ? kTcMinChunk : kMinChunk;
-    int64_t longest = 0;
-    for (const Node& nd : a->nodes)
+    int64_t longest = 0, tc_nodes = 0;
+    for (const Node& nd : a->nodes) {
         if (nd.tc == tc) longest = std::max<int64_t>(longest, nd.n_pages);
+        tc_nodes += nd.tc;
+    }
     int64_t best = std::max<int64_t>(longest, 1);
     double best_cost = 1e300;
     for (int64_t parts = 1; parts <= 512 && (parts == 1 || (longest + parts - 1) / parts >= least); parts += parts < 32 ? 1 : parts / 16) {
         int64_t chunk = (longest + parts - 1) / parts;
         if (tc) chunk += chunk & 1;   // it takes two pages at a time
-        int64_t items = 0, pages = 0;
+        int64_t items = 0, few = 0;
+        double pages = 0;
         for (const Node& nd : a->nodes) {
             if (nd.tc != tc) continue;
-            const int64_t tiles = (nd.n_tokens * (int64_t)group + tile - 1) / tile * a->pool->n_kv;
+            const int64_t rows = nd.n_tokens * (int64_t)group, tiles = (rows + tile - 1) / tile * a->pool->n_kv;
             items += tiles * ((nd.n_pages + chunk - 1) / chunk);
-            pages += tiles * nd.n_pages;
+            pages += tiles * nd.n_pages * (tc && rows <= kTcRows / 2 ? 0.5 : 1.0);   // its tiles share the pages out
+            few += rows <= kTcRows / 2;
         }
-        const double waves = (double)((items + slots - 1) / slots) * (chunk + kSplitCost);
-        const double even = (double)(pages + items * kSplitCost) / slots + (items > slots ? chunk : 0);
-        const double cost = std::min(waves, std::max(even, (double)(chunk + kSplitCost))) + (parts > 1 ? kJoinCost : 0);
+        const double split = tc ? kTcSplitCost : kSplitCost, longest_item = tc && few == tc_nodes ? chunk * 0.5 : chunk;
+        const double waves = (double)((items + slots - 1) / slots) * (longest_item + split);
+        const double even = (pages + items * split) / slots + (items > slots ? longest_item : 0);
+        const double cost = std::min(waves, std::max(even, longest_item + split)) + (parts > 1 ? kJoinCost : 0);
         if (cost < best_cost) { best_cost = cost; best = chunk; }
     }
     return best;

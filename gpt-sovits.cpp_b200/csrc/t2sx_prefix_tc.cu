@@ -40,6 +40,7 @@ constexpr int kKeys = kPoolPage;      // keys of a tile
 constexpr int kTileM = kTcRows / 2;   // rows of a tile
 constexpr int kSoftWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kThreads = 352;   // one MMA warp per tile
 constexpr int kTileCols = 256, kTmemCols = 2 * kTileCols, kOutCol = 2 * kKeys;
+constexpr int kAhead = 4;   // pages that a CTA asks for at its start, no more than the rings hold
 // A tile's weights against the reference maximum add up to less than this, or the reference is moved: f16 ends at
 // 2^16, and 64 weights at the reference itself make 2^13.
 constexpr float kSumLimit = 32768.0f;
@@ -50,6 +51,7 @@ struct TcShape {
     // of its barriers (a wait by parity does not tell a phase from the one before the last)
     static constexpr int STAGES = D == 128 ? 4 : 8;
     static_assert(STAGES % 2 == 0, "see above");
+    static_assert(STAGES >= kAhead, "the first pages wait for no stage");
     static constexpr int PITCH = D == 32 ? 64 : 128;               // bytes of a row of a swizzled block
     static constexpr int HALVES = D == 128 ? 2 : 1;                // blocks of 64 dims
     static constexpr int TILE = kKeys * D * 2, Q = kTileM * D * 2;
@@ -200,7 +202,7 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     auto tile_pages = [&](int tile) { return alternate ? (n - tile + 1) / 2 : n; };
     auto tile_rows = [&](int tile) { return alternate ? it.rows : min(kTileM, it.rows - tile * kTileM); };
     auto nth = [&](int tile, int k) { return alternate ? 2 * k + tile : k; };
-    if (tid == 0) {
+    if (warp == kTmaWarp && lane == 0) {
         const int users = alternate ? 1 : 2;   // tiles that read a page
         for (int s = 0; s < NS; ++s) { bar_init(k_full(s), 1); bar_init(k_empty(s), users); bar_init(v_full(s), 1); bar_init(v_empty(s), users); }
         for (int tile = 0; tile < 2; ++tile) {
@@ -213,6 +215,7 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         bar_init(zero_bar, 31);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        fence_proxy_async_smem();
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(tmem_holder)), "r"(kTmemCols) : "memory");
@@ -227,6 +230,26 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     const int head = kvh * group + g;
     dependents_wait();     // the step's own keys and values
     dependents_launch();   // not before: the launch after this one reads them, too
+    auto load_k = [&](int j, int z) {
+        const int s = j % NS;
+        bar_expect_tx(k_full(s), S::TILE);
+        for (int h = 0; h < S::HALVES; ++h) tma_load_3d(sk + s * S::TILE + h * (kKeys * 128), &map_k, h * 64, kvh * kKeys, z, k_full(s));
+    };
+    auto load_v = [&](int j, int z) {
+        const int s = j % NS;
+        bar_expect_tx(v_full(s), S::TILE);
+        for (int h = 0; h < S::HALVES; ++h) tma_load_3d(sv + s * S::TILE + h * (kKeys * 128), &map_v, h * 64, kvh * kKeys, z, v_full(s));
+    };
+    const int ahead = min(n, kAhead);
+    int page = 0;
+    if (warp == kTmaWarp) {   // the first pages come while the others fetch Q
+        page = lane < n ? pv.pages[it.pages_at + lane] : 0;
+        for (int j = 0; j < ahead; ++j) {
+            const int z = layer_page + __shfl_sync(~0u, page, j);
+            if (lane == 0) { load_k(j, z); load_v(j, z); }
+        }
+        __syncwarp();
+    }
     if (warp < kSoftWarps && !(alternate && tile == 1)) {
         // a warp's 32 rows, neighbouring lanes on neighbouring 16-byte words of a row
         constexpr int W = D / 8, R = 32 / W;
@@ -259,7 +282,7 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     bool gone = false;
     if (warp == kTmaWarp) {
         // ---- copies ----
-        int page = 0, j = 0;
+        int j = ahead;
         for (; j < n; ++j) {
             if ((j & 31) == 0) page = j + lane < n ? pv.pages[it.pages_at + j + lane] : 0;
             const int z = layer_page + __shfl_sync(~0u, page, j & 31), s = j % NS;
@@ -268,15 +291,10 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
                 const uint32_t phase = ((j / NS) & 1) ^ 1;
                 ok = bar_wait(k_empty(s), phase, abort_flag, spin);
                 if (ok) {
-                    bar_expect_tx(k_full(s), S::TILE);
-                    for (int h = 0; h < S::HALVES; ++h) tma_load_3d(sk + s * S::TILE + h * (kKeys * 128), &map_k, h * 64, kvh * kKeys, z, k_full(s));
+                    load_k(j, z);
                     ok = bar_wait(v_empty(s), phase, abort_flag, spin);
-                    if (ok) {
-                        bar_expect_tx(v_full(s), S::TILE);
-                        for (int h = 0; h < S::HALVES; ++h) tma_load_3d(sv + s * S::TILE + h * (kKeys * 128), &map_v, h * 64, kvh * kKeys, z, v_full(s));
-                    } else {
-                        ok = 2;   // K of this page is under way
-                    }
+                    if (ok) load_v(j, z);
+                    else ok = 2;   // K of this page is under way
                 }
             }
             ok = __shfl_sync(~0u, ok, 0);
