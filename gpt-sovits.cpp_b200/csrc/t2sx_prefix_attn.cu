@@ -30,11 +30,11 @@ constexpr int kShortItem = 1024;     // keys: up to which, on average, items tha
                                      // their own: 126 us with them, 134 without; 64 sequences of 9000, 8 heads of 64: 162, 134
 constexpr int kMinChunk = 2;         // pages of a split at least
 constexpr int kSplitCost = 4, kTcSplitCost = 8, kJoinCost = 4;   // in pages: what a split costs beside its pages, and joining parts
-constexpr int kTcMinRowDims = 2049;  // rows x head dim of a node from which the tcgen05 kernel takes it (see build_items)
+constexpr double kClear = 1.5;       // a node's costs with one kernel and the other differ clearly (see choose_kernels)
 constexpr int kTcMinChunk = 4;       // pages of a split of such a node at least
 constexpr int kFoldParts = 4;        // parts of a token up to which the item of its own pages folds them in, one after the other:
                                      // 2048 sequences, 32 to a prompt, take 340 us so and 351 with a launch that joins them; with up
-                                     // to eight parts 256 sequences of one long prompt take 117 instead of 107
+                                     // to eight parts 256 sequences of one long prompt took 117 when they took 107 so
 constexpr int kSmallWork = 2048;     // pages x head dim of a CTA of a small step at most, an eighth of it with two CTAs to an SM
 
 __device__ __forceinline__ void mma16816(__half, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -420,7 +420,7 @@ k_attend_tiles(PlanView pv, Tensors<T> x, int item0, int heads_per, int folds) {
 // Joining the parts: out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.  Bound by the parts' bytes, which the launch before
 // has just left in the L2 cache, and by latency.
 //
-// Four warps, each with a (token, query head) of few parts (at most 32; 256 sequences of one long prompt take 107 us so and
+// Four warps, each with a (token, query head) of few parts (at most 32; 256 sequences of one long prompt took 107 us so and
 // 113 with a CTA for each of their rows): the lanes are D / 4 columns of four dims x 32 / (D / 4) parts.
 template <typename T, int D>
 __global__ void __launch_bounds__(128)
@@ -693,6 +693,37 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
     }
 }
 
+// The kernels of the nodes, by cost.  In pages of the tcgen05 kernel's two tiles, an SM's time: such a CTA costs its start and end and
+// its pages (half as much each where its two tiles share them out); a warp tile of 16 rows costs a share of that for each of its pages
+// and for kSplitCost more.  In us, with the tcgen05 kernel and without:
+//   heads of 128: 16 prompts of 4032 with 16 rows 63, 56; with 24 61, 77;   32 prompts of 500 with 32 rows 45, 46;
+//   heads of 64:  16 of 4032 with 24 rows 38, 44;   32 of 1000 with 32 rows and 250 positions each of their own 56, 49;
+//                 32 of 500 with 64 rows 37, 40;    32 of 3000 with 64 rows 64, 105
+//   heads of 32:  16 of 4032 with 48 rows 23, 25, with 64 23, 30;   40 of 350 with 48 rows, 16 K/V heads, 105, 88
+// Nodes that are near the balance (up to kClear of it) go all one way, by their sum: launches of both kinds cost more than
+// the better choice gains (8 prompts of 1500 with 24 rows, heads of 64: 17 with, 19 without, 26 with some of each).
+static void choose_kernels(t2sx_plan* a) {
+    const int group = a->n_heads / a->pool->n_kv, dim = a->pool->dim;
+    const double share = dim == 128 ? 0.7 : dim == 64 ? 0.4 : 0.28;
+    auto costs = [&](const Node& nd) {   // warp tiles, tcgen05
+        const int64_t rows = (int64_t)nd.n_tokens * group, items = (rows + kTcRows - 1) / kTcRows, tiles = (rows + kTileRows - 1) / kTileRows;
+        return std::make_pair(tiles * share * (nd.n_pages + kSplitCost), items * kTcSplitCost + nd.n_pages * (rows <= kTcRows / 2 ? 0.5 : items));
+    };
+    double warp = 0, tc = 0;
+    for (Node& nd : a->nodes) {
+        nd.tc = !a->small && (int64_t)nd.n_tokens * group > kTileRows;
+        if (!nd.tc) continue;
+        const auto c = costs(nd);
+        warp += c.first;
+        tc += c.second;
+    }
+    for (Node& nd : a->nodes) {
+        if (!nd.tc) continue;
+        const auto c = costs(nd);
+        nd.tc = c.first > kClear * c.second || (c.first * kClear > c.second && warp > tc);
+    }
+}
+
 // Pages of a split, for the nodes of one kind: of the even divisions of the longest node, the one that ends first,
 // where a split costs its pages and as much again as kSplitCost of them, `slots` of them run at a time, and
 // they start the longest first.
@@ -733,11 +764,7 @@ static int64_t best_chunk(const t2sx_plan* a, bool tc, int64_t slots) {
 static int64_t build_items(t2sx_plan* a) {
     const int group = a->n_heads / a->pool->n_kv, n_kv = a->pool->n_kv;
     a->items.clear(); a->joins.clear();
-    // The tcgen05 kernel reads a page once for up to 256 rows, a warp tile for 16, but a page of few rows costs the former
-    // as much as one of many: 20 and 32 rows of one 32768-position prompt with 8 K/V heads took 46 and 50 us with it and
-    // 55 and 56 without at head dim 128; at 64, 16 prompts of 4032 with 32 and 48 rows took 54 and 45 with, 47 and 60
-    // without; at 32, with 48 and 64 rows, 30 and 31 with, 25 and 31 without.
-    for (Node& nd : a->nodes) nd.tc = !a->small && (int64_t)nd.n_tokens * group * a->pool->dim >= kTcMinRowDims;
+    choose_kernels(a);
     const int64_t warp_chunk = a->small ? INT32_MAX : best_chunk(a, false, (int64_t)a->n_sm * resident_warps(a->pool->dim));
     const int64_t tc_chunk = best_chunk(a, true, a->n_sm);
     a->tokens.resize(a->node_rows.size());

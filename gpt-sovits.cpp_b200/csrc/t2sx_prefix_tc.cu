@@ -17,7 +17,8 @@
 // the K index), so a page costs the two tiles 2 x (8 x 64 + 4 x 64) = 1536 cycles at head dim 128, and the loop takes
 // 1526.  At head dim 64 the MMAs take 1024, the exponentials (8 cycles to a warp's instruction) 1066, and the loop
 // 1555.  A step of 256 sequences over one prompt of 16384 positions (32 heads, 8 K/V heads of 128 dims, bf16; up to 256
-// positions each of their own) takes 107 us with all its launches, some 65 of them here.  When it took 116, it took with
+// positions each of their own) takes 94 us with all its launches, some 70 of them here: 60 in the loop, 10 in a CTA's start
+// and end.  When it took 116, it took with
 //   scores of 128 keys in one buffer (N 128): 135, and 128 with 16 softmax warps, since the MMAs then wait for the
 //              softmax; there is no TMEM for a second buffer of that size beside two outputs;
 //   one tile per CTA, two CTAs per SM: 153;    16 softmax warps on these buffers: 117;
