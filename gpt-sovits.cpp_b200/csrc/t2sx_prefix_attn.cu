@@ -25,9 +25,10 @@ constexpr int kTileRows = 16;        // rows of a warp's tile (the m of mma.m16n
 constexpr int kWarpsPerPlace = 3;    // warps of a launch for each one that the device holds at a time, where items are many
 constexpr int kLongItem = 256;       // keys: shorter items of several K/V heads share a warp; 2048 sequences with 20 positions each of
                                      // their own take 87 us so and 93 without, with 100 each 116 and 123
-constexpr int kShortItem = 1024;     // keys: up to which, on average, items that are more than the warps that the device holds take the tiles for short
-                                     // ones (see TileShape).  256 sequences over one prompt, 8 heads of 128, 500 positions each of
-                                     // their own: 126 us with them, 134 without; 64 sequences of 9000, 8 heads of 64: 162, 134
+constexpr int kShortItem = 8;        // keys per head dim: up to which, on average, items that are more than the warps that the device
+                                     // holds take the tiles for short ones (see TileShape).  256 sequences over one prompt, 8 heads of
+                                     // 128, 500 positions each of their own: 126 us with them, 134 without; 64 sequences of 9000, 8
+                                     // heads of 64: 162, 134; 2048 sequences of 500, 16 heads of 32, from cold caches: 374, 365
 constexpr int kMinChunk = 2;         // pages of a split at least
 constexpr int kSplitCost = 4, kTcSplitCost = 8, kJoinCost = 4;   // in pages: what a split costs beside its pages, and joining parts
 constexpr double kClear = 1.5;       // a node's costs with one kernel and the other differ clearly (see choose_kernels)
@@ -954,7 +955,7 @@ static cudaError_t launch_attend(t2sx_plan* a, Tensors<T> x, int layer, cudaStre
     // One choice for both launches: between kernels of different shares of shared memory an SM has to run empty (2048
     // sequences of 500 positions take 350 us with one launch of each kind, 340 with two of either).
     const int64_t n_items = w.n_shared + w.n_own;
-    const bool is_short = n_items * w.n_kv > (int64_t)a->n_sm * S::RESIDENT && a->launch_keys[0] + a->launch_keys[1] <= n_items * kShortItem;
+    const bool is_short = n_items * w.n_kv > (int64_t)a->n_sm * S::RESIDENT && a->launch_keys[0] + a->launch_keys[1] <= n_items * kShortItem * D;
     auto tiles = [&](int which, bool early) {   // 0: pages of several sequences, 1: the others
         const int n = which ? w.n_own : w.n_shared;
         if (!n) return cudaSuccess;
