@@ -3,7 +3,8 @@
 // A sequence is a list of page ids kept on the host; a page counts its users.  Forking shares full
 // pages by counting and copies the filled positions of the last, partial one, so pages with several
 // users are never written.  Data moves only in k_move_pages: a fork's partial pages, a copy's pages,
-// a compaction's pages; the sources of one launch are never among its destinations.
+// a compaction's pages; the sources of one launch are never among its destinations (a fork or copy
+// whose source is also one of its destinations is refused, a compaction moves pages across a line).
 #include "t2sx_pool.cuh"
 
 #include <algorithm>
@@ -115,6 +116,12 @@ int derive(t2sx_pool* p, int32_t n, const int32_t* srcs, const int32_t* dsts, cu
             const int64_t len = p->len[srcs[i]];
             need += share ? (len % kPoolPage != 0) : pages_of(len);
         }
+        // a source that this call fills would be copied while it is written, and its pages are not in `need`
+        bool both = false;
+        for (int32_t i = 0; i < n; ++i) p->mark[dsts[i]] = 1;
+        for (int32_t i = 0; i < n; ++i) both |= p->mark[srcs[i]] != 0;
+        for (int32_t i = 0; i < n; ++i) p->mark[dsts[i]] = 0;
+        if (both) return bad("pool fork/copy: a source is also a destination of the call");
         if (need > p->n_free) return t2sx_set_error(T2SX_ERR_OOM, "pool fork/copy: not enough free pages");
         // everything that can fail on the host is allocated before the state changes
         p->moves.clear();

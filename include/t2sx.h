@@ -282,8 +282,9 @@ T2SX_API int t2sx_pool_table(t2sx_pool* p, int32_t n, const int32_t* seqs, int32
 /* counts[i] (>= 0) positions more for sequence seqs[i] (distinct), in order; their values are
  * undefined until written.  T2SX_ERR_OOM if the pool has not enough pages. */
 T2SX_API int t2sx_pool_extend(t2sx_pool* p, int32_t n, const int32_t* seqs, const int64_t* counts);
-/* dsts[i] (empty, distinct; T2SX_ERR_STATE otherwise) becomes a continuation of srcs[i]: it
- * shares the full pages and gets its own copy of the filled positions of a partial last one. */
+/* dsts[i] (distinct; T2SX_ERR_STATE if one is not empty) becomes a continuation of srcs[i]: it
+ * shares the full pages and gets its own copy of the filled positions of a partial last one.  A
+ * source may serve several destinations, but is none itself (T2SX_ERR_INVALID). */
 T2SX_API int t2sx_pool_fork(t2sx_pool* p, int32_t n, const int32_t* srcs, const int32_t* dsts, void* stream);
 /* As fork, but sharing nothing: dsts[i] gets pages of its own for all positions. */
 T2SX_API int t2sx_pool_copy(t2sx_pool* p, int32_t n, const int32_t* srcs, const int32_t* dsts, void* stream);

@@ -1,0 +1,92 @@
+"""The host side of the candidate operators (page lists, plans, launch shapes, the order of device work) on a fake
+CUDA runtime: nothing here needs or touches a GPU."""
+import ctypes as C
+import os
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SOURCES = ("t2sx_pool.cu", "t2sx_prefix_attn.cu", "t2sx_prefix_tc.cu", "t2sx_logprobs.cu")
+K_STORE, V_STORE, Q = 1 << 20, 1 << 21, 1 << 22   # addresses: nothing reads what stands there
+
+
+@pytest.fixture(scope="module")
+def fake_lib(tmp_path_factory):
+    import build
+    import t2sx
+    tmp = tmp_path_factory.mktemp("fake_cuda")
+    jobs = []
+    for name in SOURCES:
+        cmd = [build.nvcc(), *build.NVCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-c", os.path.join(build.CSRC, name), "-o", str(tmp / (name + ".o"))]
+        jobs.append((name, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    for name, job in jobs:
+        out = job.communicate()[0]
+        assert job.returncode == 0, (name, out)
+    gxx = shutil.which("g++")
+    assert gxx, "g++ is required"
+    so = str(tmp / "libfake.so")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(build.nvcc()))), "include")
+    r = subprocess.run([gxx, "-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden", "-Wl,-Bsymbolic", "-I", cuda, os.path.join(ROOT, "tests", "cpp", "fake_cuda.cpp"),
+                        *[str(tmp / (n + ".o")) for n in SOURCES], "-o", so], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    lib = C.CDLL(so)
+    for name, (res, args) in t2sx.SIGNATURES.items():
+        if name.startswith(("t2sx_pool_", "t2sx_plan_")) or name in ("t2sx_token_logprobs", "t2sx_last_error"):
+            getattr(lib, name).restype, getattr(lib, name).argtypes = res, args
+    for name in ("fake_launches", "fake_grid_x", "fake_synced", "fake_recorded"):
+        getattr(lib, name).restype = C.c_longlong
+    lib.fake_recorded.argtypes, lib.fake_fail_launch.argtypes = [C.c_void_p], [C.c_longlong]
+    return lib
+
+
+@pytest.fixture
+def host(fake_lib, monkeypatch):
+    """The binding on the fake runtime."""
+    import t2sx
+    monkeypatch.setattr(t2sx, "_lib", fake_lib)
+    fake_lib.fake_reset()
+    yield t2sx
+    while OPEN:   # while the binding still has the library that they come from
+        OPEN.pop().close()
+
+
+OPEN = []
+
+
+def _pool(t2sx, pages, seqs, dim=32, kv=1, layers=1):
+    OPEN.append(t2sx.PagePool(t2sx.F16, layers, pages, kv, dim, seqs, K_STORE, V_STORE))
+    return OPEN[-1]
+
+
+def _state(pool):
+    return pool.available(), [pool.length(s) for s in range(pool.max_seqs)], [pool.table([s]).tolist() for s in range(pool.max_seqs)]
+
+
+def _refused(t2sx, code, call):
+    with pytest.raises(t2sx.T2SXError) as e:
+        call()
+    assert e.value.code == code, e.value
+
+
+@pytest.mark.parametrize("op", ["fork", "copy"])
+def test_source_among_the_destinations(host, fake_lib, op):
+    """A sequence that a call fills is not a source of that call: its pages would be copied while they are
+    written, and they are not counted.  Refused before anything changes, whatever the order of the pairs."""
+    pool = _pool(host, pages=40, seqs=6)
+    pool.extend([0], [70])
+    derive = getattr(pool, op)
+    before = _state(pool)
+    for srcs, dsts in (([0, 1], [1, 2]), ([1, 0], [2, 1]), ([0, 1, 2], [1, 2, 3]), ([0, 3, 1], [1, 2, 3]), ([4], [4])):
+        _refused(host, host.ERR_INVALID, lambda: derive(srcs, dsts))
+        assert _state(pool) == before and fake_lib.fake_launches() == 0
+    # as many pages as one copy needs: the second one's were taken from beyond the list of free pages
+    small = _pool(host, pages=3 if op == "fork" else 4, seqs=4)
+    small.extend([0], [70])
+    before = _state(small)
+    _refused(host, host.ERR_INVALID, lambda: getattr(small, op)([0, 1], [1, 2]))
+    assert _state(small) == before
+    # ids of the refused calls are free for others; the same source for several is no such case
+    derive([0, 0, 5], [1, 2, 3])
+    assert [pool.length(s) for s in range(6)] == [70, 70, 70, 0, 0, 0]
