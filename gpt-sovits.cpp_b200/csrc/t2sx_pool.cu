@@ -127,6 +127,7 @@ int derive(t2sx_pool* p, int32_t n, const int32_t* srcs, const int32_t* dsts, cu
         p->moves.clear();
         p->moves.reserve((size_t)need);
         for (int32_t i = 0; i < n; ++i) p->table[dsts[i]].reserve(p->table[srcs[i]].size());
+        p->shares += share;
         for (int32_t i = 0; i < n; ++i) {
             const int64_t len = p->len[srcs[i]];
             const std::vector<int32_t>& from = p->table[srcs[i]];

@@ -36,6 +36,7 @@ struct t2sx_pool {
     size_t first_free_word = 0;                // no word before it has a free page
     int64_t n_free = 0;
     uint64_t version = 0;                      // changes when a page may have passed to another owner
+    uint64_t shares = 0;                       // changes when a page may have got another user
     std::vector<uint8_t> mark;                 // [max_seqs] scratch of the argument checks
     std::vector<t2sx::PageMove> moves;         // scratch of a call
     int n_plans = 0;

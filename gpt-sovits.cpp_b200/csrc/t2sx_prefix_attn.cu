@@ -550,6 +550,8 @@ struct t2sx_plan {
     CUtensorMap map_k, map_v;
     int32_t *err = nullptr, *err_dev = nullptr;   // pinned: what a kernel that gave up a wait reports
     uint64_t version = 0;          // of the pool at the update
+    uint64_t shares = 0;           // of the pool when shared_rows was found
+    std::vector<int32_t> row_pages;   // that the rows' own positions are in
     // host copy of what the device gets, in pinned memory: two buffers, so that an update need not
     // wait for the previous one's upload
     uint8_t* host[2] = {};
@@ -862,6 +864,7 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
         a->shared_rows = false;
         a->info.resize(rows);
         a->row0.resize(n);
+        a->row_pages.clear();
         int32_t r = 0;
         for (int32_t i = 0; i < n; ++i) {
             a->row0[i] = r;
@@ -869,6 +872,7 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
                 const int32_t limit = (int32_t)(p->len[seqs[i]] - n_new[i] + j + 1);
                 const int32_t page = p->table[seqs[i]][(limit - 1) / kPoolPage];
                 a->shared_rows |= p->users[page] > 1;
+                if (j == 0 || page != a->row_pages.back()) a->row_pages.push_back(page);
                 a->info[r] = Token{r, limit, page, 0, 0, 0, 0, 0};
             }
         }
@@ -934,6 +938,7 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
         w.part_o = (float*)a->work;
         w.part_ml = (float2*)(a->work + o_bytes);
         a->version = p->version;
+        a->shares = p->shares;
         a->ready = true;
         return T2SX_OK;
     });
@@ -1037,6 +1042,10 @@ extern "C" int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, 
         return bad("t2sx_plan_attend: strides must be multiples of 8 and no less than a row");
     if (((uintptr_t)q_dev | (uintptr_t)out_dev | (uintptr_t)k_new_dev | (uintptr_t)v_new_dev) & 15 || ((uintptr_t)lse_dev & 3))
         return bad("t2sx_plan_attend: tensors must be 16-byte aligned");
+    if (a->shares != p->shares) {   // forks since: full pages of the rows may be shared by now
+        for (int32_t page : a->row_pages) a->shared_rows |= p->users[page] > 1;
+        a->shares = p->shares;
+    }
     if (k_new_dev && a->shared_rows)
         return t2sx_set_error(T2SX_ERR_STATE, "t2sx_plan_attend: a row's position is in a page of several sequences, which is not written");
     if (int rc = plan_error(a)) return rc;

@@ -303,8 +303,8 @@ T2SX_API void t2sx_plan_free(t2sx_plan* a);
 /* The step's sequences (distinct) and their last n_new[i] (>= 0, <= length) positions: rows are
  * these positions in the order of the call.  Pages that sequences have in common from their
  * start on are found here, whatever the order.  The pool's later fork, copy and extend calls
- * leave a plan valid; after a release or a compact that moved pages attend gives T2SX_ERR_STATE
- * until the next update. */
+ * leave a plan valid (but what a fork has made a shared page is no longer written, see below); after
+ * a release or a compact that moved pages attend gives T2SX_ERR_STATE until the next update. */
 T2SX_API int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, const int32_t* n_new, void* stream);
 /* Row r with query head h, at position lim - 1 of its sequence:
  *     out = sum_{j < lim} softmax_j(scale * q . k_j) v_j,   lse = log sum_{j < lim} exp(scale * q . k_j)
@@ -312,7 +312,7 @@ T2SX_API int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, cons
  * elements apart (multiples of 8); lse_dev: f32 [rows][n_heads] or null.  With k_new_dev and
  * v_new_dev ([rows][n_kv_heads][head_dim], rows kv_stride elements apart) the rows' keys and
  * values are first written to the cache (T2SX_ERR_STATE if a row's position is in a page of several
- * sequences); null: they are there already.  All 16-byte aligned.
+ * sequences by then); null: they are there already.  All 16-byte aligned.
  * Cache positions below a sequence's length must hold finite values; beyond it anything may stand.
  * Products are accumulated, and maxima and sums held, in f32; the softmax weights are rounded to
  * the pool's type before they multiply v, as the tensor cores take them. */

@@ -90,3 +90,41 @@ def test_source_among_the_destinations(host, fake_lib, op):
     # ids of the refused calls are free for others; the same source for several is no such case
     derive([0, 0, 5], [1, 2, 3])
     assert [pool.length(s) for s in range(6)] == [70, 70, 70, 0, 0, 0]
+
+
+def _plan(pool, heads):
+    OPEN.append(pool.plan(heads))
+    return OPEN[-1]
+
+
+def _attend(plan, new=False, layer=0, stream=0):
+    plan.attend(layer, Q, Q, 1.0, k_new_ptr=Q if new else None, v_new_ptr=Q if new else None, stream=stream)
+
+
+def test_fork_between_update_and_attend(host, fake_lib):
+    """A fork that comes to share the page of a plan's row: the row's keys and values are not written there any
+    more; attending without writing them goes on, and so do rows in pages that are still their sequence's own."""
+    pool = _pool(host, pages=40, seqs=6)
+    pool.extend([0, 1], [64, 70])
+    plan, other = _plan(pool, 1), _plan(pool, 1)
+    plan.update([0, 1], [1, 1])
+    other.update([1], [1])
+    _attend(plan, new=True)
+    pool.fork([1], [2])   # shares the first page of 1; its row is in the second one
+    _attend(plan, new=True)
+    pool.fork([0], [3])
+    fake_lib.fake_reset()
+    for _ in range(2):
+        _refused(host, host.ERR_STATE, lambda: _attend(plan, new=True))
+    assert fake_lib.fake_launches() == 0
+    _attend(plan)
+    _attend(other, new=True)
+    # the row after that page is the sequence's own again
+    pool.extend([0], [1])
+    plan.update([0, 1], [1, 1])
+    _attend(plan, new=True)
+    plan.update([0, 1], [2, 1])
+    _refused(host, host.ERR_STATE, lambda: _attend(plan, new=True))
+    pool.release([3])
+    plan.update([0, 1], [2, 1])
+    _attend(plan, new=True)
