@@ -84,8 +84,8 @@ int launch_moves(t2sx_pool* p, const std::vector<PageMove>& moves, cudaStream_t 
         if (n <= kFewMoves) launch_list<kFewMoves>(p, moves.data() + at, n, st);
         else launch_list<kMovesPerLaunch>(p, moves.data() + at, n, st);
         POOL_CK(cudaGetLastError());
+        p->end(st);
     }
-    p->end(st);
     return T2SX_OK;
 }
 

@@ -60,8 +60,9 @@ struct t2sx_pool {
         if ((size_t)(p >> 6) < first_free_word) first_free_word = p >> 6;
         ++n_free;
     }
-    // Device work of a call goes between begin and end: work on another stream is waited for there.  The event is
-    // recorded when the stream changes, not after every call (which took a fifth of a small call's time on the host).
+    // Device work of a call comes after begin, which waits for work on another stream; end follows each piece that was queued,
+    // so that a call which fails halfway leaves a right `last`.  The event is recorded when the stream changes, not after
+    // every call (which took a fifth of a small call's time on the host).
     cudaError_t begin(cudaStream_t st) {
         if (!worked || st == last) return cudaSuccess;
         cudaError_t e = cudaEventRecord(done, last);

@@ -926,9 +926,11 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
         POOL_CK(grow(a->work, a->work_bytes, o_bytes + part_rows * 8));
         auto put = [&](size_t at, auto const& v) { if (!v.empty()) memcpy(a->host[b] + at, v.data(), v.size() * sizeof(v[0])); };
         put(o_info, a->info); put(o_items, a->items); put(o_tokens, a->tokens); put(o_pages, a->pages); put(o_joins, a->joins);
-        if (bytes) POOL_CK(cudaMemcpyAsync(a->dev, a->host[b], bytes, cudaMemcpyHostToDevice, st));
+        if (bytes) {
+            POOL_CK(cudaMemcpyAsync(a->dev, a->host[b], bytes, cudaMemcpyHostToDevice, st));
+            p->end(st);
+        }
         POOL_CK(cudaEventRecord(a->sent[b], st));
-        p->end(st);
         PlanView& w = a->view;
         w.rows_of = (const Token*)(a->dev + o_info);
         w.items = (const Item*)(a->dev + o_items);
@@ -955,8 +957,13 @@ static cudaError_t launch_attend(t2sx_plan* a, Tensors<T> x, int layer, cudaStre
         cudaFuncSetAttribute(k_attend_tiles<T, D, 1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Short::RING);
         cudaFuncSetAttribute(k_attend_tiles<T, D, kTeam<D>, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTeam<D> * S::RING);
     });
+    auto queued = [&](cudaError_t e) {   // a launch's status; what was queued before a failure is the pool's work, too
+        if (e == cudaSuccess) a->pool->end(st);
+        return e;
+    };
     if (a->small)
-        return launch(k_attend_tiles<T, D, kTeam<D>, false>, dim3((unsigned)w.n_own * w.n_kv), 32 * kTeam<D>, kTeam<D> * S::RING, st, false, w, x, 0, 1, 1);
+        return queued(launch(k_attend_tiles<T, D, kTeam<D>, false>, dim3((unsigned)w.n_own * w.n_kv), 32 * kTeam<D>, kTeam<D> * S::RING, st, false, w, x, 0,
+                             1, 1));
     // One choice for both launches: between kernels of different shares of shared memory an SM has to run empty (2048
     // sequences of 500 positions take 350 us with one launch of each kind, 340 with two of either).
     const int64_t n_items = w.n_shared + w.n_own;
@@ -969,8 +976,9 @@ static cudaError_t launch_attend(t2sx_plan* a, Tensors<T> x, int layer, cudaStre
         const int64_t keys = a->launch_keys[which] / n;
         const int64_t places = (int64_t)a->n_sm * (is_short ? Short::RESIDENT : S::RESIDENT);
         const int64_t heads = std::min<int64_t>({(int64_t)w.n_kv, (int64_t)n * w.n_kv / (places * kWarpsPerPlace) + 1, kLongItem / (keys + 1) + 1});
-        return launch(is_short ? k_attend_tiles<T, D, 1, true> : k_attend_tiles<T, D, 1, false>, dim3((unsigned)(n * ((w.n_kv + heads - 1) / heads))), 32,
-                      is_short ? Short::RING : S::RING, st, early, w, x, w.n_tc + (which ? w.n_shared : 0), (int)heads, which ? (int)a->folds : 0);
+        return queued(launch(is_short ? k_attend_tiles<T, D, 1, true> : k_attend_tiles<T, D, 1, false>, dim3((unsigned)(n * ((w.n_kv + heads - 1) / heads))),
+                             32, is_short ? Short::RING : S::RING, st, early, w, x, w.n_tc + (which ? w.n_shared : 0), (int)heads,
+                             which ? (int)a->folds : 0));
     };
     cudaError_t e = cudaSuccess;
     bool early = false;   // a launch of this call comes before
@@ -980,11 +988,11 @@ static cudaError_t launch_attend(t2sx_plan* a, Tensors<T> x, int layer, cudaStre
             const int64_t vecs = (int64_t)w.rows * w.n_kv * row_vec;
             k_write_rows<<<(unsigned)((vecs + 255) / 256), 256, 0, st>>>(w.rows_of, w.rows, (const uint4*)x.k_new, (const uint4*)x.v_new,
                                                                         x.kv_stride / 8, (uint4*)x.k, (uint4*)x.v, w.n_kv, row_vec);
-            e = cudaGetLastError();
+            e = queued(cudaGetLastError());
             x.k_new = x.v_new = nullptr;
             early = true;
         }
-        if (e == cudaSuccess) e = launch_tc(w, x, a->pool, a->map_k, a->map_v, layer * a->pool->n_pages, a->err_dev, early, st);
+        if (e == cudaSuccess) e = queued(launch_tc(w, x, a->pool, a->map_k, a->map_v, layer * a->pool->n_pages, a->err_dev, early, st));
         early = true;
     }
     if (e == cudaSuccess) e = tiles(0, early);
@@ -992,8 +1000,8 @@ static cudaError_t launch_attend(t2sx_plan* a, Tensors<T> x, int layer, cudaStre
     if (e == cudaSuccess) e = tiles(1, early);
     if (e == cudaSuccess && w.n_joins) {
         const int64_t rows = (int64_t)w.n_joins * a->n_heads;
-        e = a->most_parts <= 32 ? launch(k_join_few<T, D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, true, w, x)
-                                : launch(k_join_parts<T, D>, dim3((unsigned)rows), 128, 0, st, true, w, x);
+        e = queued(a->most_parts <= 32 ? launch(k_join_few<T, D>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, true, w, x)
+                                       : launch(k_join_parts<T, D>, dim3((unsigned)rows), 128, 0, st, true, w, x));
     }
     return e;
 }
@@ -1055,6 +1063,5 @@ extern "C" int t2sx_plan_attend(t2sx_plan* a, int32_t layer, const void* q_dev, 
     POOL_CK(p->begin(st));
     auto go = p->type == T2SX_TYPE_F16 ? attend<__half> : attend<__nv_bfloat16>;
     POOL_CK(go(a, layer, q_dev, q_stride, k_new_dev, v_new_dev, kv_stride, scale, out_dev, out_stride, lse_dev, st));
-    p->end(st);
     return T2SX_OK;
 }

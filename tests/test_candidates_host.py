@@ -128,3 +128,38 @@ def test_fork_between_update_and_attend(host, fake_lib):
     pool.release([3])
     plan.update([0, 1], [2, 1])
     _attend(plan, new=True)
+
+
+def test_failed_call_leaves_its_device_work_known(host, fake_lib):
+    """Where a later launch of a call fails, the earlier ones are the pool's last work: the next call on another stream
+    waits for them.  A call whose first launch fails leaves none."""
+    pool = _pool(host, pages=2000, seqs=900, kv=16)
+    pool.extend([0], [70])
+    fake_lib.fake_fail_launch(2)
+    _refused(host, host.ERR_CUDA, lambda: pool.fork([0] * 700, list(range(1, 701)), 11))   # two launches of 512 copies at most
+    pool.fork([0], [801], 12)
+    assert fake_lib.fake_recorded(11) == 1
+    fake_lib.fake_fail_launch(1)
+    _refused(host, host.ERR_CUDA, lambda: pool.fork([0], [802], 13))
+    pool.fork([0], [803], 12)
+    assert fake_lib.fake_recorded(13) == 0 and fake_lib.fake_recorded(12) == 1   # for the call on 13 that failed
+    pool.fork([0], [804], 14)
+    assert fake_lib.fake_recorded(12) == 2
+
+    shared = _pool(host, pages=600, seqs=130, kv=16)
+    shared.extend([0], [64])
+    shared.fork([0] * 128, list(range(1, 129)))
+    seqs = list(range(1, 129))
+    shared.extend(seqs, [1] * 128)
+    plan = _plan(shared, 16)
+    plan.update(seqs, [1] * 128, 21)
+    fake_lib.fake_reset()
+    _attend(plan, stream=21)
+    launches = fake_lib.fake_launches()
+    assert launches > 1
+    for nth in range(1, launches + 1):
+        fake_lib.fake_reset()
+        fake_lib.fake_fail_launch(nth)
+        _refused(host, host.ERR_CUDA, lambda: _attend(plan, stream=100 + nth))
+        _attend(plan, stream=200 + nth)
+        assert fake_lib.fake_recorded(100 + nth) == (nth > 1)
