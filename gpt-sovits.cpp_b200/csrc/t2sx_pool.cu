@@ -103,6 +103,12 @@ bool distinct(t2sx_pool* p, int32_t n, const int32_t* seqs) {
     return ok;
 }
 
+void clear(t2sx_pool* p, int32_t seq) {
+    for (int32_t page : p->table[seq]) p->drop(page);
+    p->table[seq].clear();
+    p->len[seq] = 0;
+}
+
 // fork (share: full pages are shared) and copy
 int derive(t2sx_pool* p, int32_t n, const int32_t* srcs, const int32_t* dsts, cudaStream_t st, bool share, const char* who) {
     if (!p || p->closed || n < 0 || (n > 0 && (!srcs || !dsts))) return bad("pool fork/copy: bad arguments");
@@ -142,7 +148,10 @@ int derive(t2sx_pool* p, int32_t n, const int32_t* srcs, const int32_t* dsts, cu
             }
             p->len[dsts[i]] = len;
         }
-        return launch_moves(p, p->moves, st);
+        const int rc = launch_moves(p, p->moves, st);
+        if (rc != T2SX_OK)   // what was copied by then stands in pages that are free again
+            for (int32_t i = 0; i < n; ++i) clear(p, dsts[i]);
+        return rc;
     });
 }
 
@@ -266,9 +275,7 @@ extern "C" int t2sx_pool_release(t2sx_pool* p, int32_t n, const int32_t* seqs) {
     if (!distinct(p, n, seqs)) return bad("t2sx_pool_release: sequence ids out of range or given twice");
     for (int32_t i = 0; i < n; ++i) {
         if (p->len[seqs[i]]) ++p->version;
-        for (int32_t page : p->table[seqs[i]]) p->drop(page);
-        p->table[seqs[i]].clear();
-        p->len[seqs[i]] = 0;
+        clear(p, seqs[i]);
     }
     return T2SX_OK;
 }
@@ -293,21 +300,27 @@ extern "C" int t2sx_pool_compact(t2sx_pool* p, int32_t* moved, void* stream) {
         p->moves.reserve(n_moves);
         for (int32_t s = 0; s < p->max_seqs; ++s)
             for (size_t j = 0; j < p->table[s].size(); ++j) {
-                int32_t& page = p->table[s][j];
+                const int32_t page = p->table[s][j];
                 if (page < n_live) continue;
                 const int32_t dst = to[page - n_live];
-                if (!p->users[dst]) {   // the first sequence that holds the page moves it
-                    p->users[dst] = p->users[page];
-                    p->moves.push_back(PageMove{page, dst, (int)std::min<int64_t>(kPoolPage, p->len[s] - (int64_t)j * kPoolPage)});
-                }
-                page = dst;
+                if (p->users[dst]) continue;
+                p->users[dst] = p->users[page];   // the first sequence that holds the page moves it
+                p->moves.push_back(PageMove{page, dst, (int)std::min<int64_t>(kPoolPage, p->len[s] - (int64_t)j * kPoolPage)});
             }
+        const int rc = launch_moves(p, p->moves, (cudaStream_t)stream);
+        if (rc != T2SX_OK) {
+            for (const PageMove& m : p->moves) p->users[m.dst] = 0;
+            return rc;
+        }
+        for (std::vector<int32_t>& t : p->table)
+            for (int32_t& page : t)
+                if (page >= n_live) page = to[page - n_live];
         for (const PageMove& m : p->moves) p->users[m.src] = 0;
         std::fill(p->free_bits.begin(), p->free_bits.end(), 0);
         for (int32_t page = n_live; page < p->n_pages; ++page) p->free_bits[page >> 6] |= (uint64_t)1 << (page & 63);
         p->first_free_word = std::min<size_t>(n_live / 64, p->free_bits.size() - 1);
         ++p->version;
         if (moved) *moved = n_moves;
-        return launch_moves(p, p->moves, (cudaStream_t)stream);
+        return T2SX_OK;
     });
 }

@@ -163,3 +163,39 @@ def test_failed_call_leaves_its_device_work_known(host, fake_lib):
         _refused(host, host.ERR_CUDA, lambda: _attend(plan, stream=100 + nth))
         _attend(plan, stream=200 + nth)
         assert fake_lib.fake_recorded(100 + nth) == (nth > 1)
+
+
+def test_failed_copies_change_nothing(host, fake_lib):
+    """fork, copy and compact whose launches fail leave lists, lengths and free pages as they were."""
+    pool = _pool(host, pages=1500, seqs=1210)
+    pool.extend([0, 1], [70, 3])
+    pool.fork([0] * 600, list(range(2, 602)))
+    for op, n, launches in (("fork", 1, 1), ("fork", 600, 2), ("copy", 1, 1), ("copy", 400, 2)):
+        for nth in range(1, launches + 1):
+            before = _state(pool)
+            fake_lib.fake_fail_launch(nth)
+            _refused(host, host.ERR_CUDA, lambda: getattr(pool, op)([0] * n, list(range(602, 602 + n))))
+            assert _state(pool) == before
+    before = _state(pool)
+    pool.fork([0] * 600, list(range(602, 1202)))
+    assert pool.available() == before[0] - 600
+    pool.release(list(range(602, 1202)))
+    assert _state(pool) == before
+
+    pool = _pool(host, pages=2500, seqs=2400)
+    pool.extend(list(range(2399)), [1] * 2399)
+    pool.extend([2399], [130])
+    pool.release(list(range(1200)))
+    pool.fork([2399], [0])   # pages of two users move, too
+    before = _state(pool)
+    for nth in (1, 2, 3):
+        fake_lib.fake_fail_launch(nth)
+        _refused(host, host.ERR_CUDA, lambda: pool.compact())
+        assert _state(pool) == before
+    held = len({p for t in before[2] for row in t for p in row})
+    assert pool.compact() == sum(p >= held for p in {p for t in before[2] for row in t for p in row})
+    after = _state(pool)
+    assert after[:2] == before[:2] and {p for t in after[2] for row in t for p in row} == set(range(held))
+    assert after[2][0][0][:2] == after[2][2399][0][:2]
+    pool.extend([1], [1])
+    assert pool.table([1])[0].tolist() == [held]
