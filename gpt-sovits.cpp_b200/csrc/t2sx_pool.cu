@@ -200,7 +200,9 @@ extern "C" int t2sx_pool_create(int32_t device, int32_t type, int32_t n_layers, 
 extern "C" void t2sx_pool_free(t2sx_pool* p) {
     if (!p || p->closed) return;
     p->closed = true;
-    if (p->n_plans == 0) t2sx_pool_release_object(p);
+    if (p->n_plans == 0) return t2sx_pool_release_object(p);
+    DeviceGuard dg;   // the object stays for its plans, the caller's storage need not
+    if (dg.set(p->device) == cudaSuccess) p->settle();
 }
 
 extern "C" int t2sx_pool_available(t2sx_pool* p, int32_t* n_pages) {

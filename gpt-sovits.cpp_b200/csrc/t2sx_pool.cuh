@@ -76,7 +76,9 @@ struct t2sx_pool {
     cudaError_t settle() {
         if (!worked) return cudaSuccess;
         cudaError_t e = cudaEventRecord(done, last);
-        return e == cudaSuccess ? cudaEventSynchronize(done) : e;
+        if (e == cudaSuccess) e = cudaEventSynchronize(done);
+        if (e == cudaSuccess) worked = false;   // nothing to wait for: `last` is not looked at any more
+        return e;
     }
 };
 

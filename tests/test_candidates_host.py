@@ -199,3 +199,20 @@ def test_failed_copies_change_nothing(host, fake_lib):
     assert after[2][0][0][:2] == after[2][2399][0][:2]
     pool.extend([1], [1])
     assert pool.table([1])[0].tolist() == [held]
+
+
+def test_free_waits(host, fake_lib):
+    """The pool's end waits for its device work, also where plans still hold the pool: the caller may free the
+    storage then."""
+    for plans in (0, 1):
+        pool = _pool(host, pages=8, seqs=4)
+        pool.extend([0], [70])
+        if plans:
+            plan = _plan(pool, 1)
+        pool.fork([0], [1], 5)
+        fake_lib.fake_reset()
+        pool.close()
+        assert fake_lib.fake_synced() == 1 and fake_lib.fake_recorded(5) == 1
+    _refused(host, host.ERR_INVALID, lambda: plan.update([], []))
+    plan.close()   # the stream may be gone by now
+    assert fake_lib.fake_recorded(5) == 1
