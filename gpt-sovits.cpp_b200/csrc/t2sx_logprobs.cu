@@ -314,9 +314,11 @@ k_logprobs(const T* __restrict__ logits, Args a) {
     const float xt = given ? to_f32(x[t]) : INFINITY, xt_below = Vec<T>::below(xt);
     unsigned short* slots = reinterpret_cast<unsigned short*>(raw + ROWS * sizeof(Shared<WARPS>));
     int n_slots = 0;
-    // the edge's element is the first one of the thread: 1 for its weight, NaN for NaN and +inf
+    // The edge's element is the first one of the thread, its weight against the rounded reference like all others' (below): the
+    // reference's rounding, up to half a unit of it, is taken out of their sum at the end.
     float m = fmaxf(edge_x, -INFINITY), ref = reference(m), slot = -INFINITY;
-    float2 s = {edge_x == -INFINITY ? 0.0f : edge_x - edge_x + 1.0f, 0.0f}, w = {0.0f, 0.0f};
+    const float edge_y = max_nan(fmaf(edge_x, kLog2e, -ref), -1e30f), edge_e = ex2(edge_y);
+    float2 s = {edge_e, 0.0f}, w = {edge_e * edge_y, 0.0f};
     int before = edge < a.vocab && (edge_x > xt || (edge_x == xt && edge < t));
     for (int base = v0, group = 0; base < v1; base += kGroup * N) {
         uint4 c[kGroup];

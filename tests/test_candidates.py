@@ -670,3 +670,21 @@ def test_candidates_together(t2sx_mod):
             assert 1 <= len(drawn) <= 9 and (len(drawn) == 9 or drawn[-1] == candidates.EOS)
             lp = scores(prompt + drawn)[len(prompt) - 1:-1].gather(1, torch.tensor(drawn)[:, None])
             assert abs(mean - lp.mean().item()) <= 2.0 ** -8, (mean, lp)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [0, 1, 30])
+@pytest.mark.parametrize("level", [0.0, 100.0, -1000.0, 10000.0, 50000.0])
+@pytest.mark.parametrize("vocab,pad", [(3, 0), (5, 2), (9, 0), (41, 0), (300, 1), (1025, 0)])
+def test_logprobs_level(t2sx_mod, dtype, level, vocab, pad):
+    """Rows at every alignment whose logits stand far from zero: what counts is their differences, also for the
+    elements before and after a row's whole vectors, which are the likely tokens here."""
+    _need_gpu()
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    rows = 16
+    x = torch.randn((rows, vocab + pad), generator=gen, device="cuda") * 2
+    for e in (0, 1, 2, -3, -2, -1):
+        x[:, :vocab][:, max(e, -vocab) if e < 0 else min(e, vocab - 1)] += 4
+    x = (x + level).to(TORCH[dtype])[:, :vocab]
+    tokens = torch.arange(rows, device="cuda", dtype=torch.int32) % vocab
+    _check_scores(t2sx_mod, x, tokens, min(5, vocab))
