@@ -671,6 +671,86 @@ def test_candidates_together(t2sx_mod):
             lp = scores(prompt + drawn)[len(prompt) - 1:-1].gather(1, torch.tensor(drawn)[:, None])
             assert abs(mean - lp.mean().item()) <= 2.0 ** -8, (mean, lp)
 
+# ---- layers, peaks, alignments -----------------------------------------------------------------------------
+
+def _forget(c, layer, seq, count):
+    """Zeros in place of the sequence's last positions in one layer: a call that writes them has to."""
+    t = torch.as_tensor(c.pool.table([seq])[0], device="cuda").long()
+    n = c.pool.length(seq)
+    pos = torch.arange(n - count, n, device="cuda")
+    for x in (c.k, c.v):
+        x[layer, t[pos // PAGE], :, pos % PAGE] = 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype,heads,kv,dim", SHAPES)
+def test_attend_layers(t2sx_mod, dtype, heads, kv, dim):
+    """Layers above the first in every form of the attention: many rows over shared pages (the tcgen05 kernel, warp tiles
+    and joins), chunks (rows written by a launch of their own), one long sequence in parts.  Rows go to
+    the call's layer and nowhere else."""
+    _need_gpu()
+    rng = np.random.default_rng(heads + dim)
+    c = Cache(t2sx_mod, dtype, 3, 700, kv, dim, 150)
+    c.extend(0, 1000)
+    c.extend(1, 130)
+    cand = list(range(2, 122))
+    c.derive("fork", [i % 2 for i in cand], cand)
+    for s in cand:
+        c.extend(s, int(rng.integers(1, 150)))
+    c.extend(130, 500)
+    c.extend(131, 9000)
+    for layer in (2, 1):
+        _attend(c, dtype, layer, cand, [1] * len(cand), heads)
+        for seqs, new in ((cand, [1] * len(cand)), ([130, 5], [333, 1]), ([131], [1])):
+            for s, n in zip(seqs, new):
+                _forget(c, layer, s, n)
+            _attend(c, dtype, layer, seqs, new, heads, write=True)
+            c.check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [1, 30])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("rows", [100, 200])
+@pytest.mark.parametrize("step", [2.5, 8.0])
+def test_attend_rising_and_falling(t2sx_mod, dtype, dim, rows, step):
+    """Scores whose level rises by `step` from page to page, eight times, and falls again, over and over: the maximum that weights
+    refer to moves several times inside an item, at once or after weights have grown.  One and two tiles of rows of
+    the tcgen05 kernel.  Scores stay below 2^6, which the tolerance needs."""
+    _need_gpu()
+    heads, kv = 8, 2
+    each = rows // (heads // kv)
+    c = Cache(t2sx_mod, dtype, 1, 60 + 2 * each, kv, dim, 1 + each)
+    gen = torch.Generator(device="cuda").manual_seed(dim + rows)
+    length = 60 * PAGE
+    c.extend(0, length)
+    page = torch.arange(length, device="cuda") // PAGE % 16
+    level = step * torch.minimum(page, 16 - page)            # 0 .. 8 and down
+    level = level * min(1.0, 56.0 / float(level.max()))
+    sign = torch.randint(0, 2, (dim,), generator=gen, device="cuda") * 2.0 - 1.0
+    noise = torch.randn(c.want[0][0].shape, generator=gen, device="cuda") * 0.3
+    c.want[0][0] = (level[None, :, None, None] / math.sqrt(dim) * sign + noise).to(TORCH[dtype])
+    t = torch.as_tensor(c.pool.table([0])[0], device="cuda").long()
+    pos = torch.arange(length, device="cuda")
+    c.k[:, t[pos // PAGE], :, pos % PAGE] = c.want[0][0].movedim(1, 0)
+    seqs = list(range(1, 1 + each))
+    c.derive("fork", [0] * each, seqs)
+    for s in seqs:
+        c.extend(s, 1 + s % 70)
+    q = (sign + torch.randn((each, heads, dim), generator=gen, device="cuda") * 0.05).to(TORCH[dtype])
+    out = torch.full_like(q, 7.0)
+    lse = torch.full((each, heads), 7.0, device="cuda")
+    scale = 1.0 / math.sqrt(dim)
+    plan = c.pool.plan(heads)
+    plan.update(seqs, [1] * each, _stream())
+    plan.attend(0, q.data_ptr(), out.data_ptr(), scale, lse_ptr=lse.data_ptr(), stream=_stream())
+    ref, mag, zref = _reference(c, 0, seqs, [1] * each, q, heads, scale)
+    assert 8 < float(zref.min()) and float(zref.max()) < 70
+    err = (out.double() - ref).abs() - (UNIT[dtype] * (mag + ref.abs()) + 2.0 ** -14 * mag + 2.0 ** -24)
+    assert (err <= 0).all(), (float((out.double() - ref).abs().max()), int((err > 0).sum()))
+    assert ((lse.double() - zref).abs() <= 2.0 ** -14 * (1 + zref.abs())).all()
+    plan.sync()
+
 
 @gpu
 @pytest.mark.parametrize("dtype", [0, 1, 30])
