@@ -333,7 +333,8 @@ T2SX_API int t2sx_plan_sync(t2sx_plan* a);
  * run out of tokens are filled up with -1 and -inf.  A row of -inf only: logprob -inf, entropy 0.
  * A row with NaN or +inf: logprob, entropy and top_logprobs NaN; NaN is not listed.  Token -1 (none,
  * padding): logprob 0, rank -1; any other id outside [0, vocab): logprob NaN, rank -1.
- * The sums are f32, the result is the same for the same row wherever it stands in a call. */
+ * The sums are f32; equal rows of a call give the same bits where their addresses are the same modulo 16 (with
+ * dense rows of odd width or another stride they need not be: the sums' order follows the address). */
 T2SX_API int t2sx_token_logprobs(int32_t device, int32_t type, int64_t rows, int64_t vocab, const void* logits_dev,
                                  int64_t stride, const int32_t* tokens_dev, int32_t top_k, float* logprob_dev,
                                  float* entropy_dev, int32_t* rank_dev, int32_t* top_ids_dev, float* top_logprobs_dev,

@@ -671,6 +671,7 @@ def test_candidates_together(t2sx_mod):
             lp = scores(prompt + drawn)[len(prompt) - 1:-1].gather(1, torch.tensor(drawn)[:, None])
             assert abs(mean - lp.mean().item()) <= 2.0 ** -8, (mean, lp)
 
+
 # ---- layers, peaks, alignments -----------------------------------------------------------------------------
 
 def _forget(c, layer, seq, count):
@@ -768,3 +769,23 @@ def test_logprobs_level(t2sx_mod, dtype, level, vocab, pad):
     x = (x + level).to(TORCH[dtype])[:, :vocab]
     tokens = torch.arange(rows, device="cuda", dtype=torch.int32) % vocab
     _check_scores(t2sx_mod, x, tokens, min(5, vocab))
+
+
+@gpu
+@pytest.mark.parametrize("dtype,rows,vocab", [(0, 700, 1025), (0, 3000, 333), (1, 40, 5001), (30, 12, 100003), (30, 2000, 1023)])
+def test_logprobs_equal_rows(t2sx_mod, dtype, rows, vocab):
+    """The same row again and again in a call: the same bits where its address is the same modulo 16, and the same within
+    the sums' error (twice 2^-17 of the span) where it is not."""
+    _need_gpu()
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    one = (torch.randn(vocab, generator=gen, device="cuda") * 2.5).to(TORCH[dtype])
+    x = one.repeat(rows, 1)
+    tokens = torch.full((rows,), vocab // 3, dtype=torch.int32, device="cuda")
+    got = _scores(t2sx_mod, x, tokens, 9)
+    span = float((one.max() - one.min()).double())
+    place = [r * vocab * x.element_size() % 16 for r in range(rows)]
+    first = [place.index(p) for p in place]
+    assert len(set(first)) > 3
+    for a in got:
+        assert torch.equal(a.view(torch.int32), a[first].view(torch.int32))
+        assert ((a.double() - a[:1].double()).abs() <= (2.0 ** -16 * span if a.dtype == torch.float32 else 0)).all()
