@@ -564,6 +564,7 @@ struct t2sx_plan {
     // scratch of an update
     std::vector<int32_t> order, next_order, group_of, count, group_page, node_rows, pages;
     std::vector<int32_t> stamp, stamp_group, row0;
+    int32_t round = 0;             // splits of all updates
     std::vector<Token> info, tokens, joins;   // the step's rows; nodes' tokens; those of several parts
     std::vector<Node> nodes;
     std::vector<Item> items;
@@ -620,12 +621,7 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
     a->order.clear();
     for (int32_t i = 0; i < n; ++i)
         if (n_new[i] > 0) a->order.push_back(i);
-    if (a->stamp.size() < (size_t)p->n_pages) { a->stamp.assign(p->n_pages, -1); a->stamp_group.assign(p->n_pages, 0); }
     struct Set { int32_t lo, hi, depth; };   // a range of `order`, and the pages above it
-    std::vector<Set> todo;
-    if (!a->order.empty()) todo.push_back({0, (int32_t)a->order.size(), 0});
-    int32_t round = 0;
-    std::fill(a->stamp.begin(), a->stamp.end(), -1);
     auto emit = [&](const Set& s, int32_t to) {
         Node nd;
         nd.tokens_at = (int32_t)a->node_rows.size();
@@ -651,6 +647,15 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
         for (int32_t j = 0; j < (int32_t)a->order.size(); ++j) emit({j, j + 1, 0}, (int32_t)p->table[seqs[a->order[j]]].size());
         return;
     }
+    // A page's stamp says in which split it was seen last.  Splits (no more of them than sequences) are numbered on from
+    // update to update, so that an update costs what its sequences have, not what the pool has.
+    if (a->stamp.empty() || a->round > INT32_MAX / 2) {
+        a->stamp_group.resize(p->n_pages);
+        a->stamp.assign(p->n_pages, -1);
+        a->round = 0;
+    }
+    std::vector<Set> todo;
+    if (!a->order.empty()) todo.push_back({0, (int32_t)a->order.size(), 0});
     while (!todo.empty()) {
         const Set s = todo.back();
         todo.pop_back();
@@ -669,7 +674,7 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
         }
         if (common > s.depth) emit(s, common);
         // split by the next page
-        const int32_t here = round++;
+        const int32_t here = a->round++;
         a->count.clear();
         a->group_of.assign(s.hi - s.lo, -1);
         for (int32_t j = s.lo; j < s.hi; ++j) {

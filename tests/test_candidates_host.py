@@ -216,3 +216,27 @@ def test_free_waits(host, fake_lib):
     _refused(host, host.ERR_INVALID, lambda: plan.update([], []))
     plan.close()   # the stream may be gone by now
     assert fake_lib.fake_recorded(5) == 1
+
+
+@pytest.mark.parametrize("n", [4, 60])
+def test_update_time_does_not_follow_the_pool(host, n):
+    """A step's plan costs what the step's sequences cost, however many pages the pool has (its first update may
+    prepare something for each of them)."""
+    import time
+
+    def best(pages):
+        pool = _pool(host, pages=pages, seqs=n + 1, kv=16)
+        pool.extend([0], [640])
+        seqs = list(range(1, n + 1))
+        pool.fork([0] * n, seqs)
+        pool.extend(seqs, [1] * n)
+        plan = _plan(pool, 16)
+        took = []
+        for _ in range(40):
+            t0 = time.perf_counter()
+            plan.update(seqs, [1] * n)
+            took.append(time.perf_counter() - t0)
+        return min(took)
+
+    small, large = best(4096), best(1 << 24)
+    assert large < 8 * small + 100e-6, (small, large)
