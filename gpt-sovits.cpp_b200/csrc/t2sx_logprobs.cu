@@ -596,7 +596,7 @@ cudaError_t launch(const T* x, Args a, int split, cudaStream_t st) {
         cudaFuncSetAttribute(k_logprobs<T, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (32 << 10) + ROWS * (int)sizeof(Shared<WARPS>));
     });
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((a.rows + ROWS - 1) / ROWS), split);
+    cfg.gridDim = dim3((unsigned)(((long long)a.rows + ROWS - 1) / ROWS), split);
     cfg.blockDim = WARPS == 1 ? 128 : N;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;

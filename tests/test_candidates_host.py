@@ -240,3 +240,11 @@ def test_update_time_does_not_follow_the_pool(host, n):
 
     small, large = best(4096), best(1 << 24)
     assert large < 8 * small + 100e-6, (small, large)
+
+
+@pytest.mark.parametrize("vocab,rows_of_a_cta", [(1, 4), (1025, 4), (5000, 1)])
+@pytest.mark.parametrize("rows", [2000, 2001, 2 ** 31 - 1, 2 ** 31 - 2])
+def test_logprobs_grid(host, fake_lib, vocab, rows_of_a_cta, rows):
+    """As many blocks as the rows need, up to the greatest number of rows."""
+    host.token_logprobs(host.F32, rows, vocab, Q, Q, Q)
+    assert fake_lib.fake_grid_x() == -(-rows // rows_of_a_cta)
