@@ -36,6 +36,7 @@ constexpr int kTcMinChunk = 4;       // pages of a split of such a node at least
 constexpr int kFoldParts = 4;        // parts of a token up to which the item of its own pages folds them in, one after the other:
                                      // 2048 sequences, 32 to a prompt, take 340 us so and 351 with a launch that joins them; with up
                                      // to eight parts 256 sequences of one long prompt took 117 when they took 107 so
+constexpr int64_t kMaxNodeTokens = 1 << 28;   // of all nodes together: 8 GB of tokens, whose places are 32-bit numbers
 constexpr int kSmallWork = 2048;     // pages x head dim of a CTA of a small step at most, an eighth of it with two CTAs to an SM
 
 __device__ __forceinline__ void mma16816(__half, float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -614,8 +615,8 @@ extern "C" void t2sx_plan_free(t2sx_plan* a) {
 }
 
 // The trie of the sequences' page lists: every entry of a list is looked at once or twice.  Sequences are
-// split by the page that follows their common run, keeping their order.
-static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int32_t* n_new) {
+// split by the page that follows their common run, keeping their order.  False: the nodes have too many tokens.
+static bool build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int32_t* n_new) {
     t2sx_pool* p = a->pool;
     a->nodes.clear(); a->node_rows.clear(); a->pages.clear();
     a->order.clear();
@@ -625,6 +626,9 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
     auto emit = [&](const Set& s, int32_t to) {
         Node nd;
         nd.tokens_at = (int32_t)a->node_rows.size();
+        int64_t tokens = nd.tokens_at;
+        for (int32_t j = s.lo; j < s.hi; ++j) tokens += n_new[a->order[j]];
+        if (tokens > kMaxNodeTokens) return false;
         for (int32_t j = s.lo; j < s.hi; ++j) {
             const int32_t i = a->order[j];
             for (int32_t k = 0; k < n_new[i]; ++k) a->node_rows.push_back(a->row0[i] + k);
@@ -642,10 +646,12 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
         nd.new_pos = s.hi - s.lo > 1 ? INT32_MAX : (int32_t)(p->len[seqs[i0]] - n_new[i0]);
         nd.new_row = a->row0[i0];
         a->nodes.push_back(nd);
+        return true;
     };
     if (a->small) {   // nothing is shared: one node for each sequence
-        for (int32_t j = 0; j < (int32_t)a->order.size(); ++j) emit({j, j + 1, 0}, (int32_t)p->table[seqs[a->order[j]]].size());
-        return;
+        for (int32_t j = 0; j < (int32_t)a->order.size(); ++j)
+            if (!emit({j, j + 1, 0}, (int32_t)p->table[seqs[a->order[j]]].size())) return false;
+        return true;
     }
     // A page's stamp says in which split it was seen last.  Splits (no more of them than sequences) are numbered on from
     // update to update, so that an update costs what its sequences have, not what the pool has.
@@ -661,7 +667,7 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
         todo.pop_back();
         const std::vector<int32_t>& t = p->table[seqs[a->order[s.lo]]];
         if (s.hi - s.lo == 1) {
-            if ((size_t)s.depth < t.size()) emit(s, (int32_t)t.size());
+            if ((size_t)s.depth < t.size() && !emit(s, (int32_t)t.size())) return false;
             continue;
         }
         int32_t common = (int32_t)t.size();
@@ -672,7 +678,7 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
             while (k < most && o[k] == t[k]) ++k;
             common = k;
         }
-        if (common > s.depth) emit(s, common);
+        if (common > s.depth && !emit(s, common)) return false;
         // split by the next page
         const int32_t here = a->round++;
         a->count.clear();
@@ -699,6 +705,7 @@ static void build_nodes(t2sx_plan* a, int32_t n, const int32_t* seqs, const int3
         for (size_t g = a->count.size(); g-- > 0;)
             todo.push_back({s.lo + a->group_page[g], s.lo + a->count[g], common});
     }
+    return true;
 }
 
 // The kernels of the nodes, by cost.  In pages of the tcgen05 kernel's two tiles, an SM's time: such a CTA costs its start and end and
@@ -892,7 +899,7 @@ extern "C" int t2sx_plan_update(t2sx_plan* a, int32_t n, const int32_t* seqs, co
         }
         const int64_t ctas = row_tiles * p->n_kv;
         a->small = ctas <= 2 * a->n_sm && longest * p->dim <= (ctas <= a->n_sm ? kSmallWork : kSmallWork / 8);
-        build_nodes(a, n, seqs, n_new);
+        if (!build_nodes(a, n, seqs, n_new)) return bad("t2sx_plan_update: too many rows over shared pages");
         const int64_t n_parts = build_items(a);
         if (n_parts >= INT32_MAX || a->items.size() * p->n_kv > (size_t)INT32_MAX ||
             a->joins.size() * (size_t)a->n_heads > (size_t)INT32_MAX)

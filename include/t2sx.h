@@ -301,7 +301,8 @@ typedef struct t2sx_plan t2sx_plan;
 T2SX_API int t2sx_plan_create(t2sx_pool* p, int32_t n_heads, t2sx_plan** out);
 T2SX_API void t2sx_plan_free(t2sx_plan* a);
 /* The step's sequences (distinct) and their last n_new[i] (>= 0, <= length) positions: rows are
- * these positions in the order of the call.  Pages that sequences have in common from their
+ * these positions in the order of the call, at most 2^24 (and 2^28 counted anew in each run of pages
+ * that a set of sequences has in common).  Pages that sequences have in common from their
  * start on are found here, whatever the order.  The pool's later fork, copy and extend calls
  * leave a plan valid (but what a fork has made a shared page is no longer written, see below); after
  * a release or a compact that moved pages attend gives T2SX_ERR_STATE until the next update. */

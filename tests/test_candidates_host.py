@@ -248,3 +248,22 @@ def test_logprobs_grid(host, fake_lib, vocab, rows_of_a_cta, rows):
     """As many blocks as the rows need, up to the greatest number of rows."""
     host.token_logprobs(host.F32, rows, vocab, Q, Q, Q)
     assert fake_lib.fake_grid_x() == -(-rows // rows_of_a_cta)
+
+
+def test_update_refuses_what_its_lists_cannot_hold(host):
+    """A chunk of 2^24 rows over pages that 17 sequences leave one after the other: each shared run lists the rows anew."""
+    pages, forks = 1 << 18, 17
+    pool = _pool(host, pages=pages + 2 * forks, seqs=forks + 1)
+    others = list(range(1, forks + 1))
+    for s in others:
+        pool.extend([0], [64])
+        pool.fork([0], [s])
+    pool.extend([0], [(1 << 24) - 64 * forks])
+    pool.extend(others, [1] * forks)
+    plan = _plan(pool, 1)
+    plan.update(others, [1] * forks)
+    rows = (1 << 24) - forks
+    _refused(host, host.ERR_INVALID, lambda: plan.update([0] + others, [rows] + [1] * forks))
+    _refused(host, host.ERR_STATE, lambda: _attend(plan))
+    plan.update([0] + others, [1] * (forks + 1))
+    _attend(plan)
