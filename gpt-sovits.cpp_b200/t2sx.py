@@ -446,7 +446,12 @@ def _ids(a, kind="i"):
     if isinstance(a, (list, tuple)):
         a = array(kind, a)
         return a.buffer_info()[0], len(a), a
-    a = np.ascontiguousarray(np.atleast_1d(a), dtype=np.int32 if kind == "i" else np.int64)
+    given = np.atleast_1d(a)
+    if given.size and given.dtype.kind not in "iu":
+        raise TypeError("integers are needed")
+    a = np.ascontiguousarray(given, dtype=np.int32 if kind == "i" else np.int64)
+    if a.dtype != given.dtype and not np.array_equal(a, given):
+        raise OverflowError(f"an integer does not fit {a.dtype}")
     return a.__array_interface__["data"][0], a.size, a
 
 

@@ -267,3 +267,23 @@ def test_update_refuses_what_its_lists_cannot_hold(host):
     _refused(host, host.ERR_STATE, lambda: _attend(plan))
     plan.update([0] + others, [1] * (forks + 1))
     _attend(plan)
+
+
+def test_ids_that_do_not_fit(host):
+    """Arrays of ids are taken for what they hold, as lists are: what is no 32-bit integer (a count: 64-bit) is not cut down to one."""
+    import numpy as np
+    pool = _pool(host, pages=8, seqs=4)
+    for ids in ([2 ** 32], np.array([2 ** 32]), np.array([2 ** 32 + 1], dtype=np.uint64), np.array([-2 ** 32])):
+        with pytest.raises(OverflowError):
+            pool.extend(ids, [1])
+    for ids in ([0.5], np.array([0.5]), np.array([1.0])):
+        with pytest.raises(TypeError):
+            pool.extend(ids, [1])
+    with pytest.raises(OverflowError):
+        pool.extend([0], np.array([2 ** 64 - 1], dtype=np.uint64))
+    assert [pool.length(s) for s in range(4)] == [0, 0, 0, 0]
+    for ids in ([0, 3], (0, 3), np.array([0, 3]), np.array([0, 9, 3], dtype=np.uint8)[::2], range(0, 4, 3), np.array([[0], [3]], dtype=np.int32)):
+        pool.extend(ids, np.array([1, 2]))
+    pool.extend(np.array([]), [])
+    pool.extend(np.int64(1), 5)
+    assert [pool.length(s) for s in range(4)] == [6, 5, 0, 12]
