@@ -64,8 +64,10 @@ class Decoder:
 
 
 def draw(dec: Decoder, prompts, each: int, steps: int, top_k: int = 15, seed: int = 0):
-    """Draws `each` continuations of every prompt (lists of token ids), `steps` tokens at most.  Returns, for
+    """Draws `each` continuations of every prompt (lists of one token id or more), `steps` tokens at most.  Returns, for
     each prompt, those kept as (mean log probability, tokens), the best first."""
+    if any(len(p) == 0 for p in prompts):
+        raise ValueError("a prompt needs a token to continue")
     dev, PAGE = torch.device("cuda", dec.device), t2sx.PagePool.PAGE
     stream = torch.cuda.current_stream().cuda_stream
     gen = torch.Generator(device=dev).manual_seed(seed)

@@ -287,3 +287,14 @@ def test_ids_that_do_not_fit(host):
     pool.extend(np.array([]), [])
     pool.extend(np.int64(1), 5)
     assert [pool.length(s) for s in range(4)] == [6, 5, 0, 12]
+
+
+def test_draw_refuses_an_empty_prompt(host, fake_lib):
+    """A prompt without tokens has no last row to draw from; it is refused before any work."""
+    import types
+    import candidates
+    dec = types.SimpleNamespace(device=0, layers=1, vocab=1025, d=512)
+    for prompts in ([[]], [[1, 2], []]):
+        with pytest.raises(ValueError):
+            candidates.draw(dec, prompts, each=2, steps=3)
+    assert fake_lib.fake_launches() == 0
