@@ -122,6 +122,13 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[N]) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
+// A wait of all threads of a warp, whose next instruction may be one that takes the warp as a whole (.sync.aligned: the loads
+// and stores of TMEM, a named barrier).  Each thread leaves the wait's loop by itself; the warp is brought together again here.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, long long limit) {
+    const bool ok = bar_wait(bar, parity, abort_flag, limit);
+    __syncwarp();
+    return ok;
+}
 // True in one lane of the warp, the leader.  The compiler knows that only one thread passes, and needs no loop around
 // the instructions that take their operands from uniform registers.
 __device__ __forceinline__ bool elect_one(uint32_t& leader) {
@@ -398,7 +405,7 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         if (stall) gone = !bar_wait(stall_bar, 0, abort_flag, spin);
         for (int k = 0; k < nt; ++k) {
             const int b = k & 1, pos = it.pos0 + nth(tile, k) * kKeys;
-            gone |= !bar_wait(s_full(tile, b), (k >> 1) & 1, abort_flag, spin);
+            gone |= !warp_wait(s_full(tile, b), (k >> 1) & 1, abort_flag, spin);
             tc_fence_after();
             uint32_t sc[kKeys];
             tmem_ld32(lanes + b * kKeys, sc);
@@ -425,7 +432,7 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
                 if (grew) m = top;
                 l *= f;
                 if (k > 0) {   // (the scores of k came after the output of page k - 2)
-                    gone |= !bar_wait(o_done(tile), (k - 1) & 1, abort_flag, spin);
+                    gone |= !warp_wait(o_done(tile), (k - 1) & 1, abort_flag, spin);
                     tc_fence_after();
 #pragma unroll
                     for (int c = 0; c < D; c += 32) {
@@ -448,7 +455,7 @@ k_attend_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
             __syncwarp();
         }
         // (not o_done: two of its phases may be outstanding here, which a wait by parity does not tell apart)
-        gone |= !bar_wait(end_bar, 0, abort_flag, spin);
+        gone |= !warp_wait(end_bar, 0, abort_flag, spin);
         gone = __any_sync(~0u, gone);
         tc_fence_after();
         // The output goes through shared memory (the place of Q and the rings), row by row, so that neighbouring lanes write
