@@ -272,10 +272,12 @@ struct Shared {   // of one row's threads in a CTA
 // WARPS == 1: a warp per row, four rows in a CTA.  Else a row per CTA, or (WARPS == 8) per cluster of `split` CTAs:
 // each takes a range of the row's vectors, and the first one joins what they found.
 //
-// Bound by issue and the exponential unit for 16-bit logits: an element is an exponential (16 a cycle and SM) and some eight
-// other instructions, packed ones counted once.  2048 rows of 100003 in bf16 with the 20 best take 85 us, 4.8 TB/s (77 without
-// list and rank); 4 rows of 131072 in f16 10.3 us, of which most is the way from launch to the joined lists; 2048 rows of 1025 in
-// f32 8.2 us.
+// While 16-bit rows are read, issue and the exponential unit bound it: an element is an exponential (16 a cycle and SM) and some eight
+// other instructions, packed ones counted once.  Over the whole of 2048 rows of 100003 in bf16 with the 20 best neither is full, nor
+// is DRAM (63, 61 and 61%): the rows of a wave come to their lists, where nothing is loaded, together.  That takes 85 us, 4.8 TB/s (77
+// without list and rank).  4 rows of 131072 in f16 take 10.3 us, of which most is the way from launch to the joined lists.
+// 2048 rows of 1025 in f32 take 9 us where 8 rows take 6: a row's phases after its loads (the maxima sorted, the slots, their vectors
+// again, places) follow one another.  Times are the device's, of calls one after another with the same logits.
 template <typename T, int WARPS>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS, WARPS == 1 ? 6 : 32 / WARPS)
 k_logprobs(const T* __restrict__ logits, Args a) {

@@ -31,7 +31,7 @@ struct MoveList {
 };
 
 // One CTA per (fan, layer, K or V, 8 heads); a head's filled positions are contiguous in its page.  Bound by
-// the bytes written: a fork's partial page is read once for up to eight copies.  512 copies of 32 pages of 24 layers
+// the bytes written: a fork's partial page is read once for up to eight copies.  Calls one after another, 512 copies of 32 pages of 24 layers
 // (16 heads of 32 dims) take 138 us, 5.5 TB/s; with a read through the L2 cache for each copy they took 306.  Rewriting
 // 32 of 64 sequences and compacting, 3.65 GB in and out, takes 557 us (6.5 TB/s).
 template <int N>

@@ -6,7 +6,15 @@
 //     m = max_j s_j,  l = sum_j 2^(s_j - m + c),  O = sum_j 2^(s_j - m + c) v_j,   s_j = scale log2(e) q . k_j
 // and a token's result follows from its parts: M = max m_i, out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i.
 // The constant c keeps small weights above the subnormal numbers of f16 (and is harmless for bf16).
+// Scores, m, l, O and the joins are f32.  The weights alone are rounded to the cache's 16-bit type, in which the tensor cores take
+// them to the product with v, so an output carries two such roundings, theirs and its own: 2.3e-4 to 2.9e-4 of its
+// length from the 64-bit result in f16 and 1.9e-3 to 2.3e-3 in bf16, where its own rounding alone makes 2.1e-4 and
+// 1.7e-3.  Weights as the sum of two 16-bit parts would take the first one away and double the products with v, a
+// third more tensor work at head dim 128.
 // A row is a (token, query head of the K/V head's group); `group` heads of a token are neighbours.
+//
+// Times in this file's comments are the device's, of calls one after another with the same tensors (what fits stays in L2), where they
+// do not say otherwise; the two sides of a rule were measured alike.
 #include "t2sx_prefix_attn.cuh"
 
 #include <algorithm>
@@ -116,7 +124,8 @@ __device__ __forceinline__ uint32_t tile_at(int row, int c) {
 // results in shared memory.
 //
 // Bound by the cache's bytes where a page has few rows: 2048 sequences, 32 to a prompt, 16 heads of 32 dims, some
-// 500 positions each of their own, take 340 us for 2.2 GB (6.4 TB/s); one sequence of 65536 positions, 8 heads of 128, 53 us.
+// 500 positions each of their own, take 340 us for 2.2 GB (6.4 TB/s); one sequence of 65536 positions, 8 heads of 128, 43 us
+// and 10 for the join, which run into one another (53 a call).
 // Warps alone (no CTA-wide barrier in the loop) because items differ in length; mma.sync because a page of a few
 // rows is a memory-bound product, whatever the tensor cores' rate.  A small step runs the W > 1 form as its only
 // launch: 6.9 us for four candidates of one prompt.

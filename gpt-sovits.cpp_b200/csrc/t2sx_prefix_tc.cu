@@ -5,8 +5,8 @@
 // page's K and V serve both; a smaller one is in both, with every second page, and the two results are joined
 // at the end.
 //   warps 0-7  the softmax, one row per thread: scores from TMEM, weights back to TMEM in 16 bits, their sum.
-//              The maximum that the weights refer to is looked for, and the output rescaled, only when a
-//              tile's weights add up to 2^15 (f16 ends at 2^16);
+//              (the sum is of the weights before that rounding, in f32).  The maximum that the weights refer to
+//              is looked for, and the output rescaled, only when a tile's weights add up to 2^15 (f16 ends at 2^16);
 //   warp 8     TMA: the K and V tiles of the pages, in two rings;
 //   warps 9-10 the MMAs, one thread for each tile: S = Q K^T (M 128, N 64) into one of two score buffers of a
 //              tile, then O += P V with P from TMEM (M 128, N head dim).  S is issued two pages ahead, so that the
@@ -15,10 +15,11 @@
 //
 // What bounds it: the tensor cores.  An MMA of M 128 and N 64 takes as long as one of N 128 (64 cycles for 16 of
 // the K index), so a page costs the two tiles 2 x (8 x 64 + 4 x 64) = 1536 cycles at head dim 128, and the loop takes
-// 1526.  At head dim 64 the MMAs take 1024, the exponentials (8 cycles to a warp's instruction) 1066, and the loop
-// 1555.  A step of 256 sequences over one prompt of 16384 positions (32 heads, 8 K/V heads of 128 dims, bf16; up to 256
-// positions each of their own) takes 94 us with all its launches, some 70 of them here: 60 in the loop, 10 in a CTA's start
-// and end.  When it took 116, it took with
+// 1526.  At head dim 64 the MMAs take 1024 and the exponentials (8 cycles to a warp's instruction) 1066, but the loop
+// 1555: a third of it is one waiting for the other.  A step of 256 sequences over one prompt of 16384 positions (32 heads, 8 K/V heads
+// of 128 dims, bf16; up to 256 positions each of their own) takes 103 us a call, calls one after another.  By itself, from cold caches,
+// this kernel takes 79 of it: 64 pages are 58 at the 1.67 GHz that it runs at, a CTA's start and end most of the rest.
+// When the call took 116, it took with
 //   scores of 128 keys in one buffer (N 128): 135, and 128 with 16 softmax warps, since the MMAs then wait for the
 //              softmax; there is no TMEM for a second buffer of that size beside two outputs;
 //   one tile per CTA, two CTAs per SM: 153;    16 softmax warps on these buffers: 117;
